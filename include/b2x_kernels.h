@@ -159,6 +159,70 @@ B2X_API int b2x_launch_wide_reduce(const void* in, uint8_t elem, int64_t A, int6
  * row-major [batch, M, N] result of element type `out_elem`. */
 B2X_API int b2x_launch_wide_gemm(const B2xGemmArgs* host_args, uint8_t out_elem, void* out, b2x_stream_t stream);
 
+/* ---- operators that a program names through stablehlo.custom_call -------------------------------------------------------
+ * A tensor of heads has a contiguous last dimension and is addressed by the element strides of its batch, head and token. */
+typedef struct { int64_t batch, head, token; } B2xHeadStrides;
+
+/* Rotary positions, with the norm of each head in the same pass.  A token at position p turns the pair i of its head's first R
+ * elements (elements i and i + R/2, or 2i and 2i + 1 when `interleaved`) by the angle 2 pi * frac(p * turns[i] / 2^64);
+ * the elements behind R pass.  With `norm` a head is first divided by the root of its mean square (plus epsilon) and
+ * multiplied by a weight per element.  Arithmetic in f32, one rounding at the end. */
+typedef struct {
+  uint8_t elem;                 /* B2xElem of x, y, dy, dx: EL_BF16, EL_F16 or EL_F32 */
+  uint8_t weight_elem;          /* EL_F32 or `elem` */
+  uint8_t n;                    /* tensors: 1 or 2 (queries and keys) */
+  uint8_t norm, interleaved;
+  int64_t B, S, D, R;           /* D <= 256 */
+  float epsilon;
+  int64_t heads[2];
+  const void* x[2]; B2xHeadStrides xs[2];
+  const void* weight[2];        /* [D] each; with `norm` */
+  const int32_t* positions;     /* [B, S]; NULL: token t is at position t */
+  const uint64_t* turns;        /* [R / 2] */
+  void* y[2]; B2xHeadStrides ys[2];       /* the result, or dx of a gradient */
+  const void* dy[2]; B2xHeadStrides dys[2];  /* gradient only */
+  float* dweight[2];            /* gradient with `norm`: [D] each */
+  void* scratch;                /* gradient with `norm`: b2x_rotary_scratch_bytes */
+} B2xRotaryArgs;
+B2X_API int b2x_launch_rotary(const B2xRotaryArgs* host_args, b2x_stream_t stream);
+/* dx of dy; without `norm` x is not read.  Two launches with `norm`: the weights' gradients are partial sums of CTAs, added in a
+ * fixed order, so that results do not differ from run to run. */
+B2X_API int64_t b2x_rotary_scratch_bytes(const B2xRotaryArgs* host_args);
+B2X_API int b2x_launch_rotary_gradient(const B2xRotaryArgs* host_args, b2x_stream_t stream);
+/* Kernels that one call enqueues. */
+B2X_API int b2x_rotary_launches(const B2xRotaryArgs* host_args, int gradient);
+
+/* Attention with grouped heads, capped scores, a bias by distance and masks:
+ *   score(i, j) = softcap * tanh(scale * q_i k_j / softcap) - slope * |p_i - j|      (softcap 0: scale * q_i k_j)
+ *   j is seen when j < lengths[b], and (causal) j <= p_i or j < prefix[b], and documents[b, p_i] == documents[b, j]
+ *   p_i = query_offset + i, or lengths[b] - Sq + i with `queries_at_end`
+ * A query that sees nothing yields 0, and -inf as its log sum.  Keys and values behind lengths[b] are not read as numbers: whatever
+ * lies there (NaN as well) does not show.  Query head h reads key head h * Hk / Hq. */
+typedef struct {
+  uint8_t elem;                 /* EL_BF16 or EL_F16 */
+  uint8_t causal, queries_at_end;
+  int64_t B, Hq, Hk, Sq, Sk, D; /* D a multiple of 8, at most 128 */
+  float scale, softcap;
+  int64_t query_offset;
+  const void* q; const void* k; const void* v;
+  B2xHeadStrides qs, ks, vs;
+  const float* slopes;          /* [Hq] or NULL */
+  const int32_t* documents;     /* [B, Sk] or NULL */
+  const int32_t* prefix;        /* [B] or NULL */
+  const int32_t* lengths;       /* [B] or NULL */
+  void* o; B2xHeadStrides os;   /* result; operand of a gradient */
+  float* lse;                   /* [B, Hq, Sq] natural log sums; NULL: not wanted (a gradient needs them) */
+  /* gradient only */
+  const void* dout; B2xHeadStrides dos;
+  void* dq; void* dk; void* dv;
+  B2xHeadStrides dqs, dks, dvs;
+  void* scratch;                /* b2x_head_attention_scratch_bytes, 16-byte aligned */
+} B2xHeadAttentionArgs;
+B2X_API int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* host_args, int gradient);
+B2X_API int b2x_head_attention_launches(const B2xHeadAttentionArgs* host_args, int gradient);
+B2X_API int b2x_launch_head_attention(const B2xHeadAttentionArgs* host_args, int32_t* status, b2x_stream_t stream);
+B2X_API int b2x_launch_head_attention_gradient(const B2xHeadAttentionArgs* host_args, int32_t* status, b2x_stream_t stream);
+
 /* Number of kernels launched through this library since load (all entry points); used by bench reporting. */
 B2X_API int64_t b2x_kernel_launch_count(void);
 

@@ -7,6 +7,7 @@
 // its outputs (reference: crates/ryft-pjrt/src/programs.rs:2492-2498).
 #pragma once
 #include <cstdint>
+#include <map>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -56,6 +57,8 @@ enum class OpKind : uint8_t {
   BROADCAST_IN_DIM, TRANSPOSE, RESHAPE,
   // contraction, reduction, collectives
   DOT_GENERAL, REDUCE, ALL_REDUCE, ALL_GATHER,
+  // an operator that the program names (custom_call.h)
+  CUSTOM_CALL,
   // terminator
   RETURN,
 };
@@ -77,6 +80,16 @@ struct Value {
   std::vector<Op*> users;
 };
 
+// A value of a custom_call's backend_config dictionary.
+struct CallAttr {
+  enum Kind { NONE, INT, FLOAT, BOOL, STRING, ARRAY } kind = NONE;
+  int64_t i = 0;
+  double f = 0;
+  bool b = false;
+  std::string s;
+  std::vector<CallAttr> items;
+};
+
 struct Op {
   OpKind kind;
   std::vector<Value*> operands;
@@ -95,6 +108,9 @@ struct Op {
   // constant payload: raw little-endian element bytes; `splat` means one element broadcast to the whole type
   std::vector<uint8_t> const_data;
   bool splat = false;
+  // custom_call
+  std::string call_target;
+  std::map<std::string, CallAttr> call_attrs;
 };
 
 struct Module {

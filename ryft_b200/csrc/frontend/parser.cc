@@ -50,7 +50,7 @@ const OpInfo kOps[] = {
     {"broadcast_in_dim", OpKind::BROADCAST_IN_DIM, 1, false}, {"transpose", OpKind::TRANSPOSE, 1, false},
     {"reshape", OpKind::RESHAPE, 1, false}, {"dot_general", OpKind::DOT_GENERAL, 2, false},
     {"reduce", OpKind::REDUCE, -1, false}, {"all_reduce", OpKind::ALL_REDUCE, -1, false},
-    {"all_gather", OpKind::ALL_GATHER, -1, false}, {"return", OpKind::RETURN, -1, false},
+    {"all_gather", OpKind::ALL_GATHER, -1, false}, {"custom_call", OpKind::CUSTOM_CALL, -1, false}, {"return", OpKind::RETURN, -1, false},
 };
 const OpInfo* find_op(const std::string& short_name) {
   for (auto& o : kOps) if (short_name == o.name) return &o;
@@ -79,6 +79,7 @@ struct Attr {
   bool b = false;
   std::string s;            // STRING, or RAW text of an attribute this reader does not interpret
   std::vector<Attr> items;  // ARRAY
+  std::map<std::string, Attr> entries;  // the dictionary of a backend_config
   // DENSE: flattened literals (text tokens) + whether the literal was a single (splat) scalar + the type
   std::vector<std::string> dense_tokens;
   bool dense_splat = false;
@@ -370,7 +371,11 @@ class Parser {
     do {
       std::string k = read_ident();
       Attr v;
-      if (try_char('=')) v = parse_attr_value();
+      if (try_char('=')) {
+        skip_ws();
+        if (k == "backend_config" && peek() == '{') { v.kind = Attr::RAW; v.entries = parse_attr_dict(); }
+        else v = parse_attr_value();
+      }
       else { v.kind = Attr::BOOL; v.b = true; }  // unit attribute
       d[k] = v;
     } while (try_char(','));
@@ -708,7 +713,33 @@ class Parser {
       else if (k == "channel_handle") op->has_channel = true;
       else if (k == "use_global_device_ids") op->use_global_device_ids = true;
       else if (k == "all_gather_dim") op->iota_dim = a.i;
+      else if (op->kind == OpKind::CUSTOM_CALL) apply_call_prop(op, k, a);
       // precision_config, algorithm, result_accuracy, frontend attributes: accepted and ignored
+    }
+  }
+
+  CallAttr call_attr(const Attr& a) {
+    CallAttr c;
+    switch (a.kind) {
+      case Attr::INT: c.kind = CallAttr::INT; c.i = a.i; break;
+      case Attr::FLOAT: c.kind = CallAttr::FLOAT; c.f = a.f; break;
+      case Attr::BOOL: c.kind = CallAttr::BOOL; c.b = a.b; break;
+      case Attr::STRING: c.kind = CallAttr::STRING; c.s = a.s; break;
+      case Attr::ARRAY: c.kind = CallAttr::ARRAY; for (auto& e : a.items) c.items.push_back(call_attr(e)); break;
+      default: break;   // describe_call asks for the kind that it needs
+    }
+    return c;
+  }
+  // api_version, has_side_effect and the like say nothing that the operators depend on
+  void apply_call_prop(Op* op, const std::string& k, const Attr& a) {
+    if (k == "call_target_name") op->call_target = a.s;
+    else if (k == "backend_config") {
+      if (a.kind == Attr::STRING && a.s.empty()) return;
+      if (a.kind != Attr::RAW) fail(kUnimplemented, "stablehlo.custom_call: backend_config must be a dictionary");
+      for (auto& e : a.entries) op->call_attrs[e.first] = call_attr(e.second);
+    } else if (k == "called_computations" && !a.items.empty()) fail(kUnimplemented, "stablehlo.custom_call: called computations are not supported");
+    else if (k == "operand_layouts" || k == "result_layouts" || k == "output_operand_aliases") {
+      if (a.kind != Attr::ARRAY || !a.items.empty()) fail(kUnimplemented, "stablehlo.custom_call: " + k + " is not supported");
     }
   }
 
@@ -912,6 +943,20 @@ class Parser {
       }
       case OpKind::ALL_REDUCE: case OpKind::ALL_GATHER:
         fail(kUnimplemented, std::string(op_name(oi->kind)) + " is only accepted in MLIR's generic form");
+      case OpKind::CUSTOM_CALL: {
+        // stablehlo.custom_call @target(%a, %b) {backend_config = {...}} : (T, T) -> T
+        expect('@');
+        op->call_target = read_ident();
+        expect('(');
+        if (!try_char(')')) {
+          do { add_operand(op, read_operand()); } while (try_char(','));
+          expect(')');
+        }
+        skip_ws();
+        if (peek() == '{') apply_props(op, parse_attr_dict());
+        parse_same_or_function_type(op);
+        break;
+      }
       default: {
         // unary / binary / ternary elementwise: operands, optional attr-dict, then the type
         skip_ws();

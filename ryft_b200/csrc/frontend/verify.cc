@@ -4,7 +4,7 @@
 #include <algorithm>
 #include <set>
 
-#include "ir.h"
+#include "custom_call.h"
 
 namespace b2x {
 namespace {
@@ -101,6 +101,7 @@ void verify_module(const Module& m) {
         }
         break;
       }
+      case OpKind::CUSTOM_CALL: describe_call(op); break;
       case OpKind::CONVERT:
         need(op, in.size() == 1 && out.size() == 1 && in[0]->type.dims == out[0]->type.dims, "shapes differ");
         break;

@@ -1,0 +1,484 @@
+// Rotary positions of queries and keys, with the norm of each head in the same pass, and the gradient of both.
+//
+//   n = x * r * w,  r = rsqrt(mean(x^2) + epsilon)          (or n = x)
+//   (y_a, y_b) = (n_a cos - n_b sin, n_b cos + n_a sin)      for every pair (a, b) of the first R elements of a head
+// and back:  dn is dy turned the other way;  g = dn * w;  dx = r (g - x r^2 mean(g x));  dw = sum over tokens and heads of dn x r.
+//
+// Bound by HBM: every element is read once and written once (the gradient reads x and dy).  A head lies across L lanes of a warp
+// (the smallest power of two that holds it with two 16-byte pieces per lane: 8 lanes for 128 elements of 16 bits), a pair's two
+// elements always in one lane, so the only exchange is the norm's sum over L lanes.  A warp keeps one token, so that the 2R
+// cosines and sines are computed once, a few per lane, shared through shared memory and then held in registers for all the
+// heads that it walks.
+//
+// Angles: a position times a frequency in f32 is off by whole turns far into a context.  Frequencies are therefore turns per
+// position as fractions of 2^64, computed in extended precision where the program is compiled; the product with the position
+// wraps exactly, and its upper 32 bits are the angle to 2^-32 of a turn at any position.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../../include/b2x_kernels.h"
+#include "common.cuh"
+
+namespace b2x {
+namespace {
+
+constexpr int kRotaryWarps = 8;
+constexpr int kRotaryRows = 2;       // heads of a lane in flight: 64 bytes of loads per thread at 128 elements of 16 bits
+
+struct RotaryParams {
+  const char* x[2];
+  const char* dy[2];
+  char* y[2];
+  B2xHeadStrides xs[2], dys[2], ys[2];
+  const char* weight[2];
+  const int32_t* positions;
+  const uint64_t* turns;
+  float* partial;              // gradient with norms: [tensor][CTA][D]
+  int64_t warps;               // warps with work
+  int32_t tokens, S, D, R;
+  int32_t heads[2], jobs[2];   // a token's heads are cut into jobs of `job_heads`
+  int32_t job_heads, lanes, units;
+  int32_t pair_units;          // half layout: units whose two pieces are partners
+  float epsilon, inv_d, sine;  // sine: 1, or -1 to turn back
+  uint8_t interleaved, norm, weight_f32;
+};
+
+template <int EL> __device__ __forceinline__ float rot_get(const uint32_t* w, int i) {
+  if constexpr (EL == EL_F32) return __uint_as_float(w[i]);
+  else {
+    const uint32_t h = (i & 1) ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+    if constexpr (EL == EL_BF16) return __uint_as_float(h << 16);
+    else return __half2float(__ushort_as_half((unsigned short)h));
+  }
+}
+template <int EL> __device__ __forceinline__ uint32_t rot_pack(float a, float b) {   // two 16-bit elements
+  if constexpr (EL == EL_BF16) { __nv_bfloat162 t = __floats2bfloat162_rn(a, b); return *reinterpret_cast<uint32_t*>(&t); }
+  else { __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&t); }
+}
+
+// V elements at `p` as floats
+template <int EL, int V> __device__ __forceinline__ void rot_load(const char* p, float (&v)[V]) {
+  constexpr int BYTES = V * (EL == EL_F32 ? 4 : 2);
+  uint32_t w[(BYTES + 3) / 4];
+  if constexpr (BYTES == 16) { const uint4 q = ld_global((const uint4*)p); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
+  else if constexpr (BYTES == 8) { const uint2 q = ld_global((const uint2*)p); w[0] = q.x; w[1] = q.y; }
+  else if constexpr (BYTES == 4) w[0] = ld_global((const uint32_t*)p);
+  else w[0] = ld_global((const uint16_t*)p);
+#pragma unroll
+  for (int i = 0; i < V; i++) v[i] = rot_get<EL>(w, i);
+}
+template <int EL, int V> __device__ __forceinline__ void rot_store(char* p, const float (&v)[V]) {
+  if constexpr (EL == EL_F32) {
+    if constexpr (V == 4) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
+    else *(float*)p = v[0];
+  } else if constexpr (V == 8) {
+    *(uint4*)p = make_uint4(rot_pack<EL>(v[0], v[1]), rot_pack<EL>(v[2], v[3]), rot_pack<EL>(v[4], v[5]), rot_pack<EL>(v[6], v[7]));
+  } else if constexpr (V == 4) {
+    *(uint2*)p = make_uint2(rot_pack<EL>(v[0], v[1]), rot_pack<EL>(v[2], v[3]));
+  } else {
+    *(uint16_t*)p = (uint16_t)(rot_pack<EL>(v[0], 0.f) & 0xffffu);
+  }
+}
+
+// NU units per lane; a unit is two pieces of V elements that start at e0 and e1 (-1: none)
+template <int EL, int V, int NU> struct RotLane {
+  static constexpr int ES = EL == EL_F32 ? 4 : 2;
+  int e[NU][2];
+  float cs[NU][V], sn[NU][V];      // of pair j: half layout (a_j, b_j); interleaved pairs of piece 0, then of piece 1
+  float w[NU][2][V];
+
+  __device__ __forceinline__ void pieces(const RotaryParams& p, int lane) {
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      const int unit = lane + u * p.lanes;
+      int a = -1, b = -1;
+      if (unit < p.units) {
+        if (p.interleaved) { a = 2 * unit * V; b = a + V; }
+        else if (unit < p.pair_units) { a = unit * V; b = a + p.R / 2; }
+        else { a = p.R + 2 * (unit - p.pair_units) * V; b = a + V; }
+        if (b >= p.D) b = -1;
+      }
+      e[u][0] = a; e[u][1] = b;
+    }
+  }
+  // which pair number j is, -1 for elements that pass
+  __device__ __forceinline__ int pair(const RotaryParams& p, int u, int j) const {
+    if (e[u][0] < 0) return -1;
+    int i;
+    if (!p.interleaved) i = e[u][0] < p.R / 2 ? e[u][0] + j : -1;
+    else if constexpr (V == 1) i = e[u][0] / 2;
+    else i = j < V / 2 ? e[u][0] / 2 + j : e[u][0] / 2 + V / 2 + (j - V / 2);
+    return i < p.R / 2 ? i : -1;
+  }
+  // cosines and sines of the warp's token
+  __device__ __forceinline__ void angles(const RotaryParams& p, int token, float2* table) {
+    const int lane = threadIdx.x & 31;
+    const int64_t pos = p.positions ? (int64_t)(int32_t)ld_global((const uint32_t*)p.positions + token) : (int64_t)(token % p.S);
+    __syncwarp();
+    for (int i = lane; i < p.R / 2; i += 32) {
+      const uint2 t = ld_global((const uint2*)(p.turns + i));
+      const uint64_t turn = (((uint64_t)t.y << 32) | t.x) * (uint64_t)pos;
+      float s, c;
+      sincospif((float)(int32_t)(turn >> 32) * (1.0f / 2147483648.0f), &s, &c);
+      table[i] = make_float2(c, s * p.sine);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        const int i = pair(p, u, j);
+        const float2 t = i >= 0 ? table[i] : make_float2(1.f, 0.f);
+        cs[u][j] = t.x; sn[u][j] = t.y;
+      }
+  }
+  __device__ __forceinline__ void weights(const RotaryParams& p, int ti) {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          w[u][s][j] = 1.f;
+          if (p.norm && e[u][s] >= 0) {
+            if (p.weight_f32) w[u][s][j] = ld_global((const float*)p.weight[ti] + e[u][s] + j);
+            else {
+              const uint32_t h = ld_global((const uint16_t*)p.weight[ti] + e[u][s] + j);
+              w[u][s][j] = rot_get<EL>(&h, 0);
+            }
+          }
+        }
+  }
+  __device__ __forceinline__ void load(const char* row, bool on, float (&v)[NU][2][V]) const {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        if (on && e[u][s] >= 0) rot_load<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
+        else {
+#pragma unroll
+          for (int j = 0; j < V; j++) v[u][s][j] = 0.f;
+        }
+      }
+  }
+  __device__ __forceinline__ void store(char* row, const float (&v)[NU][2][V]) const {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+        if (e[u][s] >= 0) rot_store<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
+  }
+  __device__ __forceinline__ void turn(const RotaryParams& p, float (&v)[NU][2][V]) const {
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+      if (V == 1 || !p.interleaved) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+          const float a = v[u][0][j], b = v[u][1][j];
+          // a pair that passes has cos 1 and sin 0; without the test an infinity in one half would make the other NaN
+          if (sn[u][j] != 0.f || cs[u][j] != 1.f) { v[u][0][j] = a * cs[u][j] - b * sn[u][j]; v[u][1][j] = b * cs[u][j] + a * sn[u][j]; }
+        }
+      } else if constexpr (V > 1) {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int j = 0; j < V / 2; j++) {
+            const int k = s * (V / 2) + j;
+            const float a = v[u][s][2 * j], b = v[u][s][2 * j + 1];
+            if (sn[u][k] != 0.f || cs[u][k] != 1.f) { v[u][s][2 * j] = a * cs[u][k] - b * sn[u][k]; v[u][s][2 * j + 1] = b * cs[u][k] + a * sn[u][k]; }
+          }
+      }
+    }
+  }
+  static __device__ __forceinline__ float dot(const float (&a)[NU][2][V], const float (&b)[NU][2][V], int lanes) {
+    float s = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int j = 0; j < V; j++) s = fmaf(a[u][k][j], b[u][k][j], s);
+    for (int off = lanes >> 1; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    return s;
+  }
+};
+
+// The head's rows of a job: tensor, first head and the head behind the last
+struct RotJob { int ti, h0, h1; };
+__device__ __forceinline__ RotJob rot_job(const RotaryParams& p, int job) {
+  const int ti = job >= p.jobs[0] ? 1 : 0;
+  const int h0 = (job - (ti ? p.jobs[0] : 0)) * p.job_heads;
+  return {ti, h0, min(h0 + p.job_heads, p.heads[ti])};
+}
+__device__ __forceinline__ int64_t rot_at(const B2xHeadStrides& s, int b, int h, int t) { return (int64_t)b * s.batch + (int64_t)h * s.head + (int64_t)t * s.token; }
+
+template <int EL, int V, int NU>
+__global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary(const __grid_constant__ RotaryParams p) {
+  __shared__ float2 table[kRotaryWarps][128];
+  constexpr int ES = EL == EL_F32 ? 4 : 2;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * kRotaryWarps + warp;
+  if (id >= p.warps) return;
+  const int all = p.jobs[0] + p.jobs[1];
+  const int token = (int)(id / all);
+  const RotJob job = rot_job(p, (int)(id - (int64_t)token * all));
+  const int b = token / p.S, t = token - b * p.S;
+  const int slots = 32 / p.lanes, slot = lane / p.lanes;
+  RotLane<EL, V, NU> me;
+  me.pieces(p, lane & (p.lanes - 1));
+  me.angles(p, token, table[warp]);
+  me.weights(p, job.ti);
+  for (int h0 = job.h0; h0 < job.h1; h0 += kRotaryRows * slots) {
+    float v[kRotaryRows][NU][2][V];
+#pragma unroll
+    for (int r = 0; r < kRotaryRows; r++) {
+      const int h = h0 + r * slots + slot;
+      me.load(p.x[job.ti] + rot_at(p.xs[job.ti], b, h, t) * ES, h < job.h1, v[r]);
+    }
+#pragma unroll
+    for (int r = 0; r < kRotaryRows; r++) {
+      const int h = h0 + r * slots + slot;
+      if (p.norm) {
+        const float f = rsqrtf(me.dot(v[r], v[r], p.lanes) * p.inv_d + p.epsilon);
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+#pragma unroll
+          for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int j = 0; j < V; j++) v[r][u][s][j] *= f * me.w[u][s][j];
+      }
+      me.turn(p, v[r]);
+      if (h < job.h1) me.store(p.y[job.ti] + rot_at(p.ys[job.ti], b, h, t) * ES, v[r]);
+    }
+  }
+}
+
+// Gradient with norms: tensor blockIdx.y; a warp walks tokens in steps of the grid and keeps its elements' share of dw
+template <int EL, int V, int NU>
+__global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary_gradient(const __grid_constant__ RotaryParams p) {
+  __shared__ float2 table[kRotaryWarps][128];
+  __shared__ float sums[kRotaryWarps][256];
+  constexpr int ES = EL == EL_F32 ? 4 : 2;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ti = blockIdx.y;
+  const int slots = 32 / p.lanes, slot = lane / p.lanes;
+  RotLane<EL, V, NU> me;
+  me.pieces(p, lane & (p.lanes - 1));
+  me.weights(p, ti);
+  float dw[NU][2][V];
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int j = 0; j < V; j++) dw[u][s][j] = 0.f;
+  const int64_t work = (int64_t)p.tokens * p.jobs[ti];
+  for (int64_t id = (int64_t)blockIdx.x * kRotaryWarps + warp; id < work; id += (int64_t)gridDim.x * kRotaryWarps) {
+    const int token = (int)(id / p.jobs[ti]);
+    const int first = (int)(id - (int64_t)token * p.jobs[ti]) * p.job_heads, last = min(first + p.job_heads, p.heads[ti]);
+    const int b = token / p.S, t = token - b * p.S;
+    me.angles(p, token, table[warp]);
+    for (int h0 = first; h0 < last; h0 += slots) {
+      const int h = h0 + slot;
+      float x[NU][2][V], g[NU][2][V];
+      me.load(p.x[ti] + rot_at(p.xs[ti], b, h, t) * ES, h < last, x);
+      me.load(p.dy[ti] + rot_at(p.dys[ti], b, h, t) * ES, h < last, g);
+      me.turn(p, g);
+      const float f = rsqrtf(me.dot(x, x, p.lanes) * p.inv_d + p.epsilon);
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int j = 0; j < V; j++) {
+            x[u][s][j] *= f;
+            if (h < last) dw[u][s][j] = fmaf(g[u][s][j], x[u][s][j], dw[u][s][j]);
+            g[u][s][j] *= me.w[u][s][j];
+          }
+      const float m = me.dot(x, g, p.lanes) * p.inv_d;
+#pragma unroll
+      for (int u = 0; u < NU; u++)
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int j = 0; j < V; j++) g[u][s][j] = f * (g[u][s][j] - x[u][s][j] * m);
+      if (h < last) me.store(p.y[ti] + rot_at(p.ys[ti], b, h, t) * ES, g);
+    }
+  }
+  // the warp's slots, then the CTA's warps, in a fixed order
+#pragma unroll
+  for (int u = 0; u < NU; u++)
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        float d = dw[u][s][j];
+        for (int off = p.lanes; off < 32; off <<= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+        if (slot == 0 && me.e[u][s] >= 0) sums[warp][me.e[u][s] + j] = d;
+      }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.D; i += kRotaryWarps * 32) {
+    float d = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRotaryWarps; k++) d += sums[k][i];
+    p.partial[((int64_t)ti * gridDim.x + blockIdx.x) * p.D + i] = d;
+  }
+}
+
+// dw[i] = sum of the CTAs' partial sums: 32 columns per CTA, 32 threads per column
+__global__ void __launch_bounds__(1024) k_rotary_fold(const float* partial, float* dw0, float* dw1, int rows, int D) {
+  __shared__ float part[32][33];
+  pdl_trigger();
+  pdl_wait();
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
+  const float* src = partial + (int64_t)blockIdx.y * rows * D;
+  float s = 0.f;
+  if (c < D) for (int i = r; i < rows; i += 32) s += ld_global(src + (int64_t)i * D + c);
+  part[r][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (r == 0 && c < D) {
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; i++) t[i & 3] += part[i][threadIdx.x];
+    (blockIdx.y ? dw1 : dw0)[c] = (t[0] + t[1]) + (t[2] + t[3]);
+  }
+}
+
+int rot_elem_size(uint8_t e) { return e == EL_F32 ? 4 : 2; }
+
+bool rot_valid(const B2xRotaryArgs* a) {
+  return (a->elem == EL_BF16 || a->elem == EL_F16 || a->elem == EL_F32) && (a->weight_elem == EL_F32 || a->weight_elem == a->elem || !a->norm) &&
+         (a->n == 1 || a->n == 2) && a->D <= 256 && a->R >= 0 && a->R <= a->D && a->R % 2 == 0 && a->B * a->S < (1ll << 31);
+}
+
+// Elements of a piece: 16 bytes where rows, pieces and partners start on that boundary, else 8 for 16-bit types, else one element.
+int rot_piece(const B2xRotaryArgs* a, bool gradient) {
+  const int es = rot_elem_size(a->elem);
+  for (int v = 16 / es; v >= 4; v /= 2) {
+    bool ok = a->D % v == 0 && (a->interleaved || (a->R / 2) % v == 0);
+    auto row = [&](const void* p, const B2xHeadStrides& s) {
+      if ((uintptr_t)p % (size_t)(v * es) != 0 || s.batch % v != 0 || s.head % v != 0 || s.token % v != 0) ok = false;
+    };
+    for (int i = 0; i < a->n; i++) {
+      row(a->y[i], a->ys[i]);
+      if (a->x[i]) row(a->x[i], a->xs[i]);
+      if (gradient && a->dy[i]) row(a->dy[i], a->dys[i]);
+    }
+    if (ok) return v;
+  }
+  return 1;
+}
+
+RotaryParams rot_params(const B2xRotaryArgs* a, int V) {
+  RotaryParams p{};
+  p.positions = a->positions; p.turns = a->turns;
+  p.tokens = (int32_t)(a->B * a->S); p.S = (int32_t)a->S; p.D = (int32_t)a->D; p.R = (int32_t)a->R;
+  p.epsilon = a->epsilon; p.inv_d = 1.0f / (float)a->D; p.sine = 1.f;
+  p.interleaved = a->interleaved; p.norm = a->norm; p.weight_f32 = a->weight_elem == EL_F32;
+  const int pieces = (p.D + V - 1) / V;
+  p.pair_units = a->interleaved ? 0 : p.R / 2 / V;
+  p.units = a->interleaved ? (pieces + 1) / 2 : p.pair_units + (pieces - 2 * p.pair_units + 1) / 2;
+  p.lanes = 1;
+  while (p.lanes < p.units && p.lanes < 32) p.lanes *= 2;
+  for (int i = 0; i < a->n; i++) {
+    p.x[i] = (const char*)a->x[i]; p.xs[i] = a->xs[i];
+    p.dy[i] = (const char*)a->dy[i]; p.dys[i] = a->dys[i];
+    p.y[i] = (char*)a->y[i]; p.ys[i] = a->ys[i];
+    p.weight[i] = (const char*)a->weight[i];
+    p.heads[i] = (int32_t)a->heads[i];
+  }
+  // a warp walks all heads of its token, unless that leaves SMs without work: then as few as one round of its slots
+  const int slots = 32 / p.lanes;
+  int most = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+  p.job_heads = (most + slots - 1) / slots * slots;
+  if (p.job_heads < slots) p.job_heads = slots;
+  while (p.job_heads > slots && (int64_t)p.tokens * ((p.heads[0] + p.job_heads - 1) / p.job_heads + (p.heads[1] + p.job_heads - 1) / p.job_heads) < (int64_t)kNumSms * 32)
+    p.job_heads = (p.job_heads / 2 + slots - 1) / slots * slots;
+  for (int i = 0; i < 2; i++) p.jobs[i] = (p.heads[i] + p.job_heads - 1) / p.job_heads;
+  p.warps = (int64_t)p.tokens * (p.jobs[0] + p.jobs[1]);
+  return p;
+}
+
+int rot_gradient_ctas(const RotaryParams& p) {
+  const int64_t jobs = p.jobs[0] > p.jobs[1] ? p.jobs[0] : p.jobs[1];
+  const int64_t ctas = ((int64_t)p.tokens * jobs + kRotaryWarps - 1) / kRotaryWarps;
+  return (int)(ctas < 1 ? 1 : ctas > kNumSms * 3 ? kNumSms * 3 : ctas);
+}
+
+template <int EL, int V, int NU>
+int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, bool norm_gradient, cudaStream_t stream) {
+  cudaError_t e;
+  if (norm_gradient) e = launch_overlapped(k_rotary_gradient<EL, V, NU>, dim3((unsigned)rot_gradient_ctas(p), a->n), dim3(kRotaryWarps * 32), 0, stream, p);
+  else e = launch_overlapped(k_rotary<EL, V, NU>, dim3((unsigned)((p.warps + kRotaryWarps - 1) / kRotaryWarps)), dim3(kRotaryWarps * 32), 0, stream, p);
+  if (e != cudaSuccess) return (int)e;
+  count_launch();
+  return (int)cudaGetLastError();
+}
+template <int EL>
+int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, int V, bool norm_gradient, cudaStream_t stream) {
+  if constexpr (EL == EL_F32) {
+    if (V == 4) return launch_rot<EL, 4, 1>(a, p, norm_gradient, stream);
+  } else {
+    if (V == 8) return launch_rot<EL, 8, 1>(a, p, norm_gradient, stream);
+    if (V == 4) return launch_rot<EL, 4, 1>(a, p, norm_gradient, stream);
+  }
+  return launch_rot<EL, 1, 4>(a, p, norm_gradient, stream);
+}
+int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, int V, bool norm_gradient, cudaStream_t stream) {
+  if (a->elem == EL_F32) return launch_rot<EL_F32>(a, p, V, norm_gradient, stream);
+  if (a->elem == EL_BF16) return launch_rot<EL_BF16>(a, p, V, norm_gradient, stream);
+  return launch_rot<EL_F16>(a, p, V, norm_gradient, stream);
+}
+
+}  // namespace
+}  // namespace b2x
+
+extern "C" int b2x_launch_rotary(const B2xRotaryArgs* a, b2x_stream_t stream) {
+  using namespace b2x;
+  if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
+  if (a->D == 0) return 0;
+  const int V = rot_piece(a, false);
+  const RotaryParams p = rot_params(a, V);
+  if (p.warps == 0) return 0;
+  return launch_rot(a, p, V, false, (cudaStream_t)stream);
+}
+
+extern "C" int64_t b2x_rotary_scratch_bytes(const B2xRotaryArgs* a) {
+  // the most CTAs of any piece size: addresses are not known yet when a program is compiled
+  return a->norm ? (int64_t)a->n * b2x::kNumSms * 3 * a->D * 4 : 0;
+}
+
+extern "C" int b2x_rotary_launches(const B2xRotaryArgs* a, int gradient) {
+  if (a->D == 0) return 0;
+  if (gradient && a->norm) return a->B * a->S == 0 ? 1 : 2;
+  return a->B * a->S * (a->heads[0] + a->heads[1]) > 0 ? 1 : 0;
+}
+
+extern "C" int b2x_launch_rotary_gradient(const B2xRotaryArgs* a, b2x_stream_t stream) {
+  using namespace b2x;
+  if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
+  if (a->D == 0) return 0;
+  const int V = rot_piece(a, true);
+  RotaryParams p = rot_params(a, V);
+  p.sine = -1.f;
+  if (!a->norm) {
+    // the rotation's transpose: the same kernel, turned the other way
+    for (int i = 0; i < a->n; i++) { p.x[i] = p.dy[i]; p.xs[i] = p.dys[i]; }
+    if (p.warps == 0) return 0;
+    return launch_rot(a, p, V, false, (cudaStream_t)stream);
+  }
+  p.partial = (float*)a->scratch;
+  const int rows = p.tokens > 0 ? rot_gradient_ctas(p) : 0;
+  if (rows > 0) {
+    const int rc = launch_rot(a, p, V, true, (cudaStream_t)stream);
+    if (rc) return rc;
+  }
+  const cudaError_t e = launch_overlapped(k_rotary_fold, dim3((unsigned)((p.D + 31) / 32), a->n), dim3(1024), 0, (cudaStream_t)stream, (const float*)p.partial,
+                                          a->dweight[0], a->dweight[1], rows, p.D);
+  if (e != cudaSuccess) return (int)e;
+  count_launch();
+  return (int)cudaGetLastError();
+}

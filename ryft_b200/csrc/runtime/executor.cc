@@ -3,6 +3,7 @@
 // with later compute steps (reference call site: PJRT_LoadedExecutable_Execute,
 // crates/ryft-pjrt/src/programs.rs:923-936).  Nothing here synchronises with the host.
 #include "../../../include/b2x_kernels.h"
+#include "call_args.h"
 #include "nccl_dyn.h"
 #include "objects.h"
 
@@ -163,6 +164,18 @@ PJRT_Error* run_plan(PJRT_LoadedExecutable* le, int local_index, int replica, co
       }
       case StepKind::SOFTMAX: {
         int rc = b2x_launch_softmax(bind(s.c_src), bind(s.c_dst), (uint8_t)s.r_out_dtype, s.rA, s.rR, cs);
+        if (rc) return kernel_error(rc, s);
+        break;
+      }
+      case StepKind::CALL: {
+        int rc;
+        if (s.call->kind == CallKind::ROTARY) {
+          const B2xRotaryArgs a = rotary_args(s, bind);
+          rc = s.call->rotary.gradient ? b2x_launch_rotary_gradient(&a, cs) : b2x_launch_rotary(&a, cs);
+        } else {
+          const B2xHeadAttentionArgs a = head_attention_args(s, bind);
+          rc = s.call->attention.gradient ? b2x_launch_head_attention_gradient(&a, dev->status_dev, cs) : b2x_launch_head_attention(&a, dev->status_dev, cs);
+        }
         if (rc) return kernel_error(rc, s);
         break;
       }

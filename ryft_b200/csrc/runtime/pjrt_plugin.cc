@@ -11,6 +11,7 @@
 #include <cstring>
 #include <sstream>
 
+#include "call_args.h"
 #include "nccl_dyn.h"
 #include "objects.h"
 
@@ -1319,6 +1320,12 @@ static int step_kernel_launches(const Step& s) {
     case StepKind::GEMM: return s.g_split_f32 ? 2 : 1;
     case StepKind::ATTENTION: return 1;
     case StepKind::SOFTMAX: return 1;
+    case StepKind::CALL: {
+      const auto nowhere = [](const BufRef&) -> void* { return nullptr; };
+      if (s.call->kind == CallKind::ROTARY) { const B2xRotaryArgs a = rotary_args(s, nowhere); return b2x_rotary_launches(&a, s.call->rotary.gradient); }
+      const B2xHeadAttentionArgs a = head_attention_args(s, nowhere);
+      return b2x_head_attention_launches(&a, s.call->attention.gradient);
+    }
     default: return 0;
   }
 }
@@ -1333,7 +1340,8 @@ static PJRT_Error* Ext_StepTiming(B2X_StepTiming_Args* a) {
     for (auto& s : plan.steps) {
       const char* kind = s.kind == StepKind::GEMM ? (s.g_tensor_core ? "gemm_tc " : "gemm_simt ") : s.kind == StepKind::REDUCE ? "reduce " :
                          s.kind == StepKind::ELEMENTWISE ? "elementwise " : s.kind == StepKind::ATTENTION ? "attention " :
-                         s.kind == StepKind::COPY ? "copy " : s.kind == StepKind::WIDE ? "wide " : s.kind == StepKind::SOFTMAX ? "softmax " : "collective ";
+                         s.kind == StepKind::COPY ? "copy " : s.kind == StepKind::WIDE ? "wide " : s.kind == StepKind::SOFTMAX ? "softmax " :
+                         s.kind == StepKind::CALL ? "call " : "collective ";
       le->step_labels.push_back(std::string(kind) + s.label);
       le->step_flops.push_back(s.flops);
       le->step_bytes.push_back(s.bytes);

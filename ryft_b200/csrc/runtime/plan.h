@@ -6,9 +6,11 @@
 // (crates/ryft-pjrt/src/programs.rs:923-936) runs it.
 #pragma once
 #include <cstdint>
+#include <memory>
 #include <string>
 #include <vector>
 
+#include "../frontend/custom_call.h"
 #include "../frontend/ir.h"
 #include "../kernels/vm.h"
 
@@ -21,7 +23,7 @@ struct BufRef {
   bool valid() const { return kind != NONE; }
 };
 
-enum class StepKind : uint8_t { ELEMENTWISE, REDUCE, GEMM, ATTENTION, ALL_REDUCE, ALL_GATHER, COPY, WIDE, SOFTMAX };
+enum class StepKind : uint8_t { ELEMENTWISE, REDUCE, GEMM, ATTENTION, ALL_REDUCE, ALL_GATHER, COPY, WIDE, SOFTMAX, CALL };
 
 struct VmBinding {
   B2xVmProgram prog{};             // tensor pointers are null in the plan; bound at launch
@@ -95,6 +97,12 @@ struct Step {
   std::vector<int64_t> w_in_strides[3];
   BufRef w_in[3], w_out;
   uint64_t w_imm = 0;
+
+  // CALL: an operator that the program names; buffers and element strides (batch, head, token) of operands and results in their order
+  std::shared_ptr<const CallSpec> call;
+  struct CallTensor { BufRef buf; int64_t batch = 0, head = 0, token = 0; };
+  std::vector<CallTensor> call_in, call_out;
+  BufRef call_table;               // rotary: turns per position of each pair
 
   // bookkeeping for cost analysis
   double flops = 0, bytes = 0;

@@ -6,6 +6,7 @@
 // becomes a standalone elementwise kernel, the prologue of a reduce kernel, or the epilogue of the GEMM that
 // produces its input.  transpose/reshape become strided views where the layout allows.  Intermediates live in one
 // arena whose offsets are assigned from value lifetimes.
+#include "call_args.h"
 #include "plan.h"
 
 #include "../../../include/b2x_kernels.h"
@@ -285,6 +286,7 @@ class Planner {
   void emit_wide_copy(const Layout& src, DType src_dt, const std::vector<int64_t>& dims, const BufRef& dst, DType dst_dt, const std::string& label);
   void emit_wide_reduce(const Op& op);
   void emit_collective(const Op& op);
+  void emit_call(const Op& op);
   void emit_outputs();
   BufRef emit_strided_copy(const Layout& src, DType dt, const std::vector<int64_t>& dims, const std::string& label);
   void push_vm_step(VmBinding&& vm, const std::string& label);
@@ -1574,6 +1576,66 @@ void Planner::emit_collective(const Op& op) {
   }
 }
 
+// ---- operators that the program names (custom_call.h) -----------------------------------------------------------------------
+// Tensors of heads keep a view's strides where rows stay contiguous and 16-byte aligned (a transpose in front of the call costs
+// nothing); everything else is copied into dense memory first.
+void Planner::emit_call(const Op& op) {
+  auto spec = std::make_shared<CallSpec>(describe_call(op));
+  const bool rotary = spec->kind == CallKind::ROTARY;
+  const bool bshd = rotary ? spec->rotary.bshd : spec->attention.bshd;
+  Step s;
+  s.kind = StepKind::CALL;
+  s.label = op.call_target + ":%" + op.results[0]->name;
+  s.call = spec;
+  auto tensor = [&](const Value* v, BufRef buf, const std::vector<int64_t>& strides) {
+    Step::CallTensor t;
+    t.buf = buf;
+    if (v->type.rank() == 4) { t.batch = strides[0]; t.head = strides[bshd ? 2 : 1]; t.token = strides[bshd ? 1 : 2]; }
+    return t;
+  };
+  for (const Value* v : op.operands) {
+    Layout L = layout_of(v);
+    const int64_t piece = 16 / dtype_size(v->type.dtype);
+    bool keep = is_row_major(v->type.dims, L.strides);
+    if (!keep && v->type.rank() == 4 && v->type.num_elements() > 0) {
+      keep = L.strides[3] == 1;
+      for (int d = 0; d < 3; d++) if (v->type.dims[d] > 1 && (L.strides[d] <= 0 || L.strides[d] % piece != 0)) keep = false;
+    }
+    if (!keep) {
+      L.buf = emit_strided_copy(L, v->type.dtype, v->type.dims, "copy:call_operand");
+      L.strides = row_major_strides(v->type.dims);
+    }
+    s.call_in.push_back(tensor(v, L.buf, L.strides));
+    s.bytes += (double)v->type.byte_size();
+  }
+  for (const Value* v : op.results) {
+    s.call_out.push_back(tensor(v, materialise(v), row_major_strides(v->type.dims)));
+    s.bytes += (double)v->type.byte_size();
+  }
+  if (rotary) {
+    const std::vector<uint64_t> turns = spec->rotary.turns();
+    s.call_table.kind = BufRef::CONST;
+    s.call_table.offset = ((int64_t)plan_.const_pool.size() + 255) / 256 * 256;
+    plan_.const_pool.resize((size_t)s.call_table.offset + std::max<size_t>(turns.size(), 1) * 8);
+    if (!turns.empty()) memcpy(plan_.const_pool.data() + s.call_table.offset, turns.data(), turns.size() * 8);
+    const B2xRotaryArgs a = rotary_args(s, [](const BufRef&) -> void* { return nullptr; });
+    s.scratch_bytes = spec->rotary.gradient ? b2x_rotary_scratch_bytes(&a) : 0;
+  } else {
+    const AttentionSpec& at = spec->attention;
+    const B2xHeadAttentionArgs a = head_attention_args(s, [](const BufRef&) -> void* { return nullptr; });
+    s.scratch_bytes = b2x_head_attention_scratch_bytes(&a, at.gradient ? 1 : 0);
+    // what the masks of the attributes leave; documents, prefixes and lengths are known at run time only
+    double pairs = (double)at.Sq * (double)at.Sk;
+    if (at.causal && !at.queries_at_end && at.prefix < 0) {
+      pairs = 0;
+      for (int64_t i = 0; i < at.Sq; i++) pairs += (double)std::min<int64_t>(at.query_offset + i + 1, at.Sk);
+    }
+    s.flops = (at.gradient ? 10.0 : 4.0) * (double)at.B * (double)at.Hq * (double)at.D * pairs;
+  }
+  if (s.scratch_bytes > 0) { s.scratch = new_temp(s.scratch_bytes); touch(s.scratch); }
+  plan_.steps.push_back(std::move(s));
+}
+
 void Planner::emit_outputs() {
   for (size_t i = 0; i < m_.outputs.size(); i++) {
     const Value* v = m_.outputs[i];
@@ -1660,6 +1722,11 @@ static void step_bufs(const Step& s, std::vector<BufRef>* reads, std::vector<Buf
       for (auto& c : s.colls) { reads->push_back(c.src); writes->push_back(c.dst); }
       break;
     case StepKind::COPY: case StepKind::SOFTMAX: reads->push_back(s.c_src); writes->push_back(s.c_dst); break;
+    case StepKind::CALL:
+      for (auto& t : s.call_in) reads->push_back(t.buf);
+      for (auto& t : s.call_out) writes->push_back(t.buf);
+      if (s.scratch.valid()) writes->push_back(s.scratch);
+      break;
   }
 }
 
@@ -1803,6 +1870,8 @@ void Planner::assign_arena() {
     fix(s.aq); fix(s.ak); fix(s.av); fix(s.ao); fix(s.c_src); fix(s.c_dst);
     for (int k = 0; k < 3; k++) fix(s.w_in[k]);
     fix(s.w_out);
+    for (auto& t : s.call_in) fix(t.buf);
+    for (auto& t : s.call_out) fix(t.buf);
     for (auto& c : s.colls) { fix(c.src); fix(c.dst); }
   }
 }
@@ -1865,6 +1934,7 @@ Plan Planner::run() {
           }
           case OpKind::TRANSPOSE: case OpKind::RESHAPE: emit_view_or_copy(op); break;
           case OpKind::ALL_REDUCE: case OpKind::ALL_GATHER: emit_collective(op); break;
+          case OpKind::CUSTOM_CALL: emit_call(op); break;
           default: unimplemented(std::string(op_name(op.kind)) + " has no lowering");
         }
     }
@@ -1973,6 +2043,13 @@ std::string Plan::dump() const {
         break;
       case StepKind::SOFTMAX:
         o << "softmax " << s.label << " [" << s.rA << "," << s.rR << "] " << buf_str(s.c_src) << " -> " << buf_str(s.c_dst) << ":" << dtype_name(s.r_out_dtype) << "\n";
+        break;
+      case StepKind::CALL:
+        o << "call " << s.label << " (";
+        for (size_t k = 0; k < s.call_in.size(); k++) o << (k ? ", " : "") << buf_str(s.call_in[k].buf);
+        o << ") -> (";
+        for (size_t k = 0; k < s.call_out.size(); k++) o << (k ? ", " : "") << buf_str(s.call_out[k].buf);
+        o << ") scratch=" << s.scratch_bytes << " B\n";
         break;
       case StepKind::COPY: o << "copy " << s.label << " " << buf_str(s.c_src) << " -> " << buf_str(s.c_dst) << " " << s.c_bytes << " B\n"; break;
     }

@@ -240,6 +240,92 @@ class Builder:
             f"tensor<{rows}x{cols}xi64>}}> : ({a.type}) -> {t}",
         )
 
+    # ---- operators of the executor, through stablehlo.custom_call --------------------------------------------------
+    def _call(self, target: str, operands: Sequence[Value], results: Sequence[TensorType], attributes: dict) -> List[Value]:
+        def text(v):
+            if isinstance(v, bool):
+                return "true" if v else "false"
+            if isinstance(v, int):
+                return f"{v} : i64"
+            if isinstance(v, float):
+                return f"{v:.17e} : f64"
+            if isinstance(v, str):
+                return f'"{v}"'
+            return "[" + ", ".join(text(x) for x in v) + "]"
+        config = ", ".join(f"{k} = {text(v)}" for k, v in attributes.items() if v is not None)
+        base = self._new(results[0]).name
+        outs = [Value(base, results[0])] if len(results) == 1 else [Value(f"{base}#{i}", t) for i, t in enumerate(results)]
+        types = str(results[0]) if len(results) == 1 else "(" + ", ".join(map(str, results)) + ")"
+        self._lines.append(
+            f"    {base}{'' if len(results) == 1 else f':{len(results)}'} = stablehlo.custom_call @{target}({', '.join(map(str, operands))}) "
+            f"{{api_version = 4 : i32, backend_config = {{{config}}}}} : ({', '.join(str(o.type) for o in operands)}) -> {types}"
+        )
+        return outs
+
+    @staticmethod
+    def _rotary_attributes(layout, rotary_dims, interleaved, base, factor, bands, epsilon, weights) -> dict:
+        assert (epsilon is None) == (weights is None), "a norm takes weights and an epsilon"
+        return {"layout": layout, "rotary_dims": rotary_dims, "interleaved": True if interleaved else None, "base": float(base), "factor": float(factor),
+                "bands": [float(x) for x in bands] if bands is not None else None, "epsilon": float(epsilon) if epsilon is not None else None}
+
+    def rotary(self, tensors: Sequence[Value], positions: Value | None = None, weights: Sequence[Value] | None = None, *, layout: str = "bhsd",
+               rotary_dims: int | None = None, interleaved: bool = False, base: float = 10000.0, factor: float = 1.0,
+               bands: Sequence[float] | None = None, epsilon: float | None = None) -> List[Value]:
+        """Rotary positions of one or two tensors of heads (queries and keys), `[B, H, S, D]` or with `layout="bshd"`
+        `[B, S, H, D]`, in one pass.  Pair i of the first `rotary_dims` elements of a head (i and i + rotary_dims/2, or 2i and
+        2i + 1 when `interleaved`) turns by position * base^(-2i/rotary_dims).  `factor` stretches positions: all of them
+        linearly, or with `bands = (low, high, original)` only wavelengths above original/low, those between original/high and
+        original/low in part.  `positions` is i32 [B, S]; without it token t is at t.  With `weights` ([D] each, f32 or the
+        tensors' type) and `epsilon`, a head is first divided by the root of its mean square and weighted.  bf16, f16 or f32,
+        heads up to 256 wide; arithmetic in f32 with one rounding."""
+        a = self._rotary_attributes(layout, rotary_dims, interleaved, base, factor, bands, epsilon, weights)
+        return self._call("b2x.rotary", [*tensors, *(weights or []), *([positions] if positions is not None else [])], [t.type for t in tensors], a)
+
+    def rotary_gradient(self, gradients: Sequence[Value], tensors: Sequence[Value] | None = None, positions: Value | None = None,
+                        weights: Sequence[Value] | None = None, *, layout: str = "bhsd", rotary_dims: int | None = None, interleaved: bool = False,
+                        base: float = 10000.0, factor: float = 1.0, bands: Sequence[float] | None = None, epsilon: float | None = None) -> List[Value]:
+        """The gradients of `rotary`: of its tensors, and with norms (which need the `tensors` themselves) of its weights
+        (f32), from those of its results."""
+        a = self._rotary_attributes(layout, rotary_dims, interleaved, base, factor, bands, epsilon, weights)
+        assert weights is None or tensors is not None, "the gradient of a norm reads the tensors"
+        extra = [*tensors, *weights] if weights is not None else []
+        results = [g.type for g in gradients] + [TensorType(w.type.dims, "f32") for w in (weights or [])]
+        return self._call("b2x.rotary_gradient", [*gradients, *extra, *([positions] if positions is not None else [])], results, a)
+
+    @staticmethod
+    def _attention_inputs(layout, scale, causal, query_offset, queries_at_end, softcap, slopes, documents, prefix, lengths):
+        extra = {"slopes": slopes, "documents": documents, "prefix": prefix, "lengths": lengths}
+        extra = {k: v for k, v in extra.items() if v is not None}
+        return list(extra.values()), {"layout": layout, "scale": float(scale) if scale is not None else None, "causal": True if causal else None,
+                                      "query_offset": query_offset or None, "queries_at_end": True if queries_at_end else None,
+                                      "softcap": float(softcap) if softcap else None, "inputs": list(extra) or None}
+
+    def attention(self, q: Value, k: Value, v: Value, *, layout: str = "bhsd", scale: float | None = None, causal: bool = False, query_offset: int = 0,
+                  queries_at_end: bool = False, softcap: float = 0.0, slopes: Value | None = None, documents: Value | None = None,
+                  prefix: Value | None = None, lengths: Value | None = None, log_sum: bool = False):
+        """softmax(scores) v over tensors of heads, `[B, H, S, D]` or with `layout="bshd"` `[B, S, H, D]`; bf16 or f16, D a
+        multiple of 8 up to 128.  The query heads may be a multiple of the key heads.  scores = softcap * tanh(scale * q k /
+        softcap) - slopes[h] * |p - j| (`scale` defaults to 1/sqrt(D)).  A query at p sees key j when j < lengths[b], and under
+        `causal` j <= p or j < prefix[b], and with `documents` (i32 [B, Sk]) both lie in one document.  Query i is at
+        query_offset + i, or with `queries_at_end` (a cache) at lengths[b] - Sq + i.  `slopes` is f32 [H], `prefix` and
+        `lengths` are i32 [B].  A query that sees nothing yields 0.  With `log_sum` also the natural log of each query's sum
+        of exponentials, f32 [B, H, Sq] (-inf where nothing is seen), which the gradient reads."""
+        extra, a = self._attention_inputs(layout, scale, causal, query_offset, queries_at_end, softcap, slopes, documents, prefix, lengths)
+        types = [q.type]
+        if log_sum:
+            d = q.type.dims
+            types.append(TensorType((d[0], d[2], d[1]) if layout == "bshd" else (d[0], d[1], d[2]), "f32"))
+        out = self._call("b2x.attention", [q, k, v, *extra], types, a)
+        return tuple(out) if log_sum else out[0]
+
+    def attention_gradient(self, q: Value, k: Value, v: Value, o: Value, log_sum: Value, do: Value, *, layout: str = "bhsd", scale: float | None = None,
+                           causal: bool = False, query_offset: int = 0, queries_at_end: bool = False, softcap: float = 0.0, slopes: Value | None = None,
+                           documents: Value | None = None, prefix: Value | None = None, lengths: Value | None = None) -> List[Value]:
+        """The gradients (dq, dk, dv) of `attention` from its result, log sums and the result's gradient `do`.  dk and dv are
+        sums over the query heads that share a key head.  Slopes are constants: they get no gradient."""
+        extra, a = self._attention_inputs(layout, scale, causal, query_offset, queries_at_end, softcap, slopes, documents, prefix, lengths)
+        return self._call("b2x.attention_gradient", [q, k, v, o, log_sum, do, *extra], [q.type, k.type, v.type], a)
+
     # ---- helpers for scalars broadcast to a shape -------------------------------------------------------------
     def splat(self, value, like: Value) -> Value:
         return self.constant(value, like.type.dims, like.type.dtype)
