@@ -29,6 +29,7 @@
 #include <atomic>
 #include <cstdlib>
 #include "../../../include/b2x_kernels.h"
+#include "attention_math.cuh"
 #include "common.cuh"
 #include "sm100.cuh"
 
@@ -77,37 +78,6 @@ struct AttnSmem {
   static constexpr int TOTAL = BAR_OFF + 256 + 1024;
 };
 
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two f32 lanes per instruction (sm_100 packed single precision) and the three-input maximum: the softmax warps are
-// bound by instruction issue, and these halve the count of everything except the exponentials themselves.
-__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t splat2(float v) { return pack2(__float_as_uint(v), __float_as_uint(v)); }
-__device__ __forceinline__ void unpack2(uint64_t v, uint32_t& lo, uint32_t& hi) { asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-// NaN-propagating, so that a NaN score poisons its row as it does in an unfused softmax
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
 template <int D, int TPR, bool PT>
 __global__ void __launch_bounds__(96 + 256 * TPR, 1)
 k_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,

@@ -4,10 +4,10 @@
 // Gradient: P = exp(s - lse), dP = dO V^T, delta = sum(dO * O), dS = P (dP - delta) (1 - tanh^2) scale; dQ = dS K, dK = dS^T Q,
 // dV = P^T dO, the last two over all query heads that share the key head.  Sums, statistics and scores in f32.
 //
-// One warp per query (forward, dQ) or per key (dK, dV); lanes share the head's width.
+// The forward pass is in head_attention_tc.cu.  Gradient: one warp per query (dQ) or per key (dK, dV); lanes share the head's width.
 #include <cmath>
 
-#include "head_attention.cuh"
+#include "head_attention_tc.cuh"
 
 namespace b2x {
 namespace {
@@ -58,37 +58,6 @@ __device__ __forceinline__ bool ha_document(const HeadAttn& p, int b, int pos, i
   if (pos < 0 || pos >= p.Sk) return false;
   *doc = (int)ld_global((const uint32_t*)p.documents + (int64_t)b * p.Sk + pos);
   return true;
-}
-
-template <int EL>
-__global__ void __launch_bounds__(128) k_head_attention_simple(const __grid_constant__ HeadAttn p) {
-  pdl_trigger();
-  pdl_wait();
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (id >= (int64_t)p.B * p.Hq * p.Sq) return;
-  const int i = (int)(id % p.Sq), h = (int)(id / p.Sq % p.Hq), b = (int)(id / p.Sq / p.Hq), u = h / p.group;
-  const HeadSequence s = head_sequence(p, b);
-  const int pos = s.first + i;
-  int doc;
-  const int end = ha_document(p, b, pos, &doc) ? head_limit(p, s, pos) : 0;
-  const float slope = p.slopes ? ld_global(p.slopes + h) : 0.f;
-  Row<EL> q, k, v;
-  q.load(p.q, ha_at(p.qs, b, h, i), p.D);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f}, bend;
-  for (int j = 0; j < end; j++) {
-    if (p.documents && (int)ld_global((const uint32_t*)p.documents + (int64_t)b * p.Sk + j) != doc) continue;
-    k.load(p.k, ha_at(p.ks, b, u, j), p.D);
-    v.load(p.v, ha_at(p.vs, b, u, j), p.D);
-    const float x = ha_score(p, q.dot(k), slope, pos, j, &bend);
-    const float mm = x > m || x != x ? x : m;
-    const float a = m == -INFINITY ? 0.f : expf(m - mm), e = x == -INFINITY ? 0.f : expf(x - mm);
-    l = l * a + e;
-#pragma unroll
-    for (int c = 0; c < 4; c++) o[c] = o[c] * a + e * v.v[c];
-    m = mm;
-  }
-  ha_store<EL>(p.o, ha_at(p.os, b, h, i), p.D, o, l == 0.f ? 0.f : 1.f / l);
-  if (p.lse && (threadIdx.x & 31) == 0) p.lse[id] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 template <int EL>
@@ -154,8 +123,13 @@ __global__ void __launch_bounds__(128) k_head_attention_dkv_simple(const __grid_
   ha_store<EL>(p.dv, ha_at(p.dvs, b, u, j), p.D, gv, 1.f);
 }
 
+// rows that 16-byte accesses can reach
+bool ha_rows(const void* p, const B2xHeadStrides& s, int64_t B, int64_t H, int64_t S) {
+  return ((uintptr_t)p & 15) == 0 && (B <= 1 || s.batch % 8 == 0) && (H <= 1 || s.head % 8 == 0) && (S <= 1 || s.token % 8 == 0);
+}
 bool ha_valid(const B2xHeadAttentionArgs* a) {
-  return (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 && (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) &&
+  return ha_rows(a->q, a->qs, a->B, a->Hq, a->Sq) && ha_rows(a->k, a->ks, a->B, a->Hk, a->Sk) && ha_rows(a->v, a->vs, a->B, a->Hk, a->Sk) &&
+         ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && (!a->lse || a->B * a->Hq * a->Sq < (1ll << 40)) && (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 && (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) &&
          a->Sq < (1ll << 30) && a->Sk < (1ll << 30) && a->query_offset >= 0 && a->query_offset < (1ll << 30) && (!a->queries_at_end || a->lengths);
 }
 
@@ -187,24 +161,26 @@ int ha_launch(void (*bf16)(HeadAttn), void (*f16)(HeadAttn), int elem, const Hea
 }  // namespace
 }  // namespace b2x
 
-extern "C" int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* a, int gradient) { return gradient ? a->B * a->Hq * a->Sq * 4 : 0; }
+extern "C" int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* a, int gradient) {
+  const int64_t ranges = a->documents ? a->B * ((a->Sk + b2x::HA_BLOCK - 1) / b2x::HA_BLOCK) * 8 : 0;
+  return gradient ? a->B * a->Hq * a->Sq * 4 : ranges;
+}
 
 extern "C" int b2x_head_attention_launches(const B2xHeadAttentionArgs* a, int gradient) {
   const int q = a->B * a->Hq * a->Sq > 0, k = a->B * a->Hk * a->Sk > 0;
-  return gradient ? q + k : q;
+  return gradient ? q + k : q + (q && k && a->documents ? 1 : 0);
 }
 
 extern "C" int b2x_launch_head_attention(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
-  (void)status;
-  if (!ha_valid(a)) return (int)cudaErrorInvalidValue;
-  return ha_launch(k_head_attention_simple<EL_BF16>, k_head_attention_simple<EL_F16>, a->elem, ha_params(a), a->B * a->Hq * a->Sq, (cudaStream_t)stream);
+  if (!ha_valid(a) || (b2x_head_attention_scratch_bytes(a, 0) > 0 && !a->scratch)) return (int)cudaErrorInvalidValue;
+  return ha_launch_forward(ha_params(a), a->elem, (int2*)a->scratch, status, (cudaStream_t)stream);
 }
 
 extern "C" int b2x_launch_head_attention_gradient(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
   (void)status;
-  if (!ha_valid(a) || !a->lse) return (int)cudaErrorInvalidValue;
+  if (!ha_valid(a) || !a->lse || (b2x_head_attention_scratch_bytes(a, 1) > 0 && !a->scratch)) return (int)cudaErrorInvalidValue;
   const HeadAttn p = ha_params(a);
   const int rc = ha_launch(k_head_attention_dq_simple<EL_BF16>, k_head_attention_dq_simple<EL_F16>, a->elem, p, a->B * a->Hq * a->Sq, (cudaStream_t)stream);
   if (rc) return rc;

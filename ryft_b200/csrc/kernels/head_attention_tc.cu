@@ -1,0 +1,605 @@
+// Attention over tiles of 128 queries on the tensor cores: persistent, one CTA per SM, two independent workers per CTA.
+//
+// A worker owns a tile at a time (drawn from a device-wide counter), walks its blocks of 128 keys with the running maximum and
+// sum of a softmax, normalises and writes its rows, and draws the next; while one worker starts or ends a tile the tensor and
+// special-function pipes work for the other.  384 threads: warps 0, 1 draw tiles and load (TMA), warps 2, 3 issue the MMAs,
+// warps 4-7 and 8-11 are the workers' softmax, one thread per query: its 128 scores are read from TMEM once and stay in
+// registers through cap, bias, mask, maximum and exponential.  Per worker Q, one K and one V stage, half a buffer of weights (the
+// second half's first keys are exponentiated while the first half multiplies), 128 score columns and the accumulator in TMEM.
+//
+// What masks leave out is left out in three grades: blocks that no query of the tile sees are neither loaded nor multiplied (the
+// keys' end follows from the last query; with documents the loading warp compares ranges of document numbers and publishes the
+// tile's blocks as bits); blocks that every query sees run without a test; in the others a row's keys are 128 bits, from the
+// row's last key and, by ballots over the warp's distinct documents, from the document numbers.
+//
+// Rows of V behind a sequence's length are set to zero in shared memory before they meet their zero weights: a product of 0 and
+// what happens to lie there might be NaN.
+#include <atomic>
+
+#include "head_attention_tc.cuh"
+
+namespace b2x {
+namespace {
+
+struct TileParams {
+  HeadAttn a;
+  const int2* ranges;          // documents' ranges per block, [B][key blocks]
+  int32_t q_tiles, group_heads, key_blocks, total;
+  float mult;                  // scores in registers times this are log2 units: scale * log2(e), or 1 where cap or bias made them so
+  float cap_in, cap_out;       // exponent 2 * scale / cap * log2(e), cap * log2(e); without a cap scale * log2(e), 0
+  int32_t scaled;              // scores are brought to log2 units before anything else (bias; scale not positive)
+  uint32_t idesc_qk, idesc_pv;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A tile as its loading warp publishes it.
+struct TileSlot {
+  int tile;                    // -1: no more
+  int b, h, q0;
+  int blocks;                  // key blocks to walk
+  int length, first, prefix;   // HeadSequence
+  uint32_t visit[HA_MASK_WORDS], compare[HA_MASK_WORDS];   // with documents: blocks to walk, and those whose documents have to be compared
+};
+
+template <int D> struct TileSmem {
+  static constexpr int Q_BYTES = HA_BLOCK * D * 2;
+  static constexpr int KV_BYTES = HA_BLOCK * D * 2;
+  static constexpr int P_BYTES = HA_BLOCK * 64 * 2;
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = Q_OFF + Q_BYTES;
+  static constexpr int V_OFF = K_OFF + KV_BYTES;
+  static constexpr int P_OFF = V_OFF + KV_BYTES;
+  static constexpr int W_BYTES = P_OFF + P_BYTES;
+  static constexpr int BAR_OFF = 2 * W_BYTES;              // 2 x 16 barriers, TMEM slot, abort flag
+  static constexpr int SLOT_OFF = BAR_OFF + 288;
+  static constexpr int TOTAL = SLOT_OFF + 4 * (int)sizeof(TileSlot) + 1024;
+};
+
+// A tile's blocks in their order: all from 0, or those whose bits are set
+struct BlockWalk {
+  const volatile TileSlot* s;
+  int j;
+  bool listed;
+  __device__ __forceinline__ void start(const volatile TileSlot* slot, bool list) { s = slot; listed = list; j = -1; next(); }
+  __device__ __forceinline__ void next() {
+    j++;
+    if (!listed) return;
+    int w = j >> 5;
+    uint32_t m = w < HA_MASK_WORDS ? s->visit[w] & (0xffffffffu << (j & 31)) : 0u;
+    while (m == 0 && ++w < HA_MASK_WORDS) m = s->visit[w];
+    j = m ? w * 32 + __ffs(m) - 1 : HA_MASK_WORDS * 32;
+  }
+};
+
+template <int D, int EL>
+__global__ void __launch_bounds__(384, 1)
+k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const __grid_constant__ TileParams p, int32_t* sched, int32_t* status) {
+  using namespace sm100;
+  using SM = TileSmem<D>;
+  constexpr int DC = D / 64;
+  constexpr uint32_t TMEM_COLS = 512;          // S0 [0,128), S1 [128,256), O0 [256, 256 + D), O1 [256 + D, 256 + 2 D)
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = (uint64_t*)(smem + SM::BAR_OFF);
+  uint32_t* tmem_slot = (uint32_t*)(bars + 32);
+  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int w = warp < 4 ? (warp & 1) : ((warp - 4) >> 2);   // worker
+  volatile TileSlot* slots = (volatile TileSlot*)(smem + SM::SLOT_OFF) + 2 * w;   // the worker's current and next tile
+  const uint32_t wb = smem_u32(bars) + (uint32_t)w * 128u;
+  const uint32_t bar_qf = wb, bar_qe = wb + 8, bar_kf = wb + 16, bar_ke = wb + 24, bar_vf = wb + 32, bar_ve = wb + 40, bar_sf = wb + 48,
+                 bar_se = wb + 56, bar_pf = wb + 64, bar_pv = wb + 72, bar_of = wb + 80, bar_tf = wb + 88 /* [2] */, bar_te = wb + 104 /* [2] */,
+                 bar_drain = wb + 120;
+  const uint32_t wbase = sbase + (uint32_t)w * SM::W_BYTES;
+  const bool listed = p.ranges != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int v = 0; v < 2; v++) {
+      const uint32_t b = smem_u32(bars) + (uint32_t)v * 128u;
+      mbar_init(b, 1); mbar_init(b + 8, 1); mbar_init(b + 16, 1); mbar_init(b + 24, 1); mbar_init(b + 32, 1); mbar_init(b + 40, 1);
+      mbar_init(b + 48, 1); mbar_init(b + 56, 4); mbar_init(b + 64, 4); mbar_init(b + 72, 1); mbar_init(b + 80, 4);
+      mbar_init(b + 88, 1); mbar_init(b + 96, 1); mbar_init(b + 104, 5); mbar_init(b + 112, 5); mbar_init(b + 120, 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+  }
+  if (warp == 2) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();          // everything above touched this SM only
+
+  if (warp < 2) {
+    // ---------------------------------------------- tiles and loads ------------------------------------------------
+    uint32_t kc = 0, vc = 0;       // K and V blocks loaded so far
+    uint32_t nq = 0;               // tiles with work so far
+    int fixed = (int)blockIdx.x * 2 + w;   // without a counter: every worker takes tiles in steps of all workers
+    for (int n = 0;; n++) {
+      // the slot's previous tile has been read by the issuer and the four softmax warps (all lanes wait: they leave together)
+      const bool free = n < 2 || mbar_wait(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21);
+      if (!__all_sync(0xffffffffu, free)) break;
+      int t = 0;
+      if (sched) {
+        if (lane == 0) t = atomicAdd(sched, 1);
+        t = __shfl_sync(0xffffffffu, t, 0);
+      } else { t = fixed; fixed += 2 * (int)gridDim.x; }
+      if (t >= p.total) t = -1;
+      volatile TileSlot* s = slots + (n & 1);
+      int bh = 0, qt = 0, blocks = 0;
+      HeadSequence seq{};
+      if (t >= 0) {
+        // groups of heads whose keys stay in L2 together; inside a group the tiles with the longest causal prefix first
+        const int per_group = p.group_heads * p.q_tiles;
+        const int g = t / per_group, in = t - g * per_group;
+        const int heads = min(p.group_heads, p.a.B * p.a.Hq - g * p.group_heads);
+        const int rank = in / heads;
+        bh = g * p.group_heads + (in - rank * heads);
+        qt = p.q_tiles - 1 - rank;
+        const int b = bh / p.a.Hq, q0 = qt * HA_BLOCK, last = min(q0 + HA_BLOCK, p.a.Sq) - 1;
+        seq = head_sequence(p.a, b);
+        const int end = head_limit(p.a, seq, seq.first + last);
+        blocks = (max(end, 0) + HA_BLOCK - 1) / HA_BLOCK;
+        if (listed) {
+          // documents of the tile's queries: the blocks that hold their positions
+          const int lo = max(seq.first + q0, 0), hi = min(seq.first + last, p.a.Sk - 1);
+          const int2* rs = p.ranges + (int64_t)b * p.key_blocks;
+          int2 mine = make_int2(0x7fffffff, (int)0x80000000);
+          if (lo <= hi) {
+            const int2 r0 = ha_range(rs + lo / HA_BLOCK), r1 = ha_range(rs + hi / HA_BLOCK);
+            mine = make_int2(min(r0.x, r1.x), max(r0.y, r1.y));
+          }
+          int count = 0;
+          for (int i = 0; i < HA_MASK_WORDS; i++) {
+            const int j = i * 32 + lane;
+            bool visit = false, compare = false;
+            if (j < blocks) {
+              const int2 r = ha_range(rs + j);
+              visit = !ha_apart(mine, r);
+              compare = !ha_one_document(mine, r);
+            }
+            const uint32_t mv = __ballot_sync(0xffffffffu, visit), mc = __ballot_sync(0xffffffffu, compare);
+            if (lane == 0) { s->visit[i] = mv; s->compare[i] = mc; }
+            count += __popc(mv);
+            if ((i + 1) * 32 >= blocks && lane == 0) { for (int k = i + 1; k < HA_MASK_WORDS; k++) s->visit[k] = 0; }
+            if ((i + 1) * 32 >= blocks) break;
+          }
+          blocks = count;
+        }
+      }
+      if (lane == 0) {
+        s->tile = t; s->b = bh / max(p.a.Hq, 1); s->h = bh % max(p.a.Hq, 1); s->q0 = qt * HA_BLOCK; s->blocks = blocks;
+        s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
+        mbar_arrive(bar_tf + 8 * (n & 1));
+      }
+      __syncwarp();
+      if (t < 0) break;
+      if (blocks == 0) continue;
+      bool ok = true;
+      if (elect_one()) {
+        const int b = bh / p.a.Hq, h = bh - b * p.a.Hq, u = h / p.a.group;
+        // Q is free once the previous tile's last Q K^T has retired
+        if (nq > 0 && !mbar_wait(bar_qe, (nq - 1) & 1, abort_flag, status, 22)) ok = false;
+        if (ok) {
+          mbar_expect_tx(bar_qf, SM::Q_BYTES);
+#pragma unroll
+          for (int c = 0; c < DC; c++) tma_load_4d(wbase + SM::Q_OFF + c * HA_CHUNK, &tmQ, bar_qf, c * 64, qt * HA_BLOCK, h, b);
+          BlockWalk wk, wv;
+          wk.start(s, listed); wv.start(s, listed);
+          uint32_t k_c = kc, v_c = vc;
+          int jk = 0, jv = 0;
+          uint32_t idle = 0;
+          while (jk < blocks || jv < blocks) {
+            bool progress = false;
+            if (jk < blocks && (k_c == 0 || mbar_try_wait(bar_ke, (k_c - 1) & 1))) {
+              mbar_expect_tx(bar_kf, SM::KV_BYTES);
+#pragma unroll
+              for (int c = 0; c < DC; c++) tma_load_4d(wbase + SM::K_OFF + c * HA_CHUNK, &tmK, bar_kf, c * 64, wk.j * HA_BLOCK, u, b);
+              jk++; k_c++; progress = true;
+              wk.next();
+            }
+            if (jv < blocks && (v_c == 0 || mbar_try_wait(bar_ve, (v_c - 1) & 1))) {
+              mbar_expect_tx(bar_vf, SM::KV_BYTES);
+#pragma unroll
+              for (int c = 0; c < DC; c++) tma_load_4d(wbase + SM::V_OFF + c * HA_CHUNK, &tmV, bar_vf, c * 64, wv.j * HA_BLOCK, u, b);
+              jv++; v_c++; progress = true;
+              wv.next();
+            }
+            if (progress) { idle = 0; continue; }
+            if (++idle > (1u << 22)) { *abort_flag = 1; if (status) atomicCAS(status, 0, 11); ok = false; break; }
+            if (idle > 16) { if (*abort_flag) { ok = false; break; } __nanosleep(idle > 4096 ? 256 : 32); }
+          }
+        }
+        if (!ok) {
+          // the other roles stop at their next wait; let copies already in flight land before shared memory goes away
+          for (uint32_t i = 0; i < 4096; i++) __nanosleep(256);
+        }
+      }
+      __syncwarp();
+      kc += (uint32_t)blocks; vc += (uint32_t)blocks; nq++;
+      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
+    }
+  } else if (warp < 4) {
+    // ---------------------------------------------- MMA issuer ------------------------------------------------------
+    if (elect_one()) {
+      uint32_t kc = 0, vc = 0, hc = 0, nq = 0;     // score blocks issued, V blocks consumed, P V half-steps issued, tiles with work
+      const uint32_t s_tmem = tmem_base + (uint32_t)(w * 128), o_tmem = tmem_base + 256u + (uint32_t)(w * D);
+      const uint32_t qa = wbase + SM::Q_OFF, ka = wbase + SM::K_OFF, va = wbase + SM::V_OFF, pa = wbase + SM::P_OFF;
+      bool ok = true;
+      auto issue_qk = [&](bool last_of_tile) -> bool {
+        if (!mbar_wait(bar_kf, kc & 1, abort_flag, status, 13)) return false;
+        // the worker's softmax has copied the previous block's scores into registers
+        if (kc > 0 && !mbar_wait(bar_se, (kc - 1) & 1, abort_flag, status, 14)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+          const uint32_t off = (uint32_t)(k >> 2) * HA_CHUNK + (uint32_t)(k & 3) * 32;
+          umma_ss<false>(s_tmem, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), p.idesc_qk, k > 0 ? 1u : 0u);
+        }
+        tc_commit(bar_sf);
+        tc_commit(bar_ke);
+        if (last_of_tile) tc_commit(bar_qe);
+        kc++;
+        return true;
+      };
+      for (int n = 0; ok; n++) {
+        if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 23)) { ok = false; break; }
+        const int t = slots[n & 1].tile, blocks = slots[n & 1].blocks;
+        mbar_arrive(bar_te + 8 * (n & 1));
+        if (t < 0) break;
+        if (blocks == 0) continue;
+        if (!mbar_wait(bar_qf, nq & 1, abort_flag, status, 12)) { ok = false; break; }
+        if (!issue_qk(blocks == 1)) { ok = false; break; }
+        for (int it = 0; it < blocks && ok; it++) {
+          // the block's scores are in the softmax warps' registers early: the next score block goes ahead of this
+          // block's products
+          if (it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
+          if (!mbar_wait(bar_vf, vc & 1, abort_flag, status, 15)) { ok = false; break; }
+          // the previous tile's rows have been read out of the accumulator
+          if (it == 0 && nq > 0 && !mbar_wait(bar_of, (nq - 1) & 1, abort_flag, status, 24)) { ok = false; break; }
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (!mbar_wait(bar_pf, hc & 1, abort_flag, status, 16)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              // A = P (K-major: 64 keys contiguous per row); B = V (MN-major: head-dim chunks of 64 are HA_CHUNK apart)
+              const int kk = 4 * h + k;
+              umma_ss<false>(o_tmem, make_smem_desc(pa + (uint32_t)k * 32, 16, 1024), make_smem_desc(va + (uint32_t)kk * 2048, HA_CHUNK, 1024), p.idesc_pv,
+                             (it > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit(bar_pv);     // the half's weights have been read; the accumulator holds them
+            hc++;
+          }
+          if (!ok) break;
+          tc_commit(bar_ve);
+          vc++;
+        }
+        nq++;
+      }
+      // everything this thread issued must retire before TMEM is released
+      tc_commit(bar_drain);
+      mbar_wait(bar_drain, 0, abort_flag, nullptr, 0);
+    }
+  } else {
+    // ---------------------------------------------- softmax ---------------------------------------------------------
+    const int quad = warp & 3;                    // TMEM lanes [32 * quad, 32 * quad + 32): fixed by the warp's number
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
+    const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(w * 128);
+    const uint32_t o_addr = tmem_base + lane_addr + 256u + (uint32_t)(w * D);
+    const uint32_t prow_s = wbase + (uint32_t)(SM::P_OFF + row * 128);
+    const uint32_t sw = (uint32_t)(row & 7);
+    uint32_t sc = 0, hc = 0;                      // score blocks consumed, half-steps of weights published
+    bool ok = true;
+    const uint64_t mult2 = splat2(p.mult);
+    // 32 scores -> exp2, partial row sums, 16 words of 16-bit pairs
+    auto exps = [&](const uint32_t (&r)[32], uint64_t mn2, uint64_t (&ps2)[2], uint32_t (&pw)[16]) {
+#pragma unroll
+      for (int h = 0; h < 16; h++) {
+        const uint64_t x2 = fma2(pack2(r[2 * h], r[2 * h + 1]), mult2, mn2);
+        uint32_t t0, t1;
+        unpack2(x2, t0, t1);
+        const float e0 = fast_exp2(__uint_as_float(t0)), e1 = fast_exp2(__uint_as_float(t1));
+        ps2[h & 1] = add2(ps2[h & 1], pack2(__float_as_uint(e0), __float_as_uint(e1)));
+        pw[h] = ha_pack<EL>(e0, e1);
+      }
+    };
+    // chunk c (32 keys = four 16-byte pieces) of the 64-key half into the swizzled buffer of weights
+    auto store = [&](int c, const uint32_t (&pw)[16]) {
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        sts_v4(prow_s + ((((uint32_t)((c & 1) * 4 + q)) ^ sw) << 4), pw[4 * q], pw[4 * q + 1], pw[4 * q + 2], pw[4 * q + 3]);
+    };
+    auto publish = [&]() {
+      tc_fence_before();
+      fence_async_shared();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_pf);
+      hc++;
+    };
+    for (int n = 0; ok; n++) {
+      if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
+      volatile TileSlot* s = slots + (n & 1);
+      const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->q0;
+      const HeadSequence seq{s->length, s->first, s->prefix};
+      // the blocks' bits stay this warp's to read until it has walked them
+      if (!listed || t < 0 || blocks == 0) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
+      if (t < 0) break;
+      const int qrow = q0 + row, pos = seq.first + qrow;
+      const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
+      int doc = 0, end = head_limit(p.a, seq, pos);
+      if (p.a.documents) {
+        if (pos >= 0 && pos < p.a.Sk) doc = (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos);
+        else end = 0;
+      }
+      float m_used = -INFINITY, l = 0.f;
+      bool poisoned = false;
+      BlockWalk walk;
+      if (blocks > 0) walk.start(s, listed);
+      for (int it = 0; it < blocks && ok; it++) {
+        const int j = walk.j;
+        const bool compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
+        if (it + 1 < blocks) walk.next();
+        else if (listed) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
+        if (!mbar_wait(bar_sf, sc & 1, abort_flag, status, 17)) { ok = false; break; }
+        tc_fence_after();
+        // keys of this block that this row sees: [0, lim], and among them those of its document
+        const int lim = end - 1 - j * HA_BLOCK;
+        const bool need_mask = compare || __any_sync(0xffffffffu, lim < HA_BLOCK - 1);
+        uint32_t r[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; c++) tmem_ld_32x32(s_addr + (uint32_t)(c * 32), r[c]);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_se);
+        sc++;
+        if (p.cap_out > 0.f) {
+          // cap * tanh(x) = cap - 2 cap / (1 + e^2x): the error is a few 2^-23 of the cap, at any score; infinities give the cap
+          const uint64_t in2 = splat2(p.cap_in), one2 = splat2(1.f), out2 = splat2(p.cap_out), twice2 = splat2(-2.f * p.cap_out);
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              uint32_t a0, a1;
+              unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), in2), a0, a1);
+              const uint64_t d = add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), one2);
+              unpack2(d, a0, a1);
+              const uint64_t q2 = pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
+              unpack2(fma2(q2, twice2, out2), r[c][2 * i], r[c][2 * i + 1]);
+            }
+        } else if (p.scaled) {
+          const uint64_t in2 = splat2(p.cap_in);
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), in2), r[c][2 * i], r[c][2 * i + 1]);
+        }
+        if (p.a.slopes) {
+          const float far = (float)(pos - j * HA_BLOCK);
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 32; i++) r[c][i] = __float_as_uint(fmaf(fabsf(far - (float)(c * 32 + i)), -slope, __uint_as_float(r[c][i])));
+        }
+        if (need_mask) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            uint32_t bits = ha_bits(lim - c * 32);
+            if (compare) {
+              const int key = j * HA_BLOCK + c * 32 + lane;
+              const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + key) : 0;
+              bits &= ha_same_document(doc, theirs, key < p.a.Sk);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i++) if (!((bits >> i) & 1u)) r[c][i] = 0xff800000u;
+          }
+        }
+        float mx;
+        {
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) mx4[i & 3] = max3(mx4[i & 3], __uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
+          mx = max3(mx4[0], mx4[1], max3(mx4[2], mx4[3], -INFINITY));
+        }
+        // a NaN score makes the whole row NaN; keep the arithmetic finite and poison the row sum at the end
+        if (mx != mx) { poisoned = true; mx = 0.f; }
+        float alpha = 1.f;
+        bool rescale = false;
+        if (it == 0) m_used = mx;
+        else if ((mx - m_used) * p.mult > 8.0f) { alpha = fast_exp2((m_used - mx) * p.mult); l *= alpha; m_used = mx; rescale = true; }
+        if (it > 0) {
+          // the previous block's second half-product has retired: the buffer of weights is free and the accumulator at rest
+          if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) { ok = false; break; }
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+            for (int c = 0; c < D / 16; c++) {
+              uint32_t o[16];
+              tmem_ld_32x16(o_addr + (uint32_t)(c * 16), o);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x16(o_addr + (uint32_t)(c * 16), o);
+            }
+            tc_wait_st();
+          }
+        }
+        if (p.a.lengths && seq.length < p.a.Sk && seq.length < (j + 1) * HA_BLOCK) {
+          // values behind the sequence's end: zero before they meet their weights of zero
+          if (!mbar_wait(bar_vf, (sc - 1) & 1, abort_flag, status, 26)) { ok = false; break; }
+          if (j * HA_BLOCK + row >= seq.length) {
+#pragma unroll 1
+            for (int c = 0; c < DC; c++)
+#pragma unroll
+              for (int q = 0; q < 8; q++) sts_v4(wbase + (uint32_t)(SM::V_OFF + c * HA_CHUNK + row * 128 + q * 16), 0, 0, 0, 0);
+          }
+        }
+        const float mneg = (m_used == -INFINITY) ? 0.f : -m_used * p.mult;
+        const uint64_t mn2 = splat2(mneg);
+        uint64_t ps2[2] = {0ull, 0ull};
+        {
+          uint32_t pw[16];
+          exps(r[0], mn2, ps2, pw); store(0, pw);
+          exps(r[1], mn2, ps2, pw); store(1, pw);
+        }
+        publish();
+        {
+          // the second half: its first 32 keys are exponentiated while the first half multiplies
+          uint32_t pw[16];
+          exps(r[2], mn2, ps2, pw);
+          if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
+          store(0, pw);
+          exps(r[3], mn2, ps2, pw); store(1, pw);
+        }
+        publish();
+        {
+          uint32_t a0, a1, b0, b1;
+          unpack2(ps2[0], a0, a1); unpack2(ps2[1], b0, b1);
+          l += (__uint_as_float(a0) + __uint_as_float(a1)) + (__uint_as_float(b0) + __uint_as_float(b1));
+        }
+      }
+      if (!ok) break;
+      // ---- the tile's last product has retired: normalise and write the rows ----
+      if (blocks > 0) {
+        if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 20)) { ok = false; break; }
+        tc_fence_after();
+      }
+      if (poisoned) l = __int_as_float(0x7fc00000);
+      const float inv = !(l <= 0.f) ? 1.0f / l : 0.f;   // a NaN sum stays NaN
+      char* orow = p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)h * p.a.os.head + (int64_t)qrow * p.a.os.token);
+#pragma unroll 1
+      for (int c = 0; c < D / 16; c++) {
+        uint32_t x[16];
+        if (blocks > 0) {
+          tmem_ld_32x16(o_addr + (uint32_t)(c * 16), x);
+          tc_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i++) x[i] = 0;
+        }
+        if (qrow < p.a.Sq) {
+#pragma unroll
+          for (int q = 0; q < 2; q++) {
+            uint32_t wd[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              // a row that sees nothing is 0, whatever weights of zero were multiplied with
+              const float f0 = inv == 0.f ? 0.f : __uint_as_float(x[q * 8 + 2 * k]) * inv, f1 = inv == 0.f ? 0.f : __uint_as_float(x[q * 8 + 2 * k + 1]) * inv;
+              wd[k] = ha_pack<EL>(f0, f1);
+            }
+            if (c * 16 + q * 8 < p.a.D) *reinterpret_cast<uint4*>(orow + 2 * (c * 16 + q * 8)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
+          }
+        }
+      }
+      if (p.a.lse && qrow < p.a.Sq)
+        p.a.lse[((int64_t)b * p.a.Hq + h) * p.a.Sq + qrow] = l == 0.f ? -INFINITY : (m_used * p.mult + fast_log2(l)) * 0.6931471805599453f;
+      tc_fence_before();
+      __syncwarp();
+      if (blocks > 0 && lane == 0) mbar_arrive(bar_of);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, TMEM_COLS); }
+  // the last CTA to leave puts the tile counter back for the stream's next launch
+  if (sched && threadIdx.x == 0 && atomicAdd(sched + 1, 1) == (int)gridDim.x - 1) { sched[0] = 0; sched[1] = 0; __threadfence(); }
+}
+
+// One warp per block of 128 tokens
+__global__ void __launch_bounds__(256) k_document_ranges(const int32_t* documents, int2* ranges, int32_t B, int32_t Sk, int32_t blocks) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (id < (int64_t)B * blocks) {
+    const int b = (int)(id / blocks), j = (int)(id - (int64_t)b * blocks);
+    int lo = 0x7fffffff, hi = (int)0x80000000;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const int t = j * HA_BLOCK + i * 32 + lane;
+      if (t < Sk) { const int d = (int)ld_global((const uint32_t*)documents + (int64_t)b * Sk + t); lo = min(lo, d); hi = max(hi, d); }
+    }
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) ranges[id] = make_int2(lo, hi);
+  }
+}
+
+template <int D, int EL>
+int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileParams& p, int32_t* sched, int32_t* status, cudaStream_t stream) {
+  using SM = TileSmem<D>;
+  auto kern = k_head_attention<D, EL>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static std::atomic<bool> configured[64];
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  const int ctas = (p.total + 1) / 2 < kNumSms ? (p.total + 1) / 2 : kNumSms;
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)ctas), dim3(384), SM::TOTAL, stream, q, k, v, p, sched, status);
+  if (e != cudaSuccess) return (int)e;
+  count_launch();
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream) {
+  const int blocks = (p.Sk + HA_BLOCK - 1) / HA_BLOCK;
+  const int64_t n = (int64_t)p.B * blocks;
+  if (n == 0) return 0;
+  const cudaError_t e = launch_overlapped(k_document_ranges, dim3((unsigned)((n + 7) / 8)), dim3(256), 0, stream, p.documents, ranges, p.B, p.Sk, blocks);
+  if (e != cudaSuccess) return (int)e;
+  count_launch();
+  return (int)cudaGetLastError();
+}
+
+int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status, cudaStream_t stream) {
+  TileParams p{};
+  p.a = a;
+  p.q_tiles = (a.Sq + HA_BLOCK - 1) / HA_BLOCK;
+  p.key_blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
+  const int64_t total = (int64_t)a.B * a.Hq * p.q_tiles;
+  if (total == 0) return 0;
+  if (total > 0x7fffff00) return (int)cudaErrorInvalidValue;
+  p.total = (int)total;
+  if (a.documents) {
+    const int rc = ha_launch_ranges(a, ranges, stream);
+    if (rc) return rc;
+  }
+  // longer sequences than a skip list covers walk all their blocks, and compare in each
+  p.ranges = a.documents && p.key_blocks <= HA_MASK_WORDS * 32 ? ranges : nullptr;
+  const int64_t kv_heads = (32ll << 20) / ((int64_t)(a.Sk > 0 ? a.Sk : 1) * a.D * 4);
+  const int64_t heads = kv_heads < 1 ? a.group : kv_heads * a.group;
+  p.group_heads = (int)(heads > (int64_t)a.B * a.Hq ? (int64_t)a.B * a.Hq : heads);
+  p.scaled = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
+  p.mult = p.scaled ? 1.0f : a.scale * kLog2e;
+  p.cap_in = a.softcap > 0.f ? 2.0f * a.scale / a.softcap * kLog2e : a.scale * kLog2e;
+  p.cap_out = a.softcap > 0.f ? a.softcap * kLog2e : 0.f;
+  const int D = a.D <= 64 ? 64 : 128;
+  const uint32_t format = elem == EL_BF16 ? 1u : 0u;
+  p.idesc_qk = sm100::make_idesc(format, false, false, HA_BLOCK, HA_BLOCK);
+  p.idesc_pv = sm100::make_idesc(format, false, true, HA_BLOCK, (uint32_t)D);
+  CUtensorMap q, k, v;
+  if (!ha_encode(&q, elem, a.q, a.qs, a.B, a.Hq, a.Sq, a.D)) return (int)cudaErrorInvalidValue;
+  if (a.Sk == 0) k = v = q;      // nothing is loaded
+  else if (!ha_encode(&k, elem, a.k, a.ks, a.B, a.Hk, a.Sk, a.D) || !ha_encode(&v, elem, a.v, a.vs, a.B, a.Hk, a.Sk, a.D)) return (int)cudaErrorInvalidValue;
+  int32_t* sched = sched_slot(stream);
+  if (D == 64) return elem == EL_BF16 ? launch_tiles<64, EL_BF16>(q, k, v, p, sched, status, stream) : launch_tiles<64, EL_F16>(q, k, v, p, sched, status, stream);
+  return elem == EL_BF16 ? launch_tiles<128, EL_BF16>(q, k, v, p, sched, status, stream) : launch_tiles<128, EL_F16>(q, k, v, p, sched, status, stream);
+}
+
+}  // namespace b2x

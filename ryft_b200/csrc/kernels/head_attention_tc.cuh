@@ -1,0 +1,81 @@
+// What the tensor-core kernels of head_attention share: tensor maps over tensors of heads, the ranges of document numbers that
+// let whole blocks be skipped, and masks as bits.
+#pragma once
+#include "attention_math.cuh"
+#include "head_attention.cuh"
+#include "sm100.cuh"
+
+namespace b2x {
+
+constexpr int HA_BLOCK = 128;                 // queries of a tile, keys of a block
+constexpr int HA_MASK_WORDS = 32;             // blocks that a tile's skip list covers: 1024, 131072 tokens
+constexpr uint32_t HA_CHUNK = 128 * 128;      // one [128 rows x 128 bytes] swizzled sub-tile
+
+// Two f32 as one word of 16-bit values, `lo` in the lower half.
+template <int EL> __device__ __forceinline__ uint32_t ha_pack(float lo, float hi) {
+  if constexpr (EL == EL_BF16) { __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&t); }
+  else { __half2 t = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&t); }
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Keys 0..31 of a chunk that lie at or below `lim` (relative to the chunk's first key).
+__device__ __forceinline__ uint32_t ha_bits(int lim) { return lim >= 31 ? 0xffffffffu : lim < 0 ? 0u : (2u << lim) - 1u; }
+
+// Which of 32 keys lie in the lane's document: lane l holds key l's (`key`; `there` says whether there is such a key).  The lanes
+// of a warp are neighbouring queries (or keys), so the loop over their distinct documents is short.
+__device__ __forceinline__ uint32_t ha_same_document(int mine, int key, bool there) {
+  uint32_t todo = 0xffffffffu, bits = 0;
+  const uint32_t valid = __ballot_sync(0xffffffffu, there);
+  while (todo) {
+    const int d = __shfl_sync(0xffffffffu, mine, __ffs(todo) - 1);
+    const uint32_t b = __ballot_sync(0xffffffffu, key == d) & valid;
+    const bool hit = mine == d;
+    if (hit) bits = b;
+    todo &= ~__ballot_sync(0xffffffffu, hit);
+  }
+  return bits;
+}
+
+// Smallest and largest document of every block of 128 tokens: one warp per block.  [B][blocks]
+__device__ __forceinline__ bool ha_apart(int2 a, int2 b) { return a.y < b.x || b.y < a.x; }
+__device__ __forceinline__ bool ha_one_document(int2 a, int2 b) { return a.x == a.y && b.x == b.y && a.x == b.x; }
+__device__ __forceinline__ int2 ha_range(const int2* r) {
+  const uint2 v = ld_global((const uint2*)r);
+  return make_int2((int)v.x, (int)v.y);
+}
+
+// 4-D tensor map (width, tokens, heads, sequences) with a box of 64 elements x 128 tokens; elements behind the width read as 0.
+inline bool ha_encode(CUtensorMap* m, int elem, const void* base, const B2xHeadStrides& s, int64_t B, int64_t H, int64_t S, int64_t D) {
+  PFN_encodeTiled fn = get_encode_tiled();
+  if (!fn || ((uintptr_t)base & 15) != 0) return false;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
+  // the stride of a dimension of one is never used, but has to be a legal one
+  int64_t st = S > 1 ? s.token : D, sh = H > 1 ? s.head : D, sb = B > 1 ? s.batch : D;
+  if (st % 8 != 0 || sh % 8 != 0 || sb % 8 != 0 || st <= 0 || sh <= 0 || sb <= 0) return false;
+  cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
+  cuuint32_t box[4] = {64, HA_BLOCK, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return fn(m, elem == EL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int32_t* sched_slot(cudaStream_t stream);   // gemm_tc.cu: a (tile counter, finished CTAs) pair per stream
+
+// Blocks of 128 tokens and the launches of the entry points.
+int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream);
+int ha_launch_forward(const HeadAttn& p, int elem, int2* ranges, int32_t* status, cudaStream_t stream);
+
+}  // namespace b2x

@@ -470,6 +470,7 @@ extern "C" int b2x_launch_rotary_gradient(const B2xRotaryArgs* a, b2x_stream_t s
     if (p.warps == 0) return 0;
     return launch_rot(a, p, V, false, (cudaStream_t)stream);
   }
+  if (!a->scratch) return (int)cudaErrorInvalidValue;
   p.partial = (float*)a->scratch;
   const int rows = p.tokens > 0 ? rot_gradient_ctas(p) : 0;
   if (rows > 0) {

@@ -5,6 +5,9 @@
 
 namespace b2x {
 
+// For questions about sizes before there is memory: operands that are there are not NULL, as at a launch.
+inline void* bind_nowhere(const BufRef& b) { return b.valid() ? (void*)16 : nullptr; }
+
 inline B2xHeadStrides head_strides(const Step::CallTensor& t) { return B2xHeadStrides{t.batch, t.head, t.token}; }
 
 template <typename Bind>

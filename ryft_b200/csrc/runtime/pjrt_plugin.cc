@@ -1321,9 +1321,8 @@ static int step_kernel_launches(const Step& s) {
     case StepKind::ATTENTION: return 1;
     case StepKind::SOFTMAX: return 1;
     case StepKind::CALL: {
-      const auto nowhere = [](const BufRef&) -> void* { return nullptr; };
-      if (s.call->kind == CallKind::ROTARY) { const B2xRotaryArgs a = rotary_args(s, nowhere); return b2x_rotary_launches(&a, s.call->rotary.gradient); }
-      const B2xHeadAttentionArgs a = head_attention_args(s, nowhere);
+      if (s.call->kind == CallKind::ROTARY) { const B2xRotaryArgs a = rotary_args(s, bind_nowhere); return b2x_rotary_launches(&a, s.call->rotary.gradient); }
+      const B2xHeadAttentionArgs a = head_attention_args(s, bind_nowhere);
       return b2x_head_attention_launches(&a, s.call->attention.gradient);
     }
     default: return 0;

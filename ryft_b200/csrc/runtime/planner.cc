@@ -1618,11 +1618,11 @@ void Planner::emit_call(const Op& op) {
     s.call_table.offset = ((int64_t)plan_.const_pool.size() + 255) / 256 * 256;
     plan_.const_pool.resize((size_t)s.call_table.offset + std::max<size_t>(turns.size(), 1) * 8);
     if (!turns.empty()) memcpy(plan_.const_pool.data() + s.call_table.offset, turns.data(), turns.size() * 8);
-    const B2xRotaryArgs a = rotary_args(s, [](const BufRef&) -> void* { return nullptr; });
+    const B2xRotaryArgs a = rotary_args(s, bind_nowhere);
     s.scratch_bytes = spec->rotary.gradient ? b2x_rotary_scratch_bytes(&a) : 0;
   } else {
     const AttentionSpec& at = spec->attention;
-    const B2xHeadAttentionArgs a = head_attention_args(s, [](const BufRef&) -> void* { return nullptr; });
+    const B2xHeadAttentionArgs a = head_attention_args(s, bind_nowhere);
     s.scratch_bytes = b2x_head_attention_scratch_bytes(&a, at.gradient ? 1 : 0);
     // what the masks of the attributes leave; documents, prefixes and lengths are known at run time only
     double pairs = (double)at.Sq * (double)at.Sk;

@@ -32,6 +32,15 @@ def test_a_call_is_one_step_and_its_operands_stay_where_they_are():
     assert "1 steps" in dump and "call b2x.attention" in dump
 
 
+def test_scratch_covers_what_the_operands_ask_for():
+    # ranges of document numbers, 8 bytes per 128 keys; the gradient's delta, 4 bytes per query and head
+    call = lambda b: dict(documents=b.arg([2, 300], "i32"), causal=True)  # noqa: E731
+    dump = plan(lambda b: [b.attention(*[heads(b, S=300) for _ in range(3)], **call(b))])
+    assert "scratch=48 B" in dump
+    dump = plan(lambda b: [b.attention(*[heads(b, S=300) for _ in range(3)], causal=True)])
+    assert "scratch=0 B" in dump
+
+
 def test_rows_that_are_not_contiguous_are_copied():
     dump = plan(lambda b: b.rotary([b.transpose(b.arg([2, 4, 64, 8], "bf16"), [0, 1, 3, 2])]))
     assert "copy:call_operand" in dump and "2 steps" in dump
