@@ -19,7 +19,6 @@ struct HeadAttn {
   float* lse;
   const char* dout;
   char* dq; char* dk; char* dv;
-  float* delta;
   int32_t B, Hq, Hk, group, Sq, Sk, D;
   int32_t offset;              // position of the first query, without queries_at_end
   float scale, softcap;

@@ -31,17 +31,6 @@ struct TileParams {
   uint32_t idesc_qk, idesc_pv;
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-// A tile as its loading warp publishes it.
-struct TileSlot {
-  int tile;                    // -1: no more
-  int b, h, q0;
-  int blocks;                  // key blocks to walk
-  int length, first, prefix;   // HeadSequence
-  uint32_t visit[HA_MASK_WORDS], compare[HA_MASK_WORDS];   // with documents: blocks to walk, and those whose documents have to be compared
-};
-
 template <int D> struct TileSmem {
   static constexpr int Q_BYTES = HA_BLOCK * D * 2;
   static constexpr int KV_BYTES = HA_BLOCK * D * 2;
@@ -54,22 +43,6 @@ template <int D> struct TileSmem {
   static constexpr int BAR_OFF = 2 * W_BYTES;              // 2 x 16 barriers, TMEM slot, abort flag
   static constexpr int SLOT_OFF = BAR_OFF + 288;
   static constexpr int TOTAL = SLOT_OFF + 4 * (int)sizeof(TileSlot) + 1024;
-};
-
-// A tile's blocks in their order: all from 0, or those whose bits are set
-struct BlockWalk {
-  const volatile TileSlot* s;
-  int j;
-  bool listed;
-  __device__ __forceinline__ void start(const volatile TileSlot* slot, bool list) { s = slot; listed = list; j = -1; next(); }
-  __device__ __forceinline__ void next() {
-    j++;
-    if (!listed) return;
-    int w = j >> 5;
-    uint32_t m = w < HA_MASK_WORDS ? s->visit[w] & (0xffffffffu << (j & 31)) : 0u;
-    while (m == 0 && ++w < HA_MASK_WORDS) m = s->visit[w];
-    j = m ? w * 32 + __ffs(m) - 1 : HA_MASK_WORDS * 32;
-  }
 };
 
 template <int D, int EL>
@@ -174,7 +147,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       if (lane == 0) {
-        s->tile = t; s->b = bh / max(p.a.Hq, 1); s->h = bh % max(p.a.Hq, 1); s->q0 = qt * HA_BLOCK; s->blocks = blocks;
+        s->tile = t; s->b = bh / max(p.a.Hq, 1); s->h = bh % max(p.a.Hq, 1); s->at = qt * HA_BLOCK; s->begin = 0; s->blocks = blocks;
         s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
         mbar_arrive(bar_tf + 8 * (n & 1));
       }
@@ -327,7 +300,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int n = 0; ok; n++) {
       if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
-      const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->q0;
+      const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
       // the blocks' bits stay this warp's to read until it has walked them
       if (!listed || t < 0 || blocks == 0) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }

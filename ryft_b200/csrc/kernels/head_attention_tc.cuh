@@ -58,8 +58,8 @@ __device__ __forceinline__ int2 ha_range(const int2* r) {
   return make_int2((int)v.x, (int)v.y);
 }
 
-// 4-D tensor map (width, tokens, heads, sequences) with a box of 64 elements x 128 tokens; elements behind the width read as 0.
-inline bool ha_encode(CUtensorMap* m, int elem, const void* base, const B2xHeadStrides& s, int64_t B, int64_t H, int64_t S, int64_t D) {
+// 4-D tensor map (width, tokens, heads, sequences) with a box of 64 elements x `rows` tokens; elements behind the width read as 0.
+inline bool ha_encode(CUtensorMap* m, int elem, const void* base, const B2xHeadStrides& s, int64_t B, int64_t H, int64_t S, int64_t D, uint32_t rows = HA_BLOCK) {
   PFN_encodeTiled fn = get_encode_tiled();
   if (!fn || ((uintptr_t)base & 15) != 0) return false;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)H, (cuuint64_t)B};
@@ -67,15 +67,45 @@ inline bool ha_encode(CUtensorMap* m, int elem, const void* base, const B2xHeadS
   int64_t st = S > 1 ? s.token : D, sh = H > 1 ? s.head : D, sb = B > 1 ? s.batch : D;
   if (st % 8 != 0 || sh % 8 != 0 || sb % 8 != 0 || st <= 0 || sh <= 0 || sb <= 0) return false;
   cuuint64_t strides[3] = {(cuuint64_t)st * 2, (cuuint64_t)sh * 2, (cuuint64_t)sb * 2};
-  cuuint32_t box[4] = {64, HA_BLOCK, 1, 1}, estr[4] = {1, 1, 1, 1};
+  cuuint32_t box[4] = {64, rows, 1, 1}, estr[4] = {1, 1, 1, 1};
   return fn(m, elem == EL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A tile as its loading warp publishes it.
+struct TileSlot {
+  int tile;                    // -1: no more
+  int b, h, at;                // sequence, head, first query (or key) of the tile
+  int begin, blocks;           // first block to walk, and how many
+  int length, first, prefix;   // HeadSequence
+  uint32_t visit[HA_MASK_WORDS], compare[HA_MASK_WORDS];   // with documents: blocks to walk, and those whose documents have to be compared
+};
+
+// A tile's blocks in their order: all from `begin`, or those whose bits are set
+struct BlockWalk {
+  const volatile TileSlot* s;
+  int j;
+  bool listed;
+  __device__ __forceinline__ void start(const volatile TileSlot* slot, bool list) { s = slot; listed = list; j = slot->begin - 1; next(); }
+  __device__ __forceinline__ void next() {
+    j++;
+    if (!listed) return;
+    int w = j >> 5;
+    uint32_t m = w < HA_MASK_WORDS ? s->visit[w] & (0xffffffffu << (j & 31)) : 0u;
+    while (m == 0 && ++w < HA_MASK_WORDS) m = s->visit[w];
+    j = m ? w * 32 + __ffs(m) - 1 : HA_MASK_WORDS * 32;
+  }
+};
+
 
 int32_t* sched_slot(cudaStream_t stream);   // gemm_tc.cu: a (tile counter, finished CTAs) pair per stream
 
 // Blocks of 128 tokens and the launches of the entry points.
 int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream);
+int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a);
+int ha_launch_gradient(const HeadAttn& p, int elem, void* scratch, int32_t* status, cudaStream_t stream);
 int ha_launch_forward(const HeadAttn& p, int elem, int2* ranges, int32_t* status, cudaStream_t stream);
 
 }  // namespace b2x
