@@ -161,7 +161,7 @@ AttentionSpec describe_attention(Reader& r, bool gradient) {
   s.queries_at_end = r.flag("queries_at_end");
   s.query_offset = r.integer("query_offset", 0);
   s.softcap = r.number("softcap", 0.0);
-  r.need(s.softcap >= 0.0, "softcap must not be negative");
+  r.need(s.softcap == 0.0 || (s.softcap >= 1e-6 && s.softcap <= 1e6), "softcap must be 0 (none) or lie in [1e-6, 1e6]");
   const std::vector<std::string> extra = r.words("inputs");
   const size_t fixed = gradient ? 6 : 3;
   r.need(op.operands.size() == fixed + extra.size(), "expects " + std::to_string(fixed) + " operands and those that `inputs` names");
@@ -200,6 +200,7 @@ AttentionSpec describe_attention(Reader& r, bool gradient) {
     if (s.log_sum) r.same(r.out(1), sums, "the log sums");
   }
   s.scale = r.number("scale", s.D > 0 ? 1.0 / std::sqrt((double)s.D) : 1.0);
+  r.need(std::fabs(s.scale) <= 1e6, "scale must lie in [-1e6, 1e6]");
   if (s.slopes >= 0) r.same(r.in(s.slopes), type_of(DType::F32, {s.Hq}), "the slopes");
   if (s.documents >= 0) r.same(r.in(s.documents), type_of(DType::S32, {s.B, s.Sk}), "the documents");
   if (s.prefix >= 0) r.same(r.in(s.prefix), type_of(DType::S32, {s.B}), "the prefix");

@@ -18,7 +18,8 @@ bool ha_rows(const void* p, const B2xHeadStrides& s, int64_t B, int64_t H, int64
 }
 bool ha_valid(const B2xHeadAttentionArgs* a) {
   return ha_rows(a->q, a->qs, a->B, a->Hq, a->Sq) && ha_rows(a->k, a->ks, a->B, a->Hk, a->Sk) && ha_rows(a->v, a->vs, a->B, a->Hk, a->Sk) &&
-         ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && (!a->lse || a->B * a->Hq * a->Sq < (1ll << 40)) && (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 && (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) &&
+         ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 &&
+         (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) && (a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e6f)) && std::fabs(a->scale) <= 1e6f &&
          a->Sq < (1ll << 30) && a->Sk < (1ll << 30) && a->query_offset >= 0 && a->query_offset < (1ll << 30) && (!a->queries_at_end || a->lengths);
 }
 

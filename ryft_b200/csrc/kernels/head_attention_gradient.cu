@@ -32,7 +32,8 @@ struct GradParams {
   const float* neg_delta;             // [B, Hq, rows]
   int32_t rows;                       // queries, rounded up to 128
   int32_t tiles, group_heads, key_blocks, total;
-  float in, cap;                      // scores times `in`: log2 units, or with a cap the exponent of tanh; cap in log2 units
+  float in;                           // scale * log2(e)
+  HeadCap cap;
   float scale;
   uint32_t idesc_s, idesc_acc;
 };
@@ -45,32 +46,34 @@ __device__ __forceinline__ int2 grad_range(const GradParams& p, const int2* rs, 
   return make_int2(min(a.x, b.x), max(a.y, b.y));
 }
 
-// P and dS of 32 scores of a row.  nl and nd are the row constants of the pair 2i, 2i + 1 (nl carries the cap, too).
-template <int EL, typename L, typename N>
+// P and dS of 32 scores of a row.  nl and nd are the row constants of the pair 2i, 2i + 1.  CAP: 0 none, 1 by the polynomial, 2 any.
+template <int EL, int CAP, typename L, typename N>
 __device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[32], const uint32_t (&dp)[32], const L& nl, const N& nd, float slope, float far,
                                            uint32_t bits, bool masked, uint32_t (&pw)[16], uint32_t (&dw)[16]) {
-  const uint64_t in2 = splat2(p.in), one2 = splat2(1.f), twice2 = splat2(-2.f * p.cap), minus2 = splat2(-1.f), four2 = splat2(4.f);
+  const uint64_t one2 = splat2(1.f);
 #pragma unroll
   for (int i = 0; i < 16; i++) {
     uint64_t x2, bend2 = 0;
     const uint64_t s2 = pack2(s[2 * i], s[2 * i + 1]);
     uint32_t a0, a1;
-    if (p.cap > 0.f) {
-      // cap * tanh = cap - 2 cap q with q = 1 / (1 + e^2x); its derivative 1 - tanh^2 = 4 q (1 - q)
-      unpack2(mul2(s2, in2), a0, a1);
-      unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), one2), a0, a1);
-      const uint64_t q2 = pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
-      x2 = fma2(q2, twice2, nl(i));
-      bend2 = mul2(mul2(q2, four2), fma2(q2, minus2, one2));
+    if constexpr (CAP == 1) {
+      const uint64_t t2 = cap_small(p.cap, s2);
+      bend2 = fma2(mul2(t2, t2), splat2(p.cap.back), one2);
+      x2 = add2(t2, nl(i));
+    } else if constexpr (CAP == 2) {
+      // cap * tanh = cap - 2 cap q; its derivative 1 - tanh^2 = 4 q (1 - q)
+      const uint64_t q2 = cap_rest(p.cap, s2);
+      bend2 = mul2(mul2(q2, splat2(4.f)), fma2(q2, splat2(-1.f), one2));
+      x2 = add2(fma2(q2, splat2(-2.f * p.cap.cap), splat2(p.cap.cap)), nl(i));
     } else {
-      x2 = fma2(s2, in2, nl(i));
+      x2 = fma2(s2, splat2(p.in), nl(i));
     }
     unpack2(x2, a0, a1);
     float x0 = __uint_as_float(a0), x1 = __uint_as_float(a1);
     if (slope != 0.f) { x0 = fmaf(fabsf(far - (float)(2 * i)), -slope, x0); x1 = fmaf(fabsf(far - (float)(2 * i + 1)), -slope, x1); }
     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
     uint64_t d2 = mul2(pack2(__float_as_uint(p0), __float_as_uint(p1)), add2(pack2(dp[2 * i], dp[2 * i + 1]), nd(i)));
-    if (p.cap > 0.f) d2 = mul2(d2, bend2);
+    if constexpr (CAP != 0) d2 = mul2(d2, bend2);
     unpack2(d2, a0, a1);
     pw[i] = ha_pack<EL>(p0, p1);
     dw[i] = ha_pack<EL>(__uint_as_float(a0), __uint_as_float(a1));
@@ -79,6 +82,16 @@ __device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (
       const uint32_t keep = ((bits >> (2 * i)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
       pw[i] &= keep; dw[i] &= keep;
     }
+  }
+}
+template <int EL, typename L, typename N>
+__device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[32], const uint32_t (&dp)[32], const L& nl, const N& nd, float slope, float far,
+                                           uint32_t bits, bool masked, uint32_t (&pw)[16], uint32_t (&dw)[16]) {
+  if (p.cap.cap > 0.f) {
+    if (__all_sync(0xffffffffu, ha_largest(s) <= p.cap.small)) grad_words<EL, 1>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
+    else grad_words<EL, 2>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
+  } else {
+    grad_words<EL, 0>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
   }
 }
 
@@ -316,7 +329,7 @@ k_attention_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
       if (t < 0) break;
       const int qrow = q0 + row, pos = seq.first + qrow;
       const int64_t at = ((int64_t)b * p.a.Hq + h) * p.rows + qrow;
-      const uint64_t nl2 = splat2(ld_global(p.neg_lse + at) + p.cap), nd2 = splat2(ld_global(p.neg_delta + at));
+      const uint64_t nl2 = splat2(ld_global(p.neg_lse + at)), nd2 = splat2(ld_global(p.neg_delta + at));
       const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
       int doc = 0, end = head_limit(p.a, seq, pos);
       if (p.a.documents) {
@@ -625,7 +638,7 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       // a unit's row constants: one value per thread, fetched a unit ahead
       auto fetch = [&](int h, int unit) {
         const int64_t at = ((int64_t)b * p.a.Hq + u * p.a.group + h) * p.rows + unit * DKV_UNIT + (tid & 63);
-        return tid < 64 ? ld_global(p.neg_lse + at) + p.cap : ld_global(p.neg_delta + at);
+        return tid < 64 ? ld_global(p.neg_lse + at) : ld_global(p.neg_delta + at);
       };
       auto advance = [&]() {                       // to the next unit, over the end of a head
         if (++it == units) { it = 0; hh++; if (hh < p.a.group) walk.start(s, listed); }
@@ -828,8 +841,8 @@ int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* stat
   int2* ranges = (int2*)(p.neg_delta + n);
   p.key_blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
   p.scale = a.scale;
-  p.in = a.softcap > 0.f ? 2.0f * a.scale / a.softcap * kLog2e : a.scale * kLog2e;
-  p.cap = a.softcap > 0.f ? a.softcap * kLog2e : 0.f;
+  p.in = a.scale * kLog2e;
+  p.cap = ha_cap(a.softcap, a.scale);
   if (a.documents) {
     const int rc = ha_launch_ranges(a, ranges, stream);
     if (rc) return rc;

@@ -26,7 +26,8 @@ struct TileParams {
   const int2* ranges;          // documents' ranges per block, [B][key blocks]
   int32_t q_tiles, group_heads, key_blocks, total;
   float mult;                  // scores in registers times this are log2 units: scale * log2(e), or 1 where cap or bias made them so
-  float cap_in, cap_out;       // exponent 2 * scale / cap * log2(e), cap * log2(e); without a cap scale * log2(e), 0
+  float in;                    // scale * log2(e)
+  HeadCap cap;
   int32_t scaled;              // scores are brought to log2 units before anything else (bias; scale not positive)
   uint32_t idesc_qk, idesc_pv;
 };
@@ -334,22 +335,22 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_se);
         sc++;
-        if (p.cap_out > 0.f) {
-          // cap * tanh(x) = cap - 2 cap / (1 + e^2x): the error is a few 2^-23 of the cap, at any score; infinities give the cap
-          const uint64_t in2 = splat2(p.cap_in), one2 = splat2(1.f), out2 = splat2(p.cap_out), twice2 = splat2(-2.f * p.cap_out);
+        if (p.cap.cap > 0.f) {
+          const float largest = max3(max3(ha_largest(r[0]), ha_largest(r[1]), 0.f), ha_largest(r[2]), ha_largest(r[3]));
+          if (__all_sync(0xffffffffu, largest <= p.cap.small)) {
 #pragma unroll
-          for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              uint32_t a0, a1;
-              unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), in2), a0, a1);
-              const uint64_t d = add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), one2);
-              unpack2(d, a0, a1);
-              const uint64_t q2 = pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
-              unpack2(fma2(q2, twice2, out2), r[c][2 * i], r[c][2 * i + 1]);
-            }
+              for (int i = 0; i < 16; i++) unpack2(cap_small(p.cap, pack2(r[c][2 * i], r[c][2 * i + 1])), r[c][2 * i], r[c][2 * i + 1]);
+          } else {
+            const uint64_t out2 = splat2(p.cap.cap), twice2 = splat2(-2.f * p.cap.cap);
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 16; i++) unpack2(fma2(cap_rest(p.cap, pack2(r[c][2 * i], r[c][2 * i + 1])), twice2, out2), r[c][2 * i], r[c][2 * i + 1]);
+          }
         } else if (p.scaled) {
-          const uint64_t in2 = splat2(p.cap_in);
+          const uint64_t in2 = splat2(p.in);
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -560,8 +561,8 @@ int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status
   p.group_heads = (int)(heads > (int64_t)a.B * a.Hq ? (int64_t)a.B * a.Hq : heads);
   p.scaled = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
   p.mult = p.scaled ? 1.0f : a.scale * kLog2e;
-  p.cap_in = a.softcap > 0.f ? 2.0f * a.scale / a.softcap * kLog2e : a.scale * kLog2e;
-  p.cap_out = a.softcap > 0.f ? a.softcap * kLog2e : 0.f;
+  p.in = a.scale * kLog2e;
+  p.cap = ha_cap(a.softcap, a.scale);
   const int D = a.D <= 64 ? 64 : 128;
   const uint32_t format = elem == EL_BF16 ? 1u : 0u;
   p.idesc_qk = sm100::make_idesc(format, false, false, HA_BLOCK, HA_BLOCK);

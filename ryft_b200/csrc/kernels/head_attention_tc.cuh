@@ -74,6 +74,54 @@ inline bool ha_encode(CUtensorMap* m, int elem, const void* base, const B2xHeadS
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// softcap * tanh(x) in log2 units, x = scale / softcap times the product.  Two ways:
+//   |x| <= 0.75 (scores up to 0.75 caps, the usual case): an odd polynomial of degree 9, the minimax fit of tanh(x) / x in x^2
+//     (exchange algorithm of Remez, relative error 6e-7), seven packed instructions for two scores on the FMA pipe;
+//   else: cap - 2 cap q with q = 1 / (1 + e^2x), two special-function instructions per score, right for any score and infinity.
+// The special-function pipe does 16 a clock and SM and has the softmax's exponential to do for every score as it is: with the
+// second way alone a block of 128 x 128 keeps it busy for 3072 cycles where the tensor pipe needs 1024.
+struct HeadCap {
+  float cap;                   // cap * log2(e); 0: none
+  float in;                    // scale / softcap
+  float exponent;              // 2 * scale / softcap * log2(e)
+  float small;                 // products up to this magnitude take the polynomial
+  float c0, c1, c2, c3, c4;    // its coefficients times `cap`
+  float back;                  // -1 / cap^2: 1 - tanh^2 = 1 + back * (cap tanh)^2
+};
+inline HeadCap ha_cap(float softcap, float scale) {
+  HeadCap h{};
+  if (!(softcap > 0.f)) return h;
+  h.cap = softcap * kLog2e;
+  h.in = scale / softcap;
+  h.exponent = 2.0f * h.in * kLog2e;
+  h.small = scale != 0.f ? 0.75f / fabsf(h.in) : 0.f;
+  h.c0 = 0.99999946f * h.cap; h.c1 = -0.3332825f * h.cap; h.c2 = 0.13258983f * h.cap; h.c3 = -0.0500563f * h.cap; h.c4 = 0.012929632f * h.cap;
+  h.back = -1.0f / (h.cap * h.cap);
+  return h;
+}
+__device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t s2) {
+  const uint64_t x = mul2(s2, splat2(h.in)), y = mul2(x, x);
+  uint64_t c = fma2(y, splat2(h.c4), splat2(h.c3));
+  c = fma2(y, c, splat2(h.c2));
+  c = fma2(y, c, splat2(h.c1));
+  c = fma2(y, c, splat2(h.c0));
+  return mul2(x, c);
+}
+// q = 1 / (1 + e^2x)
+__device__ __forceinline__ uint64_t cap_rest(const HeadCap& h, uint64_t s2) {
+  uint32_t a0, a1;
+  unpack2(mul2(s2, splat2(h.exponent)), a0, a1);
+  unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), splat2(1.f)), a0, a1);
+  return pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
+}
+// Largest magnitude of 32 products, NaN if one is
+__device__ __forceinline__ float ha_largest(const uint32_t (&r)[32]) {
+  float m[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 16; i++) m[i & 1] = max3(m[i & 1], fabsf(__uint_as_float(r[2 * i])), fabsf(__uint_as_float(r[2 * i + 1])));
+  return max3(m[0], m[1], 0.f);
+}
+
 // A tile as its loading warp publishes it.
 struct TileSlot {
   int tile;                    // -1: no more
