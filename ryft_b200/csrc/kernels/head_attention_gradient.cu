@@ -16,6 +16,7 @@
 //
 // 384 threads: warp 0 draws tiles and loads (TMA), warp 1 issues the MMAs, warps 4-11 do the arithmetic.
 #include <atomic>
+#include <type_traits>
 
 #include "head_attention_tc.cuh"
 
@@ -32,7 +33,7 @@ struct GradParams {
   const float* neg_delta;             // [B, Hq, rows]
   int32_t rows;                       // queries, rounded up to 128
   int32_t tiles, group_heads, key_blocks, total;
-  float in;                           // scale * log2(e)
+  uint64_t in2;                       // scale * log2(e)
   HeadCap cap;
   float scale;
   uint32_t idesc_s, idesc_acc;
@@ -46,53 +47,67 @@ __device__ __forceinline__ int2 grad_range(const GradParams& p, const int2* rs, 
   return make_int2(min(a.x, b.x), max(a.y, b.y));
 }
 
-// P and dS of 32 scores of a row.  nl and nd are the row constants of the pair 2i, 2i + 1.  CAP: 0 none, 1 by the polynomial, 2 any.
-template <int EL, int CAP, typename L, typename N>
-__device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[32], const uint32_t (&dp)[32], const L& nl, const N& nd, float slope, float far,
-                                           uint32_t bits, bool masked, uint32_t (&pw)[16], uint32_t (&dw)[16]) {
-  const uint64_t one2 = splat2(1.f);
+// P and dS of 16 scores of a row as 16-bit words.  nl and nd are the row constants of the pair 2i, 2i + 1; far is the distance of
+// the first, bits say which are seen.  CAP: 0 none, 1 by the polynomial, 2 any.
+template <int EL, int CAP, bool SLOPE, bool MASK, typename L, typename N>
+__device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[16], const uint32_t (&dp)[16], const L& nl, const N& nd, float slope, float far, uint32_t bits,
+                                           uint32_t (&pw)[8], uint32_t (&dw)[8]) {
 #pragma unroll
-  for (int i = 0; i < 16; i++) {
+  for (int i = 0; i < 8; i++) {
     uint64_t x2, bend2 = 0;
     const uint64_t s2 = pack2(s[2 * i], s[2 * i + 1]);
     uint32_t a0, a1;
     if constexpr (CAP == 1) {
-      const uint64_t t2 = cap_small(p.cap, s2);
-      bend2 = fma2(mul2(t2, t2), splat2(p.cap.back), one2);
+      const uint64_t t2 = cap_small(p.cap, mul2(s2, p.cap.in2));
+      bend2 = fma2(mul2(t2, t2), p.cap.back2, splat2(1.f));
       x2 = add2(t2, nl(i));
     } else if constexpr (CAP == 2) {
       // cap * tanh = cap - 2 cap q; its derivative 1 - tanh^2 = 4 q (1 - q)
-      const uint64_t q2 = cap_rest(p.cap, s2);
-      bend2 = mul2(mul2(q2, splat2(4.f)), fma2(q2, splat2(-1.f), one2));
-      x2 = add2(fma2(q2, splat2(-2.f * p.cap.cap), splat2(p.cap.cap)), nl(i));
+      const uint64_t q2 = cap_rest(mul2(s2, p.cap.in2));
+      bend2 = mul2(mul2(q2, splat2(4.f)), fma2(q2, splat2(-1.f), splat2(1.f)));
+      x2 = add2(fma2(q2, p.cap.twice2, p.cap.out2), nl(i));
     } else {
-      x2 = fma2(s2, splat2(p.in), nl(i));
+      x2 = fma2(s2, p.in2, nl(i));
     }
     unpack2(x2, a0, a1);
     float x0 = __uint_as_float(a0), x1 = __uint_as_float(a1);
-    if (slope != 0.f) { x0 = fmaf(fabsf(far - (float)(2 * i)), -slope, x0); x1 = fmaf(fabsf(far - (float)(2 * i + 1)), -slope, x1); }
+    if constexpr (SLOPE) { x0 = fmaf(fabsf(far - (float)(2 * i)), -slope, x0); x1 = fmaf(fabsf(far - (float)(2 * i + 1)), -slope, x1); }
     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
     uint64_t d2 = mul2(pack2(__float_as_uint(p0), __float_as_uint(p1)), add2(pack2(dp[2 * i], dp[2 * i + 1]), nd(i)));
     if constexpr (CAP != 0) d2 = mul2(d2, bend2);
     unpack2(d2, a0, a1);
     pw[i] = ha_pack<EL>(p0, p1);
     dw[i] = ha_pack<EL>(__uint_as_float(a0), __uint_as_float(a1));
-    if (masked) {
+    if constexpr (MASK) {
       // both words' halves: what is not seen is 0, whatever was computed there
       const uint32_t keep = ((bits >> (2 * i)) & 1u ? 0xffffu : 0u) | ((bits >> (2 * i + 1)) & 1u ? 0xffff0000u : 0u);
       pw[i] &= keep; dw[i] &= keep;
     }
   }
 }
-template <int EL, typename L, typename N>
-__device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[32], const uint32_t (&dp)[32], const L& nl, const N& nd, float slope, float far,
-                                           uint32_t bits, bool masked, uint32_t (&pw)[16], uint32_t (&dw)[16]) {
-  if (p.cap.cap > 0.f) {
-    if (__all_sync(0xffffffffu, ha_largest(s) <= p.cap.small)) grad_words<EL, 1>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
-    else grad_words<EL, 2>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
-  } else {
-    grad_words<EL, 0>(p, s, dp, nl, nd, slope, far, bits, masked, pw, dw);
-  }
+// Runs body<CAP, SLOPE, MASK>: every form is a stretch of straight code of its own, chosen once per block, because branches inside it
+// left the warps waiting for instructions.
+template <typename F> __device__ __forceinline__ void grad_choose(int cap, bool slope, bool mask, const F& body) {
+  using std::integral_constant;
+#define B2X_GRAD_FORM(C, S, M) body(integral_constant<int, C>{}, integral_constant<bool, S>{}, integral_constant<bool, M>{})
+#define B2X_GRAD_CAP(C) if (slope) B2X_GRAD_FORM(C, true, true); else if (mask) B2X_GRAD_FORM(C, false, true); else B2X_GRAD_FORM(C, false, false)
+  if (cap == 1) { B2X_GRAD_CAP(1); }
+  else if (cap == 0) { B2X_GRAD_CAP(0); }
+  else { B2X_GRAD_CAP(2); }
+#undef B2X_GRAD_CAP
+#undef B2X_GRAD_FORM
+}
+// Waits for the loads behind two sets of registers; naming them keeps their uses behind the wait.
+__device__ __forceinline__ void grad_wait(uint32_t (&a)[16], uint32_t (&b)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(a[0]), "+r"(a[1]), "+r"(a[2]), "+r"(a[3]), "+r"(a[4]), "+r"(a[5]), "+r"(a[6]), "+r"(a[7]), "+r"(a[8]), "+r"(a[9]), "+r"(a[10]), "+r"(a[11]),
+                 "+r"(a[12]), "+r"(a[13]), "+r"(a[14]), "+r"(a[15])
+               :
+               : "memory");
+  asm volatile("" : "+r"(b[0]), "+r"(b[1]), "+r"(b[2]), "+r"(b[3]), "+r"(b[4]), "+r"(b[5]), "+r"(b[6]), "+r"(b[7]), "+r"(b[8]), "+r"(b[9]), "+r"(b[10]), "+r"(b[11]),
+                    "+r"(b[12]), "+r"(b[13]), "+r"(b[14]), "+r"(b[15])
+               :
+               : "memory");
 }
 
 // Lets the loads in flight land before shared memory goes away.
@@ -346,13 +361,25 @@ k_attention_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         const uint32_t st = sc & 1;
         if (!mbar_wait(bar_sf, sc & 1, abort_flag, status, 52)) { ok = false; break; }
         tc_fence_after();
-        uint32_t sr[2][32], dr[2][32];
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(half * 64 + c * 32), sr[c]);
-          tmem_ld_32x32(tmem_base + lane_addr + 128u + (uint32_t)(half * 64 + c * 32), dr[c]);
+        int cap = 0;
+        if (p.cap.cap > 0.f) {
+          uint32_t t[32];
+          tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(half * 64), t);
+          tc_wait_ld();
+          float largest = ha_largest(t);
+          tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(half * 64 + 32), t);
+          tc_wait_ld();
+          largest = max3(largest, ha_largest(t), 0.f);
+          cap = __all_sync(0xffffffffu, largest <= p.cap.small) ? 1 : 2;
         }
-        tc_wait_ld();
+        uint32_t sr[4][16], dr[4][16];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          tmem_ld_32x16(tmem_base + lane_addr + (uint32_t)(half * 64 + c * 16), sr[c]);
+          tmem_ld_32x16(tmem_base + lane_addr + 128u + (uint32_t)(half * 64 + c * 16), dr[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++) grad_wait(sr[c], dr[c]);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_se);
@@ -369,22 +396,28 @@ k_attention_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ 
         // the product that read this buffer of dS two blocks ago has retired
         if (sc >= 2 && !mbar_wait(bar_dd + 8 * st, ((sc >> 1) - 1) & 1, abort_flag, status, 53)) { ok = false; break; }
         tc_fence_after();
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-          const int k0 = half * 64 + c * 32;
-          uint32_t bits = 0xffffffffu;
-          if (masked) {
-            bits = ha_bits(lim - k0);
+          for (int c = 0; c < 2; c++) {
+            const int k0 = half * 64 + c * 32;
+            seen[c] = ha_bits(lim - k0);
             if (compare) {
               const int key = j * HA_BLOCK + k0 + lane;
               const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + key) : 0;
-              bits &= ha_same_document(doc, theirs, key < p.a.Sk);
+              seen[c] &= ha_same_document(doc, theirs, key < p.a.Sk);
             }
           }
-          uint32_t pw[16], dw[16];
-          grad_words<EL>(p, sr[c], dr[c], [&](int) { return nl2; }, [&](int) { return nd2; }, slope, (float)(pos - j * HA_BLOCK - k0), bits, masked, pw, dw);
-          tmem_st_32x16(tmem_base + lane_addr + 384u + st * 64u + (uint32_t)(k0 / 2), dw);
         }
+        grad_choose(cap, slope != 0.f, masked, [&](auto C, auto S, auto M) {
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            const int k0 = half * 64 + c * 16;
+            uint32_t pw[8], dw[8];
+            grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr[c], dr[c], [&](int) { return nl2; }, [&](int) { return nd2; }, slope, (float)(pos - j * HA_BLOCK - k0), seen[c >> 1] >> (16 * (c & 1)), pw, dw);
+            tmem_st_32x8(tmem_base + lane_addr + 384u + st * 64u + (uint32_t)(k0 / 2), dw);
+          }
+        });
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -668,38 +701,60 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         const int i0 = unit * DKV_UNIT;            // the unit's first query
         const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
         const bool masked = compare || __any_sync(0xffffffffu, from > i0);
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (masked) {
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-          uint32_t sr[32], dr[32], pw[16], dw[16];
-          tmem_ld_32x32(s_addr + (uint32_t)(c * 32), sr);
-          tmem_ld_32x32(s_addr + 64u + (uint32_t)(c * 32), dr);
-          tc_wait_ld();
-          const int q0 = i0 + c * 32;
-          uint32_t bits = 0xffffffffu;
-          if (masked) {
-            bits = ~ha_bits(min(max(from - q0, 0), 32) - 1);
+          for (int c = 0; c < 2; c++) {
+            const int q0 = i0 + c * 32;
+            seen[c] = ~ha_bits(min(max(from - q0, 0), 32) - 1);
             if (compare) {
               const int pos = seq.first + q0 + lane;
               const bool has = pos >= 0 && pos < p.a.Sk && q0 + lane < p.a.Sq;
               const int theirs = has ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos) : 0;
-              bits &= ha_same_document(doc, theirs, has);
+              seen[c] &= ha_same_document(doc, theirs, has);
             }
           }
-          const uint32_t nl_at = rows_at + (uint32_t)(c * 128), nd_at = nl_at + 256;
-          uint64_t nlv[16], ndv[16];
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            uint32_t w0, w1, w2, w3;
-            lds_v4(nl_at + (uint32_t)(i * 16), w0, w1, w2, w3);
-            nlv[2 * i] = pack2(w0, w1); nlv[2 * i + 1] = pack2(w2, w3);
-            lds_v4(nd_at + (uint32_t)(i * 16), w0, w1, w2, w3);
-            ndv[2 * i] = pack2(w0, w1); ndv[2 * i + 1] = pack2(w2, w3);
-          }
-          grad_words<EL>(p, sr, dr, [&](int i) { return nlv[i]; }, [&](int i) { return ndv[i]; }, slope, (float)(key - seq.first - q0), bits, masked, pw, dw);
-          // words of 32 queries into 16 columns that this row has read
-          tmem_st_32x16(s_addr + (uint32_t)(c * 16), pw);
-          tmem_st_32x16(s_addr + 64u + (uint32_t)(c * 16), dw);
         }
+        int cap = 0;
+        if (p.cap.cap > 0.f) {
+          uint32_t t[32];
+          tmem_ld_32x32(s_addr, t);
+          tc_wait_ld();
+          float largest = ha_largest(t);
+          tmem_ld_32x32(s_addr + 32u, t);
+          tc_wait_ld();
+          largest = max3(largest, ha_largest(t), 0.f);
+          cap = __all_sync(0xffffffffu, largest <= p.cap.small) ? 1 : 2;
+        }
+        grad_choose(cap, slope != 0.f, masked, [&](auto C, auto S, auto M) {
+          uint32_t sr[2][16], dr[2][16];
+          tmem_ld_32x16(s_addr, sr[0]);
+          tmem_ld_32x16(s_addr + 64u, dr[0]);
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            grad_wait(sr[c & 1], dr[c & 1]);
+            if (c < 3) {                            // the next sixteen are on their way while these are worked on
+              tmem_ld_32x16(s_addr + (uint32_t)((c + 1) * 16), sr[(c + 1) & 1]);
+              tmem_ld_32x16(s_addr + 64u + (uint32_t)((c + 1) * 16), dr[(c + 1) & 1]);
+            }
+            const uint32_t nl_at = rows_at + (uint32_t)(c * 64), nd_at = nl_at + 256;
+            uint64_t nlv[8], ndv[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              uint32_t w0, w1, w2, w3;
+              lds_v4(nl_at + (uint32_t)(i * 16), w0, w1, w2, w3);
+              nlv[2 * i] = pack2(w0, w1); nlv[2 * i + 1] = pack2(w2, w3);
+              lds_v4(nd_at + (uint32_t)(i * 16), w0, w1, w2, w3);
+              ndv[2 * i] = pack2(w0, w1); ndv[2 * i + 1] = pack2(w2, w3);
+            }
+            uint32_t pw[8], dw[8];
+            grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr[c & 1], dr[c & 1], [&](int i) { return nlv[i]; }, [&](int i) { return ndv[i]; }, slope, (float)(key - seq.first - i0 - c * 16),
+                                          seen[c >> 1] >> (16 * (c & 1)), pw, dw);
+            // words of 16 queries into 8 columns that this row has read
+            tmem_st_32x8(s_addr + (uint32_t)(c * 8), pw);
+            tmem_st_32x8(s_addr + 64u + (uint32_t)(c * 8), dw);
+          }
+        });
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -841,7 +896,7 @@ int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* stat
   int2* ranges = (int2*)(p.neg_delta + n);
   p.key_blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
   p.scale = a.scale;
-  p.in = a.scale * kLog2e;
+  p.in2 = ha_pair(a.scale * kLog2e);
   p.cap = ha_cap(a.softcap, a.scale);
   if (a.documents) {
     const int rc = ha_launch_ranges(a, ranges, stream);

@@ -26,7 +26,7 @@ struct TileParams {
   const int2* ranges;          // documents' ranges per block, [B][key blocks]
   int32_t q_tiles, group_heads, key_blocks, total;
   float mult;                  // scores in registers times this are log2 units: scale * log2(e), or 1 where cap or bias made them so
-  float in;                    // scale * log2(e)
+  uint64_t in2;                // scale * log2(e)
   HeadCap cap;
   int32_t scaled;              // scores are brought to log2 units before anything else (bias; scale not positive)
   uint32_t idesc_qk, idesc_pv;
@@ -341,20 +341,20 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
             for (int c = 0; c < 4; c++)
 #pragma unroll
-              for (int i = 0; i < 16; i++) unpack2(cap_small(p.cap, pack2(r[c][2 * i], r[c][2 * i + 1])), r[c][2 * i], r[c][2 * i + 1]);
+              for (int i = 0; i < 16; i++)
+                unpack2(cap_small(p.cap, mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), r[c][2 * i], r[c][2 * i + 1]);
           } else {
-            const uint64_t out2 = splat2(p.cap.cap), twice2 = splat2(-2.f * p.cap.cap);
 #pragma unroll
             for (int c = 0; c < 4; c++)
 #pragma unroll
-              for (int i = 0; i < 16; i++) unpack2(fma2(cap_rest(p.cap, pack2(r[c][2 * i], r[c][2 * i + 1])), twice2, out2), r[c][2 * i], r[c][2 * i + 1]);
+              for (int i = 0; i < 16; i++)
+                unpack2(fma2(cap_rest(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), p.cap.twice2, p.cap.out2), r[c][2 * i], r[c][2 * i + 1]);
           }
         } else if (p.scaled) {
-          const uint64_t in2 = splat2(p.in);
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), in2), r[c][2 * i], r[c][2 * i + 1]);
+            for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.in2), r[c][2 * i], r[c][2 * i + 1]);
         }
         if (p.a.slopes) {
           const float far = (float)(pos - j * HA_BLOCK);
@@ -561,7 +561,7 @@ int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status
   p.group_heads = (int)(heads > (int64_t)a.B * a.Hq ? (int64_t)a.B * a.Hq : heads);
   p.scaled = a.softcap > 0.f || a.slopes || !(a.scale > 0.f);
   p.mult = p.scaled ? 1.0f : a.scale * kLog2e;
-  p.in = a.scale * kLog2e;
+  p.in2 = ha_pair(a.scale * kLog2e);
   p.cap = ha_cap(a.softcap, a.scale);
   const int D = a.D <= 64 ? 64 : 128;
   const uint32_t format = elem == EL_BF16 ? 1u : 0u;

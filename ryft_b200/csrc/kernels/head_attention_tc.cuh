@@ -1,6 +1,8 @@
 // What the tensor-core kernels of head_attention share: tensor maps over tensors of heads, the ranges of document numbers that
 // let whole blocks be skipped, and masks as bits.
 #pragma once
+#include <cstring>
+
 #include "attention_math.cuh"
 #include "head_attention.cuh"
 #include "sm100.cuh"
@@ -80,37 +82,47 @@ constexpr float kLog2e = 1.4426950408889634f;
 //   else: cap - 2 cap q with q = 1 / (1 + e^2x), two special-function instructions per score, right for any score and infinity.
 // The special-function pipe does 16 a clock and SM and has the softmax's exponential to do for every score as it is: with the
 // second way alone a block of 128 x 128 keeps it busy for 3072 cycles where the tensor pipe needs 1024.
+//
+// Constants are held as pairs, so that packed instructions take them as they are: splitting one value in front of every use cost
+// two moves each.
 struct HeadCap {
   float cap;                   // cap * log2(e); 0: none
-  float in;                    // scale / softcap
-  float exponent;              // 2 * scale / softcap * log2(e)
-  float small;                 // products up to this magnitude take the polynomial
-  float c0, c1, c2, c3, c4;    // its coefficients times `cap`
-  float back;                  // -1 / cap^2: 1 - tanh^2 = 1 + back * (cap tanh)^2
+  float small;                 // products up to this magnitude take the polynomial: 0.75 caps
+  uint64_t in2;                // scale / softcap
+  uint64_t c0, c1, c2, c3, c4; // the polynomial's coefficients times `cap`
+  uint64_t back2;              // -1 / cap^2: 1 - tanh^2 = 1 + back * (cap tanh)^2
+  uint64_t out2, twice2;       // cap, -2 cap
 };
+inline uint64_t ha_pair(float v) {
+  uint32_t u;
+  memcpy(&u, &v, 4);
+  return ((uint64_t)u << 32) | u;
+}
 inline HeadCap ha_cap(float softcap, float scale) {
   HeadCap h{};
   if (!(softcap > 0.f)) return h;
   h.cap = softcap * kLog2e;
-  h.in = scale / softcap;
-  h.exponent = 2.0f * h.in * kLog2e;
-  h.small = scale != 0.f ? 0.75f / fabsf(h.in) : 0.f;
-  h.c0 = 0.99999946f * h.cap; h.c1 = -0.3332825f * h.cap; h.c2 = 0.13258983f * h.cap; h.c3 = -0.0500563f * h.cap; h.c4 = 0.012929632f * h.cap;
-  h.back = -1.0f / (h.cap * h.cap);
+  h.in2 = ha_pair(scale / softcap);
+  h.small = scale != 0.f ? 0.75f * softcap / fabsf(scale) : 0.f;
+  h.c0 = ha_pair(0.99999946f * h.cap); h.c1 = ha_pair(-0.3332825f * h.cap); h.c2 = ha_pair(0.13258983f * h.cap);
+  h.c3 = ha_pair(-0.0500563f * h.cap); h.c4 = ha_pair(0.012929632f * h.cap);
+  h.back2 = ha_pair(-1.0f / (h.cap * h.cap));
+  h.out2 = ha_pair(h.cap); h.twice2 = ha_pair(-2.0f * h.cap);
   return h;
 }
-__device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t s2) {
-  const uint64_t x = mul2(s2, splat2(h.in)), y = mul2(x, x);
-  uint64_t c = fma2(y, splat2(h.c4), splat2(h.c3));
-  c = fma2(y, c, splat2(h.c2));
-  c = fma2(y, c, splat2(h.c1));
-  c = fma2(y, c, splat2(h.c0));
+// cap * tanh(x) of a pair
+__device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t x) {
+  const uint64_t y = mul2(x, x);
+  uint64_t c = fma2(y, h.c4, h.c3);
+  c = fma2(y, c, h.c2);
+  c = fma2(y, c, h.c1);
+  c = fma2(y, c, h.c0);
   return mul2(x, c);
 }
 // q = 1 / (1 + e^2x)
-__device__ __forceinline__ uint64_t cap_rest(const HeadCap& h, uint64_t s2) {
+__device__ __forceinline__ uint64_t cap_rest(uint64_t x) {
   uint32_t a0, a1;
-  unpack2(mul2(s2, splat2(h.exponent)), a0, a1);
+  unpack2(mul2(x, splat2(2.f * kLog2e)), a0, a1);
   unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), splat2(1.f)), a0, a1);
   return pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
 }
