@@ -5,14 +5,17 @@
 // all where one kernel that adds dQ in memory would need five, but no sum depends on the order in which CTAs run, and no f32 copy
 // of dQ is written and read.
 //
-// dQ (k_attention_dq): S = Q K^T and dP = dO V^T into TMEM, eight warps take half a row each into registers, hand the
-// buffers back (the next block's products run meanwhile) and write dS = P (dP - delta) as 16-bit words into TMEM, from where it
-// is the left operand of dQ += dS K: it never passes through shared memory, whose bandwidth bounds the products.
+// Both are one kernel, k_attention_gradient: a tile of 128 rows (queries with their dO; or keys with their values) stays in shared
+// memory, units of 64 of the other side pass by in four stages.  Two products per unit, S and dP (transposed for keys), go into one
+// of two pairs of TMEM buffers of 64 columns, so that four warps turn one pair into P and dS while the tensor pipe works for the other.
+// P and dS are written in place as 16-bit words (a row's words take columns that it has read) and are the left operands of the
+// second products, dQ += dS K, or dV += P^T dO and dK += dS^T Q: they never pass through shared memory, whose bandwidth bounds
+// the products.  Accumulators and buffers fill TMEM at a width of 128.  Query heads that share a key head follow one another into the
+// same accumulators of dK and dV.
 //
-// dK, dV (k_attention_dkv): S^T = K Q^T and dP^T = V dO^T for 64 queries at a time into one of two pairs of TMEM buffers, so that
-// four warps turn one pair into P^T and dS^T (in place: a row's words take the columns that it has read) while the tensor pipe
-// works on the other; then dV += P^T dO and dK += dS^T Q.  The two accumulators and the buffers fill TMEM at a width of 128.
-// Query heads that share a key head follow one another into the same accumulators.
+// The arithmetic of a unit is a loop over 16 columns whose body is one of nine forms (cap, bias, mask), chosen once per unit: with
+// the four steps unrolled, or with the forms' branches inside, the warps waited for instructions more than for anything else
+// (ncu, training_capped's dK and dV: 505 us with branches inside, 416 unrolled, 336 as a loop).
 //
 // 384 threads: warp 0 draws tiles and loads (TMA), warp 1 issues the MMAs, warps 4-11 do the arithmetic.
 #include <atomic>
@@ -23,8 +26,8 @@
 namespace b2x {
 namespace {
 
-constexpr int DKV_UNIT = 64;          // queries per step of dK, dV
-constexpr int DKV_STAGES = 4;
+constexpr int GRAD_UNIT = 64;         // keys (dQ) or queries (dK, dV) per step
+constexpr int GRAD_STAGES = 4;
 
 struct GradParams {
   HeadAttn a;
@@ -134,359 +137,49 @@ __device__ __forceinline__ void grad_write_row(uint32_t taddr, char* row, bool t
   }
 }
 
-// ---- dQ --------------------------------------------------------------------------------------------------------------------
-template <int D> struct DqSmem {
-  static constexpr int T_BYTES = HA_BLOCK * D * 2;
-  static constexpr int Q_OFF = 0, DO_OFF = T_BYTES;
-  static constexpr int K_OFF = 2 * T_BYTES;                // 2 stages
-  static constexpr int V_OFF = 4 * T_BYTES;                // 2 stages
-  static constexpr int BAR_OFF = 6 * T_BYTES;
-  static constexpr int SLOT_OFF = BAR_OFF + 256;
-  static constexpr int TOTAL = SLOT_OFF + 2 * (int)sizeof(TileSlot) + 1024;
-};
-
-template <int D, int EL>
-__global__ void __launch_bounds__(384, 1)
-k_attention_dq(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmK,
-               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ GradParams p, int32_t* sched, int32_t* status) {
-  using namespace sm100;
-  using SM = DqSmem<D>;
-  constexpr int DC = D / 64;
-  constexpr uint32_t TMEM_COLS = 512;          // S [0,128), dP [128,256), dQ [256, 256 + D), dS [384,448) and [448,512)
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  const uint32_t sbase = smem_u32(smem);
-  const uint32_t b0 = sbase + SM::BAR_OFF;
-  const uint32_t bar_qf = b0, bar_qe = b0 + 8, bar_kf = b0 + 16 /* [2] */, bar_ke = b0 + 32, bar_vf = b0 + 48, bar_ve = b0 + 64, bar_sf = b0 + 80, bar_se = b0 + 88,
-                 bar_df = b0 + 96 /* [2] */, bar_dd = b0 + 112 /* [2] */, bar_of = b0 + 128, bar_tf = b0 + 136 /* [2] */, bar_te = b0 + 152 /* [2] */, bar_end = b0 + 168,
-                 bar_drain = b0 + 176;
-  uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 192);
-  volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-  volatile TileSlot* slots = (volatile TileSlot*)(smem + SM::SLOT_OFF);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool listed = p.ranges != nullptr;
-
-  if (threadIdx.x == 0) {
-    mbar_init(bar_qf, 1); mbar_init(bar_qe, 1); mbar_init(bar_sf, 1); mbar_init(bar_se, 8); mbar_init(bar_of, 8); mbar_init(bar_end, 1); mbar_init(bar_drain, 1);
-    for (uint32_t s = 0; s < 16; s += 8) {
-      mbar_init(bar_kf + s, 1); mbar_init(bar_ke + s, 1); mbar_init(bar_vf + s, 1); mbar_init(bar_ve + s, 1);
-      mbar_init(bar_df + s, 8); mbar_init(bar_dd + s, 1); mbar_init(bar_tf + s, 1); mbar_init(bar_te + s, 9);
-    }
-    *abort_flag = 0;
-    mbar_fence_init();
-    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmDO); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
-  }
-  if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  pdl_trigger();
-  pdl_wait();          // everything above touched this SM only
-
-  if (warp == 0) {
-    // ---------------------------------------------- tiles and loads ------------------------------------------------
-    uint32_t kc = 0, nq = 0;       // blocks loaded, tiles with work
-    int fixed = (int)blockIdx.x;
-    for (int n = 0;; n++) {
-      const bool free = n < 2 || mbar_wait(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 31);
-      if (!__all_sync(0xffffffffu, free)) break;
-      int t = 0;
-      if (sched) {
-        if (lane == 0) t = atomicAdd(sched, 1);
-        t = __shfl_sync(0xffffffffu, t, 0);
-      } else { t = fixed; fixed += (int)gridDim.x; }
-      if (t >= p.total) t = -1;
-      volatile TileSlot* s = slots + (n & 1);
-      int b = 0, h = 0, q0 = 0, blocks = 0;
-      HeadSequence seq{};
-      if (t >= 0) {
-        const int per_group = p.group_heads * p.tiles;
-        const int g = t / per_group, in = t - g * per_group;
-        const int heads = min(p.group_heads, p.a.B * p.a.Hq - g * p.group_heads);
-        const int rank = in / heads, bh = g * p.group_heads + (in - rank * heads);
-        b = bh / p.a.Hq; h = bh - b * p.a.Hq; q0 = (p.tiles - 1 - rank) * HA_BLOCK;
-        const int last = min(q0 + HA_BLOCK, p.a.Sq) - 1;
-        seq = head_sequence(p.a, b);
-        blocks = (max(head_limit(p.a, seq, seq.first + last), 0) + HA_BLOCK - 1) / HA_BLOCK;
-        if (listed) {
-          const int2* rs = p.ranges + (int64_t)b * p.key_blocks;
-          const int2 mine = grad_range(p, rs, seq.first + q0, seq.first + last);
-          int count = 0;
-          for (int i = 0; i < HA_MASK_WORDS; i++) {
-            const int j = i * 32 + lane;
-            bool visit = false, compare = false;
-            if (j < blocks) { const int2 r = ha_range(rs + j); visit = !ha_apart(mine, r); compare = !ha_one_document(mine, r); }
-            const uint32_t mv = __ballot_sync(0xffffffffu, visit), mc = __ballot_sync(0xffffffffu, compare);
-            if (lane == 0) { s->visit[i] = mv; s->compare[i] = mc; }
-            count += __popc(mv);
-          }
-          blocks = count;
-        }
-      }
-      if (lane == 0) {
-        s->tile = t; s->b = b; s->h = h; s->at = q0; s->begin = 0; s->blocks = blocks;
-        s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
-        mbar_arrive(bar_tf + 8 * (n & 1));
-      }
-      __syncwarp();
-      if (t < 0) break;
-      if (blocks == 0) continue;
-      if (elect_one()) {
-        const int u = h / p.a.group;
-        bool ok = nq == 0 || mbar_wait(bar_qe, (nq - 1) & 1, abort_flag, status, 32);
-        if (ok) {
-          mbar_expect_tx(bar_qf, 2 * SM::T_BYTES);
-#pragma unroll
-          for (int c = 0; c < DC; c++) {
-            tma_load_4d(sbase + SM::Q_OFF + c * HA_CHUNK, &tmQ, bar_qf, c * 64, q0, h, b);
-            tma_load_4d(sbase + SM::DO_OFF + c * HA_CHUNK, &tmDO, bar_qf, c * 64, q0, h, b);
-          }
-          BlockWalk walk;
-          walk.start(s, listed);
-          for (int it = 0; it < blocks && ok; it++) {
-            const uint32_t k = kc + (uint32_t)it, st = k & 1, turn = k >> 1;
-            if (turn > 0) ok = mbar_wait(bar_ke + 8 * st, (turn - 1) & 1, abort_flag, status, 33);
-            if (!ok) break;
-            mbar_expect_tx(bar_kf + 8 * st, SM::T_BYTES);
-#pragma unroll
-            for (int c = 0; c < DC; c++) tma_load_4d(sbase + SM::K_OFF + st * SM::T_BYTES + c * HA_CHUNK, &tmK, bar_kf + 8 * st, c * 64, walk.j * HA_BLOCK, u, b);
-            if (turn > 0) ok = mbar_wait(bar_ve + 8 * st, (turn - 1) & 1, abort_flag, status, 34);
-            if (!ok) break;
-            mbar_expect_tx(bar_vf + 8 * st, SM::T_BYTES);
-#pragma unroll
-            for (int c = 0; c < DC; c++) tma_load_4d(sbase + SM::V_OFF + st * SM::T_BYTES + c * HA_CHUNK, &tmV, bar_vf + 8 * st, c * 64, walk.j * HA_BLOCK, u, b);
-            walk.next();
-          }
-        }
-        if (!ok) grad_linger();
-      }
-      __syncwarp();
-      kc += (uint32_t)blocks; nq++;
-      if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
-    }
-  } else if (warp == 1) {
-    // ---------------------------------------------- MMA issuer ------------------------------------------------------
-    if (elect_one()) {
-      uint32_t kc = 0, dc = 0, nq = 0;     // blocks whose scores are issued, blocks added to dQ, tiles with work
-      const uint32_t qa = sbase + SM::Q_OFF, da = sbase + SM::DO_OFF;
-      bool ok = true;
-      auto issue_scores = [&](bool last_of_tile) -> bool {
-        const uint32_t st = kc & 1, ph = (kc >> 1) & 1;
-        const uint32_t ka = sbase + SM::K_OFF + st * SM::T_BYTES, va = sbase + SM::V_OFF + st * SM::T_BYTES;
-        // the previous block's scores are in registers
-        if (kc > 0 && !mbar_wait(bar_se, (kc - 1) & 1, abort_flag, status, 41)) return false;
-        if (!mbar_wait(bar_kf + 8 * st, ph, abort_flag, status, 42)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t off = (uint32_t)(k >> 2) * HA_CHUNK + (uint32_t)(k & 3) * 32;
-          umma_ss<false>(tmem_base, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
-        }
-        if (!mbar_wait(bar_vf + 8 * st, ph, abort_flag, status, 43)) return false;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t off = (uint32_t)(k >> 2) * HA_CHUNK + (uint32_t)(k & 3) * 32;
-          umma_ss<false>(tmem_base + 128u, make_smem_desc(da + off, 16, 1024), make_smem_desc(va + off, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
-        }
-        tc_commit(bar_sf);
-        tc_commit(bar_ve + 8 * st);
-        if (last_of_tile) tc_commit(bar_qe);
-        kc++;
-        return true;
-      };
-      for (int n = 0; ok; n++) {
-        if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 44)) { ok = false; break; }
-        const int t = slots[n & 1].tile, blocks = slots[n & 1].blocks;
-        mbar_arrive(bar_te + 8 * (n & 1));
-        if (t < 0) break;
-        if (blocks == 0) continue;
-        if (!mbar_wait(bar_qf, nq & 1, abort_flag, status, 45)) { ok = false; break; }
-        if (!issue_scores(blocks == 1)) { ok = false; break; }
-        for (int it = 0; it < blocks && ok; it++) {
-          if (it + 1 < blocks && !issue_scores(it + 2 == blocks)) { ok = false; break; }
-          const uint32_t st = dc & 1, ph = (dc >> 1) & 1;
-          if (!mbar_wait(bar_df + 8 * st, ph, abort_flag, status, 46)) { ok = false; break; }
-          // the previous tile's rows have been read out of the accumulator
-          if (it == 0 && nq > 0 && !mbar_wait(bar_of, (nq - 1) & 1, abort_flag, status, 47)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t ka = sbase + SM::K_OFF + st * SM::T_BYTES;
-#pragma unroll
-          for (int k = 0; k < HA_BLOCK / 16; k++)
-            // A = dS from TMEM: 16 keys are 8 columns; B = K (MN-major: head-dim chunks of 64 are HA_CHUNK apart)
-            umma_ts_f16(tmem_base + 256u, tmem_base + 384u + st * 64u + (uint32_t)(k * 8), make_smem_desc(ka + (uint32_t)k * 2048, HA_CHUNK, 1024), p.idesc_acc,
-                        (it > 0 || k > 0) ? 1u : 0u);
-          tc_commit(bar_ke + 8 * st);
-          tc_commit(bar_dd + 8 * st);
-          if (it + 1 == blocks) tc_commit(bar_end);
-          dc++;
-        }
-        nq++;
-      }
-      // everything this thread issued must retire before TMEM is released
-      tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, abort_flag, nullptr, 0);
-    }
-  } else if (warp >= 4) {
-    // ---------------------------------------------- P and dS --------------------------------------------------------
-    const int half = (warp - 4) >> 2;             // keys [64 * half, 64 * half + 64) of a block
-    const int quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
-    uint32_t sc = 0, nq = 0;                      // blocks done, tiles with work
-    bool ok = true;
-    for (int n = 0; ok; n++) {
-      if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 51)) { ok = false; break; }
-      volatile TileSlot* s = slots + (n & 1);
-      const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->at;
-      const HeadSequence seq{s->length, s->first, s->prefix};
-      if (!listed || t < 0 || blocks == 0) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
-      if (t < 0) break;
-      const int qrow = q0 + row, pos = seq.first + qrow;
-      const int64_t at = ((int64_t)b * p.a.Hq + h) * p.rows + qrow;
-      const uint64_t nl2 = splat2(ld_global(p.neg_lse + at)), nd2 = splat2(ld_global(p.neg_delta + at));
-      const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
-      int doc = 0, end = head_limit(p.a, seq, pos);
-      if (p.a.documents) {
-        if (pos >= 0 && pos < p.a.Sk) doc = (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos);
-        else end = 0;
-      }
-      BlockWalk walk;
-      if (blocks > 0) walk.start(s, listed);
-      for (int it = 0; it < blocks && ok; it++) {
-        const int j = walk.j;
-        const bool compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
-        if (it + 1 < blocks) walk.next();
-        else if (listed) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
-        const uint32_t st = sc & 1;
-        if (!mbar_wait(bar_sf, sc & 1, abort_flag, status, 52)) { ok = false; break; }
-        tc_fence_after();
-        int cap = 0;
-        if (p.cap.cap > 0.f) {
-          uint32_t t[32];
-          tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(half * 64), t);
-          tc_wait_ld();
-          float largest = ha_largest(t);
-          tmem_ld_32x32(tmem_base + lane_addr + (uint32_t)(half * 64 + 32), t);
-          tc_wait_ld();
-          largest = max3(largest, ha_largest(t), 0.f);
-          cap = __all_sync(0xffffffffu, largest <= p.cap.small) ? 1 : 2;
-        }
-        uint32_t sr[4][16], dr[4][16];
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          tmem_ld_32x16(tmem_base + lane_addr + (uint32_t)(half * 64 + c * 16), sr[c]);
-          tmem_ld_32x16(tmem_base + lane_addr + 128u + (uint32_t)(half * 64 + c * 16), dr[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; c++) grad_wait(sr[c], dr[c]);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_se);
-        const int lim = end - 1 - j * HA_BLOCK;
-        const bool masked = compare || __any_sync(0xffffffffu, lim < HA_BLOCK - 1);
-        if (half == 0 && p.a.lengths && seq.length < p.a.Sk && seq.length < (j + 1) * HA_BLOCK && j * HA_BLOCK + row >= seq.length) {
-          // keys behind the sequence's end: zero before they meet their dS of zero (the scores have been computed: K has landed)
-#pragma unroll 1
-          for (int c = 0; c < DC; c++)
-#pragma unroll
-            for (int q = 0; q < 8; q++) sts_v4(sbase + (uint32_t)(SM::K_OFF + st * SM::T_BYTES + c * HA_CHUNK + row * 128 + q * 16), 0, 0, 0, 0);
-          fence_async_shared();
-        }
-        // the product that read this buffer of dS two blocks ago has retired
-        if (sc >= 2 && !mbar_wait(bar_dd + 8 * st, ((sc >> 1) - 1) & 1, abort_flag, status, 53)) { ok = false; break; }
-        tc_fence_after();
-        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const int k0 = half * 64 + c * 32;
-            seen[c] = ha_bits(lim - k0);
-            if (compare) {
-              const int key = j * HA_BLOCK + k0 + lane;
-              const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + key) : 0;
-              seen[c] &= ha_same_document(doc, theirs, key < p.a.Sk);
-            }
-          }
-        }
-        grad_choose(cap, slope != 0.f, masked, [&](auto C, auto S, auto M) {
-#pragma unroll
-          for (int c = 0; c < 4; c++) {
-            const int k0 = half * 64 + c * 16;
-            uint32_t pw[8], dw[8];
-            grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr[c], dr[c], [&](int) { return nl2; }, [&](int) { return nd2; }, slope, (float)(pos - j * HA_BLOCK - k0), seen[c >> 1] >> (16 * (c & 1)), pw, dw);
-            tmem_st_32x8(tmem_base + lane_addr + 384u + st * 64u + (uint32_t)(k0 / 2), dw);
-          }
-        });
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_df + 8 * st);
-        sc++;
-      }
-      if (!ok) break;
-      if (blocks > 0) {
-        if (!mbar_wait(bar_end, nq & 1, abort_flag, status, 54)) { ok = false; break; }
-        tc_fence_after();
-        nq++;
-      }
-      // each half of the warps writes half of the width
-      char* out = p.a.dq + 2 * ((int64_t)b * p.a.dqs.batch + (int64_t)h * p.a.dqs.head + (int64_t)qrow * p.a.dqs.token) + half * D;
-      grad_write_row<EL, D / 2>(tmem_base + lane_addr + 256u + (uint32_t)(half * (D / 2)), out, qrow < p.a.Sq, p.a.D - half * (D / 2), p.scale, blocks == 0);
-      tc_fence_before();
-      __syncwarp();
-      if (blocks > 0 && lane == 0) mbar_arrive(bar_of);
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, TMEM_COLS); }
-  // the last CTA to leave puts the tile counter back for the stream's next launch
-  if (sched && threadIdx.x == 0 && atomicAdd(sched + 1, 1) == (int)gridDim.x - 1) { sched[0] = 0; sched[1] = 0; __threadfence(); }
-}
-
-// ---- dK, dV ----------------------------------------------------------------------------------------------------------------
-template <int D> struct DkvSmem {
-  static constexpr int T_BYTES = HA_BLOCK * D * 2;         // K, V
-  static constexpr int U_BYTES = DKV_UNIT * D * 2;         // Q, dO of a unit
-  static constexpr int K_OFF = 0, V_OFF = T_BYTES;
-  static constexpr int Q_OFF = 2 * T_BYTES;                // DKV_STAGES x (Q, dO)
-  static constexpr int ROW_OFF = Q_OFF + DKV_STAGES * 2 * U_BYTES;   // row constants: 2 groups x 2 turns x (64 + 64) floats
+// ---- the tile kernel -------------------------------------------------------------------------------------------------------
+template <int D> struct GradSmem {
+  static constexpr int T_BYTES = HA_BLOCK * D * 2;         // the tile's Q and dO, or K and V
+  static constexpr int U_BYTES = GRAD_UNIT * D * 2;        // a unit's K and V, or Q and dO
+  static constexpr int T0_OFF = 0, T1_OFF = T_BYTES;
+  static constexpr int U_OFF = 2 * T_BYTES;                // GRAD_STAGES x 2
+  static constexpr int ROW_OFF = U_OFF + GRAD_STAGES * 2 * U_BYTES;   // row constants: 2 groups x 2 turns x (64 + 64) floats
   static constexpr int BAR_OFF = ROW_OFF + 2 * 2 * 512;
   static constexpr int SLOT_OFF = BAR_OFF + 256;
   static constexpr int TOTAL = SLOT_OFF + 2 * (int)sizeof(TileSlot) + 1024;
 };
 
-template <int D, int EL>
+// KEYS: tiles of keys (dK, dV); else tiles of queries (dQ).  t0, t1: Q and dO, or K and V; u0, u1: K and V, or Q and dO.
+template <int D, int EL, bool KEYS>
 __global__ void __launch_bounds__(384, 1)
-k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ GradParams p, int32_t* sched, int32_t* status) {
+k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_constant__ CUtensorMap tmT1, const __grid_constant__ CUtensorMap tmU0,
+                     const __grid_constant__ CUtensorMap tmU1, const __grid_constant__ GradParams p, int32_t* sched, int32_t* status) {
   using namespace sm100;
-  using SM = DkvSmem<D>;
+  using SM = GradSmem<D>;
   constexpr int DC = D / 64;
-  constexpr uint32_t U_CHUNK = DKV_UNIT * 128;             // one [64 rows x 128 bytes] swizzled sub-tile
-  constexpr uint32_t TMEM_COLS = 512;          // pair g: S^T [128 g, +64), dP^T [128 g + 64, +64); dV [256, 256 + D), dK [256 + D, 256 + 2 D)
+  constexpr uint32_t U_CHUNK = GRAD_UNIT * 128;            // one [64 rows x 128 bytes] swizzled sub-tile
+  constexpr uint32_t TMEM_COLS = 512;          // pair g: S [128 g, +64), dP [128 g + 64, +64); dQ or dV [256, 256 + D), dK [256 + D, 256 + 2 D)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
   const uint32_t b0 = sbase + SM::BAR_OFF;
-  const uint32_t bar_kf = b0, bar_ke = b0 + 8, bar_qf = b0 + 16 /* [4] */, bar_qe = b0 + 48 /* [4] */, bar_sf = b0 + 80 /* [2] */, bar_pf = b0 + 96 /* [2] */,
-                 bar_end = b0 + 112, bar_of = b0 + 120, bar_tf = b0 + 128 /* [2] */, bar_te = b0 + 144 /* [2] */, bar_drain = b0 + 160, bar_rf = b0 + 168 /* [2] */;
+  const uint32_t bar_tl = b0, bar_tu = b0 + 8 /* tile loaded, tile used */, bar_uf = b0 + 16 /* [4] */, bar_ue = b0 + 48 /* [4] */, bar_sf = b0 + 80 /* [2] */,
+                 bar_pf = b0 + 96 /* [2] */, bar_end = b0 + 112, bar_of = b0 + 120, bar_tf = b0 + 128 /* [2] */, bar_te = b0 + 144 /* [2] */, bar_drain = b0 + 160,
+                 bar_rf = b0 + 168 /* [2] */;
   uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 192);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile TileSlot* slots = (volatile TileSlot*)(smem + SM::SLOT_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool listed = p.ranges != nullptr;
-  const int units_all = (p.a.Sq + DKV_UNIT - 1) / DKV_UNIT;
+  const int repeat = KEYS ? p.a.group : 1;     // heads that pass by a tile
 
   if (threadIdx.x == 0) {
-    mbar_init(bar_kf, 1); mbar_init(bar_ke, 1); mbar_init(bar_end, 1); mbar_init(bar_of, 8); mbar_init(bar_drain, 1);
-    for (uint32_t s = 0; s < 8 * DKV_STAGES; s += 8) { mbar_init(bar_qf + s, 1); mbar_init(bar_qe + s, 1); }
+    mbar_init(bar_tl, 1); mbar_init(bar_tu, 1); mbar_init(bar_end, 1); mbar_init(bar_of, 8); mbar_init(bar_drain, 1);
+    for (uint32_t s = 0; s < 8 * GRAD_STAGES; s += 8) { mbar_init(bar_uf + s, 1); mbar_init(bar_ue + s, 1); }
     for (uint32_t s = 0; s < 16; s += 8) { mbar_init(bar_sf + s, 1); mbar_init(bar_pf + s, 4); mbar_init(bar_rf + s, 4); mbar_init(bar_tf + s, 1); mbar_init(bar_te + s, 9); }
     *abort_flag = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tmQ); tma_prefetch_desc(&tmDO); tma_prefetch_desc(&tmK); tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmT0); tma_prefetch_desc(&tmT1); tma_prefetch_desc(&tmU0); tma_prefetch_desc(&tmU1);
   }
   if (warp == 1) { tmem_alloc(smem_u32(tmem_slot), TMEM_COLS); tmem_relinquish(); }
   tc_fence_before();
@@ -498,7 +191,7 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
 
   if (warp == 0) {
     // ---------------------------------------------- tiles and loads ------------------------------------------------
-    uint32_t uc = 0, nk = 0;       // units loaded, tiles with work
+    uint32_t uc = 0, nt = 0;       // units loaded, tiles with work
     int fixed = (int)blockIdx.x;
     for (int n = 0;; n++) {
       const bool free = n < 2 || mbar_wait(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 61);
@@ -510,32 +203,49 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       } else { t = fixed; fixed += (int)gridDim.x; }
       if (t >= p.total) t = -1;
       volatile TileSlot* s = slots + (n & 1);
-      int b = 0, u = 0, j0 = 0, begin = 0, units = 0;
+      int b = 0, h = 0, at = 0, begin = 0, units = 0;
       HeadSequence seq{};
       if (t >= 0) {
-        // the first keys are seen by most queries: their tiles first
+        // the tiles with the most units first: the last queries, the first keys; inside a group of heads that stay in L2 together
+        const int all = KEYS ? p.a.Hk : p.a.Hq;
         const int per_group = p.group_heads * p.tiles;
         const int g = t / per_group, in = t - g * per_group;
-        const int heads = min(p.group_heads, p.a.B * p.a.Hk - g * p.group_heads);
-        const int rank = in / heads, bu = g * p.group_heads + (in - rank * heads);
-        b = bu / p.a.Hk; u = bu - b * p.a.Hk; j0 = rank * HA_BLOCK;
+        const int heads = min(p.group_heads, p.a.B * all - g * p.group_heads);
+        const int rank = in / heads, bh = g * p.group_heads + (in - rank * heads);
+        b = bh / all; h = bh - b * all;
+        at = (KEYS ? rank : p.tiles - 1 - rank) * HA_BLOCK;
         seq = head_sequence(p.a, b);
-        if (j0 < seq.length) {
-          if (p.a.causal && j0 >= seq.prefix) begin = min(max(j0 - seq.first, 0) / DKV_UNIT, units_all);
-          units = units_all - begin;
+        int stop;                                // the unit behind the last
+        if constexpr (KEYS) {
+          stop = (p.a.Sq + GRAD_UNIT - 1) / GRAD_UNIT;
+          if (at >= seq.length) stop = 0;
+          else if (p.a.causal && at >= seq.prefix) begin = min(max(at - seq.first, 0) / GRAD_UNIT, stop);
+        } else {
+          const int last = min(at + HA_BLOCK, p.a.Sq) - 1;
+          stop = (max(head_limit(p.a, seq, seq.first + last), 0) + GRAD_UNIT - 1) / GRAD_UNIT;
         }
+        units = stop - begin;
         if (listed) {
           const int2* rs = p.ranges + (int64_t)b * p.key_blocks;
-          const int2 mine = ha_range(rs + j0 / HA_BLOCK);
+          int2 mine;
+          if constexpr (KEYS) mine = ha_range(rs + at / HA_BLOCK);
+          else mine = grad_range(p, rs, seq.first + at, seq.first + min(at + HA_BLOCK, p.a.Sq) - 1);
           int count = 0;
           for (int i = 0; i < HA_MASK_WORDS; i++) {
             const int k = i * 32 + lane;
             bool visit = false, compare = false;
-            if (units > 0 && k >= begin && k < units_all) {
-              const int lo = seq.first + k * DKV_UNIT;
-              const int2 r = grad_range(p, rs, lo, min(lo + DKV_UNIT, seq.first + p.a.Sq) - 1);
+            if (k >= begin && k < stop) {
+              int2 r;
+              bool all_there = true;
+              if constexpr (KEYS) {
+                const int lo = seq.first + k * GRAD_UNIT;
+                r = grad_range(p, rs, lo, min(lo + GRAD_UNIT, seq.first + p.a.Sq) - 1);
+                all_there = lo >= 0 && lo + GRAD_UNIT <= p.a.Sk;
+              } else {
+                r = ha_range(rs + k * GRAD_UNIT / HA_BLOCK);
+              }
               visit = !ha_apart(mine, r);
-              compare = !ha_one_document(mine, r) || lo < 0 || lo + DKV_UNIT > p.a.Sk;
+              compare = !ha_one_document(mine, r) || !all_there;
             }
             const uint32_t mv = __ballot_sync(0xffffffffu, visit), mc = __ballot_sync(0xffffffffu, compare);
             if (lane == 0) { s->visit[i] = mv; s->compare[i] = mc; }
@@ -545,7 +255,7 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         }
       }
       if (lane == 0) {
-        s->tile = t; s->b = b; s->h = u; s->at = j0; s->begin = begin; s->blocks = units;
+        s->tile = t; s->b = b; s->h = h; s->at = at; s->begin = begin; s->blocks = units;
         s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
         mbar_arrive(bar_tf + 8 * (n & 1));
       }
@@ -553,28 +263,28 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       if (t < 0) break;
       if (units == 0) continue;
       if (elect_one()) {
-        bool ok = nk == 0 || mbar_wait(bar_ke, (nk - 1) & 1, abort_flag, status, 62);
+        bool ok = nt == 0 || mbar_wait(bar_tu, (nt - 1) & 1, abort_flag, status, 62);
         if (ok) {
-          mbar_expect_tx(bar_kf, 2 * SM::T_BYTES);
+          mbar_expect_tx(bar_tl, 2 * SM::T_BYTES);
 #pragma unroll
           for (int c = 0; c < DC; c++) {
-            tma_load_4d(sbase + SM::K_OFF + c * HA_CHUNK, &tmK, bar_kf, c * 64, j0, u, b);
-            tma_load_4d(sbase + SM::V_OFF + c * HA_CHUNK, &tmV, bar_kf, c * 64, j0, u, b);
+            tma_load_4d(sbase + SM::T0_OFF + c * HA_CHUNK, &tmT0, bar_tl, c * 64, at, h, b);
+            tma_load_4d(sbase + SM::T1_OFF + c * HA_CHUNK, &tmT1, bar_tl, c * 64, at, h, b);
           }
           uint32_t k = uc;
-          for (int hh = 0; hh < p.a.group && ok; hh++) {
-            const int h = u * p.a.group + hh;
+          for (int hh = 0; hh < repeat && ok; hh++) {
+            const int uh = KEYS ? h * p.a.group + hh : h / p.a.group;
             BlockWalk walk;
             walk.start(s, listed);
             for (int it = 0; it < units; it++, k++) {
-              const uint32_t st = k % DKV_STAGES, turn = k / DKV_STAGES;
-              if (turn > 0 && !mbar_wait(bar_qe + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
-              mbar_expect_tx(bar_qf + 8 * st, 2 * SM::U_BYTES);
-              const uint32_t qa = sbase + SM::Q_OFF + st * 2 * SM::U_BYTES;
+              const uint32_t st = k % GRAD_STAGES, turn = k / GRAD_STAGES;
+              if (turn > 0 && !mbar_wait(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
+              mbar_expect_tx(bar_uf + 8 * st, 2 * SM::U_BYTES);
+              const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES;
 #pragma unroll
               for (int c = 0; c < DC; c++) {
-                tma_load_4d(qa + c * U_CHUNK, &tmQ, bar_qf + 8 * st, c * 64, walk.j * DKV_UNIT, h, b);
-                tma_load_4d(qa + SM::U_BYTES + c * U_CHUNK, &tmDO, bar_qf + 8 * st, c * 64, walk.j * DKV_UNIT, h, b);
+                tma_load_4d(ua + c * U_CHUNK, &tmU0, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
+                tma_load_4d(ua + SM::U_BYTES + c * U_CHUNK, &tmU1, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
               }
               if (it + 1 < units) walk.next();
             }
@@ -583,175 +293,208 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
         if (!ok) grad_linger();
       }
       __syncwarp();
-      uc += (uint32_t)(units * p.a.group); nk++;
+      uc += (uint32_t)(units * repeat); nt++;
       if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
     }
   } else if (warp == 1) {
     // ---------------------------------------------- MMA issuer ------------------------------------------------------
     if (elect_one()) {
-      uint32_t sc = 0, uc = 0, nk = 0;     // units whose scores are issued, units added to dK and dV, tiles with work
-      const uint32_t ka = sbase + SM::K_OFF, va = sbase + SM::V_OFF;
+      uint32_t sc = 0, uc = 0, nt = 0;     // units whose scores are issued, units added to the accumulators, tiles with work
+      const uint32_t ta = sbase + SM::T0_OFF, tb = sbase + SM::T1_OFF;
       bool ok = true;
       auto issue_scores = [&](bool last_of_tile) -> bool {
-        const uint32_t st = sc % DKV_STAGES, g = sc & 1;
-        const uint32_t qa = sbase + SM::Q_OFF + st * 2 * SM::U_BYTES, da = qa + SM::U_BYTES;
-        if (!mbar_wait(bar_qf + 8 * st, (sc / DKV_STAGES) & 1, abort_flag, status, 71)) return false;
+        const uint32_t st = sc % GRAD_STAGES, g = sc & 1;
+        const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
+        if (!mbar_wait(bar_uf + 8 * st, (sc / GRAD_STAGES) & 1, abort_flag, status, 71)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
           const uint32_t in = (uint32_t)(k & 3) * 32, c = (uint32_t)(k >> 2);
-          umma_ss<false>(tmem_base + g * 128u, make_smem_desc(ka + c * HA_CHUNK + in, 16, 1024), make_smem_desc(qa + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
+          umma_ss<false>(tmem_base + g * 128u, make_smem_desc(ta + c * HA_CHUNK + in, 16, 1024), make_smem_desc(ua + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
         }
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
           const uint32_t in = (uint32_t)(k & 3) * 32, c = (uint32_t)(k >> 2);
-          umma_ss<false>(tmem_base + g * 128u + 64u, make_smem_desc(va + c * HA_CHUNK + in, 16, 1024), make_smem_desc(da + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
+          umma_ss<false>(tmem_base + g * 128u + 64u, make_smem_desc(tb + c * HA_CHUNK + in, 16, 1024), make_smem_desc(ub + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
         }
         tc_commit(bar_sf + 8 * g);
-        if (last_of_tile) tc_commit(bar_ke);
+        if (last_of_tile) tc_commit(bar_tu);
         sc++;
         return true;
       };
       for (int n = 0; ok; n++) {
         if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 72)) { ok = false; break; }
-        const int t = slots[n & 1].tile, total = slots[n & 1].blocks * p.a.group;
+        const int t = slots[n & 1].tile, total = slots[n & 1].blocks * repeat;
         mbar_arrive(bar_te + 8 * (n & 1));
         if (t < 0) break;
         if (total == 0) continue;
-        if (!mbar_wait(bar_kf, nk & 1, abort_flag, status, 73)) { ok = false; break; }
+        if (!mbar_wait(bar_tl, nt & 1, abort_flag, status, 73)) { ok = false; break; }
         for (int it = 0; it < 2 && it < total && ok; it++) ok = issue_scores(it + 1 == total);
         for (int it = 0; it < total && ok; it++) {
-          const uint32_t st = uc % DKV_STAGES, g = uc & 1;
-          const uint32_t qa = sbase + SM::Q_OFF + st * 2 * SM::U_BYTES, da = qa + SM::U_BYTES;
+          const uint32_t st = uc % GRAD_STAGES, g = uc & 1;
+          const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
           if (!mbar_wait(bar_pf + 8 * g, (uc >> 1) & 1, abort_flag, status, 74)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulators
-          if (it == 0 && nk > 0 && !mbar_wait(bar_of, (nk - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
+          if (it == 0 && nt > 0 && !mbar_wait(bar_of, (nt - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
           tc_fence_after();
+          // A = P or dS from TMEM: 16 of the unit are 8 columns; B = the unit's rows (MN-major: chunks of 64 of the width are U_CHUNK apart)
+          if constexpr (KEYS) {
 #pragma unroll
-          for (int k = 0; k < DKV_UNIT / 16; k++)
-            umma_ts_f16(tmem_base + 256u, tmem_base + g * 128u + (uint32_t)(k * 8), make_smem_desc(da + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < GRAD_UNIT / 16; k++)
+              umma_ts_f16(tmem_base + 256u, tmem_base + g * 128u + (uint32_t)(k * 8), make_smem_desc(ub + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+          }
 #pragma unroll
-          for (int k = 0; k < DKV_UNIT / 16; k++)
-            umma_ts_f16(tmem_base + 256u + (uint32_t)D, tmem_base + g * 128u + 64u + (uint32_t)(k * 8), make_smem_desc(qa + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc,
-                        (it > 0 || k > 0) ? 1u : 0u);
-          tc_commit(bar_qe + 8 * st);
+          for (int k = 0; k < GRAD_UNIT / 16; k++)
+            umma_ts_f16(tmem_base + 256u + (KEYS ? (uint32_t)D : 0u), tmem_base + g * 128u + 64u + (uint32_t)(k * 8), make_smem_desc(ua + (uint32_t)k * 2048, U_CHUNK, 1024),
+                        p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+          tc_commit(bar_ue + 8 * st);
           if (it + 1 == total) tc_commit(bar_end);
           uc++;
           // the tensor pipe keeps this thread's order: the pair's next scores come after the products that read it
           if (it + 2 < total && !issue_scores(it + 3 == total)) { ok = false; break; }
         }
-        nk++;
+        nt++;
       }
       // everything this thread issued must retire before TMEM is released
       tc_commit(bar_drain);
       mbar_wait(bar_drain, 0, abort_flag, nullptr, 0);
     }
   } else if (warp >= 4) {
-    // ---------------------------------------------- P^T and dS^T ----------------------------------------------------
+    // ---------------------------------------------- P and dS --------------------------------------------------------
     const int g = (warp - 4) >> 2;                // this group's pair of buffers: units of this parity
     const int quad = warp & 3, row = quad * 32 + lane, tid = (int)threadIdx.x - 128 - g * 128;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(g * 128);
-    uint32_t uc = 0, mine = 0, nk = 0;            // units of all groups before this tile, this group's units, tiles with work
+    uint32_t uc = 0, mine = 0, nt = 0;            // units of all groups before this tile, this group's units, tiles with work
     bool ok = true;
     for (int n = 0; ok; n++) {
       if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
-      const int t = s->tile, units = s->blocks, b = s->b, u = s->h, j0 = s->at;
+      const int t = s->tile, units = s->blocks, b = s->b, th = s->h, at = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
       if (t < 0) break;
-      const int key = j0 + row;
-      const bool there = key < seq.length;
-      // the first query that sees this key; none where there is no such key
-      const int from = !there ? 0x3fffffff : p.a.causal && key >= seq.prefix ? key - seq.first : -0x3fffffff;
-      const int doc = p.a.documents && key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + key) : 0;
-      const int total = units * p.a.group;
+      const int total = units * repeat, self = at + row;   // this row's query or key
+      // queries: keys up to `edge` are seen; keys: queries from `edge` on see this key
+      const int pos = KEYS ? self : seq.first + self;
+      int edge;
+      bool there;
+      if constexpr (KEYS) {
+        there = self < seq.length;
+        edge = !there ? 0x3fffffff : p.a.causal && self >= seq.prefix ? self - seq.first : -0x3fffffff;
+      } else {
+        there = !p.a.documents || (pos >= 0 && pos < p.a.Sk);
+        edge = there ? head_limit(p.a, seq, pos) - 1 : -1;
+      }
+      const int doc = p.a.documents && pos >= 0 && pos < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos) : 0;
+      uint64_t nl2 = 0, nd2 = 0;
+      if constexpr (!KEYS) {
+        const int64_t rc = ((int64_t)b * p.a.Hq + th) * p.rows + self;
+        nl2 = splat2(ld_global(p.neg_lse + rc)); nd2 = splat2(ld_global(p.neg_delta + rc));
+      }
       BlockWalk walk;
-      int hh = 0, it = 0;                          // head of the group, unit of the head
-      // a unit's row constants: one value per thread, fetched a unit ahead
-      auto fetch = [&](int h, int unit) {
-        const int64_t at = ((int64_t)b * p.a.Hq + u * p.a.group + h) * p.rows + unit * DKV_UNIT + (tid & 63);
-        return tid < 64 ? ld_global(p.neg_lse + at) : ld_global(p.neg_delta + at);
+      int hh = 0, it = 0;                          // head that passes by, unit of the head
+      // keys: a unit's row constants, one value per thread, fetched a unit ahead
+      auto fetch = [&](int head, int unit) {
+        const int64_t rc = ((int64_t)b * p.a.Hq + th * p.a.group + head) * p.rows + unit * GRAD_UNIT + (tid & 63);
+        return ld_global((tid < 64 ? p.neg_lse : p.neg_delta) + rc);
       };
       auto advance = [&]() {                       // to the next unit, over the end of a head
-        if (++it == units) { it = 0; hh++; if (hh < p.a.group) walk.start(s, listed); }
+        if (++it == units) { it = 0; hh++; if (hh < repeat) walk.start(s, listed); }
         else walk.next();
       };
       int k = 0;
       float ahead = 0.f;
       if (total > 0) {
         walk.start(s, listed);
-        if (((uc + (uint32_t)k) & 1) != (uint32_t)g) { k++; advance(); }
-        if (k < total) ahead = fetch(hh, walk.j);
+        if ((uc & 1) != (uint32_t)g) { k++; advance(); }
+        if (KEYS && k < total) ahead = fetch(hh, walk.j);
       }
       while (k < total && ok) {
-        const int unit = walk.j, h = u * p.a.group + hh;
+        const int unit = walk.j, head = KEYS ? th * p.a.group + hh : th;
+        const uint32_t stage = (uc + (uint32_t)k) % GRAD_STAGES;
         const bool compare = listed ? (s->compare[unit >> 5] >> (unit & 31)) & 1 : p.a.documents != nullptr;
         const uint32_t rows_at = sbase + (uint32_t)(SM::ROW_OFF + (g * 2 + (int)(mine & 1)) * 512);
-        asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_at + (uint32_t)tid * 4), "f"(ahead) : "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_rf + 8 * g);
+        if constexpr (KEYS) {
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(rows_at + (uint32_t)tid * 4), "f"(ahead) : "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_rf + 8 * g);
+        }
         k += 2;
         advance();
-        if (k - 1 < total) { advance(); if (k < total) ahead = fetch(hh, walk.j); }
+        if (k - 1 < total) { advance(); if (KEYS && k < total) ahead = fetch(hh, walk.j); }
         // the group's four warps have stored theirs (and read those of two units ago)
-        if (!mbar_wait(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
+        if (KEYS && !mbar_wait(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
         if (!mbar_wait(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
         tc_fence_after();
-        const int i0 = unit * DKV_UNIT;            // the unit's first query
-        const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
-        const bool masked = compare || __any_sync(0xffffffffu, from > i0);
+        const int u0 = unit * GRAD_UNIT;           // the unit's first key or query
+        const float slope = p.a.slopes ? ld_global(p.a.slopes + head) * kLog2e : 0.f;
+        const bool masked = compare || __any_sync(0xffffffffu, KEYS ? edge > u0 : edge < u0 + GRAD_UNIT - 1);
+        if constexpr (!KEYS) {
+          if (p.a.lengths && seq.length < p.a.Sk && seq.length < u0 + GRAD_UNIT) {
+            // keys behind the sequence's end: zero before they meet their dS of zero (the scores have been computed: K has landed)
+            if (tid < GRAD_UNIT && u0 + tid >= seq.length) {
+#pragma unroll 1
+              for (int c = 0; c < DC; c++)
+#pragma unroll
+                for (int q = 0; q < 8; q++) sts_v4(sbase + (uint32_t)SM::U_OFF + stage * 2 * SM::U_BYTES + (uint32_t)(c * U_CHUNK + tid * 128 + q * 16), 0, 0, 0, 0);
+            }
+            fence_async_shared();
+          }
+        }
         uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
         if (masked) {
 #pragma unroll
           for (int c = 0; c < 2; c++) {
-            const int q0 = i0 + c * 32;
-            seen[c] = ~ha_bits(min(max(from - q0, 0), 32) - 1);
+            const int first = u0 + c * 32;
+            seen[c] = KEYS ? ~ha_bits(min(max(edge - first, 0), 32) - 1) : ha_bits(edge - first);
             if (compare) {
-              const int pos = seq.first + q0 + lane;
-              const bool has = pos >= 0 && pos < p.a.Sk && q0 + lane < p.a.Sq;
-              const int theirs = has ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos) : 0;
+              const int other = KEYS ? seq.first + first + lane : first + lane;    // position
+              const bool has = other >= 0 && other < p.a.Sk && (!KEYS || first + lane < p.a.Sq);
+              const int theirs = has ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + other) : 0;
               seen[c] &= ha_same_document(doc, theirs, has);
             }
           }
         }
         int cap = 0;
         if (p.cap.cap > 0.f) {
-          uint32_t t[32];
-          tmem_ld_32x32(s_addr, t);
+          uint32_t v[32];
+          tmem_ld_32x32(s_addr, v);
           tc_wait_ld();
-          float largest = ha_largest(t);
-          tmem_ld_32x32(s_addr + 32u, t);
+          float largest = ha_largest(v);
+          tmem_ld_32x32(s_addr + 32u, v);
           tc_wait_ld();
-          largest = max3(largest, ha_largest(t), 0.f);
+          largest = max3(largest, ha_largest(v), 0.f);
           cap = __all_sync(0xffffffffu, largest <= p.cap.small) ? 1 : 2;
         }
+        // distance of this row from the unit's first
+        const float far = (float)(KEYS ? self - seq.first - u0 : pos - u0);
         grad_choose(cap, slope != 0.f, masked, [&](auto C, auto S, auto M) {
-          uint32_t sr[2][16], dr[2][16];
-          tmem_ld_32x16(s_addr, sr[0]);
-          tmem_ld_32x16(s_addr + 64u, dr[0]);
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; c++) {
-            grad_wait(sr[c & 1], dr[c & 1]);
-            if (c < 3) {                            // the next sixteen are on their way while these are worked on
-              tmem_ld_32x16(s_addr + (uint32_t)((c + 1) * 16), sr[(c + 1) & 1]);
-              tmem_ld_32x16(s_addr + 64u + (uint32_t)((c + 1) * 16), dr[(c + 1) & 1]);
-            }
-            const uint32_t nl_at = rows_at + (uint32_t)(c * 64), nd_at = nl_at + 256;
-            uint64_t nlv[8], ndv[8];
+            uint32_t sr[16], dr[16], pw[8], dw[8];
+            tmem_ld_32x16(s_addr + (uint32_t)(c * 16), sr);
+            tmem_ld_32x16(s_addr + 64u + (uint32_t)(c * 16), dr);
+            const uint32_t bits = (c < 2 ? seen[0] : seen[1]) >> (16 * (c & 1));
+            if constexpr (KEYS) {
+              const uint32_t nl_at = rows_at + (uint32_t)(c * 64), nd_at = nl_at + 256;
+              uint64_t nlv[8], ndv[8];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              uint32_t w0, w1, w2, w3;
-              lds_v4(nl_at + (uint32_t)(i * 16), w0, w1, w2, w3);
-              nlv[2 * i] = pack2(w0, w1); nlv[2 * i + 1] = pack2(w2, w3);
-              lds_v4(nd_at + (uint32_t)(i * 16), w0, w1, w2, w3);
-              ndv[2 * i] = pack2(w0, w1); ndv[2 * i + 1] = pack2(w2, w3);
+              for (int i = 0; i < 4; i++) {
+                uint32_t w0, w1, w2, w3;
+                lds_v4(nl_at + (uint32_t)(i * 16), w0, w1, w2, w3);
+                nlv[2 * i] = pack2(w0, w1); nlv[2 * i + 1] = pack2(w2, w3);
+                lds_v4(nd_at + (uint32_t)(i * 16), w0, w1, w2, w3);
+                ndv[2 * i] = pack2(w0, w1); ndv[2 * i + 1] = pack2(w2, w3);
+              }
+              grad_wait(sr, dr);
+              grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr, dr, [&](int i) { return nlv[i]; }, [&](int i) { return ndv[i]; }, slope, far - (float)(c * 16),
+                                                                                         bits, pw, dw);
+              // words of 16 queries into 8 columns that this row has read
+              tmem_st_32x8(s_addr + (uint32_t)(c * 8), pw);
+            } else {
+              grad_wait(sr, dr);
+              grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr, dr, [&](int) { return nl2; }, [&](int) { return nd2; }, slope, far - (float)(c * 16), bits, pw, dw);
             }
-            uint32_t pw[8], dw[8];
-            grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr[c & 1], dr[c & 1], [&](int i) { return nlv[i]; }, [&](int i) { return ndv[i]; }, slope, (float)(key - seq.first - i0 - c * 16),
-                                          seen[c >> 1] >> (16 * (c & 1)), pw, dw);
-            // words of 16 queries into 8 columns that this row has read
-            tmem_st_32x8(s_addr + (uint32_t)(c * 8), pw);
             tmem_st_32x8(s_addr + 64u + (uint32_t)(c * 8), dw);
           }
         });
@@ -766,14 +509,20 @@ k_attention_dkv(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1));   // the tile's list has been walked
       if (total > 0) {
-        if (!mbar_wait(bar_end, nk & 1, abort_flag, status, 83)) { ok = false; break; }
+        if (!mbar_wait(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
         tc_fence_after();
-        nk++;
+        nt++;
       }
-      // one group writes dV, the other dK
-      const B2xHeadStrides& o = g == 0 ? p.a.dvs : p.a.dks;
-      char* out = (g == 0 ? p.a.dv : p.a.dk) + 2 * ((int64_t)b * o.batch + (int64_t)u * o.head + (int64_t)key * o.token);
-      grad_write_row<EL, D>(tmem_base + lane_addr + 256u + (uint32_t)(g * D), out, key < p.a.Sk, p.a.D, g == 0 ? 1.f : p.scale, total == 0);
+      if constexpr (KEYS) {
+        // one group writes dV, the other dK
+        const B2xHeadStrides& o = g == 0 ? p.a.dvs : p.a.dks;
+        char* out = (g == 0 ? p.a.dv : p.a.dk) + 2 * ((int64_t)b * o.batch + (int64_t)th * o.head + (int64_t)self * o.token);
+        grad_write_row<EL, D>(tmem_base + lane_addr + 256u + (uint32_t)(g * D), out, self < p.a.Sk, p.a.D, g == 0 ? 1.f : p.scale, total == 0);
+      } else {
+        // each group writes half of the width
+        char* out = p.a.dq + 2 * ((int64_t)b * p.a.dqs.batch + (int64_t)th * p.a.dqs.head + (int64_t)self * p.a.dqs.token + g * (D / 2));
+        grad_write_row<EL, D / 2>(tmem_base + lane_addr + 256u + (uint32_t)(g * (D / 2)), out, self < p.a.Sq, p.a.D - g * (D / 2), p.scale, total == 0);
+      }
       tc_fence_before();
       __syncwarp();
       if (total > 0 && lane == 0) mbar_arrive(bar_of);
@@ -823,59 +572,49 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
   }
 }
 
-template <typename K, typename... A>
-int grad_launch(K kern, std::atomic<bool>* configured, int smem, int ctas, cudaStream_t stream, A&&... args) {
+// The tiles of one side: dQ, or with KEYS dK and dV
+template <int D, int EL, bool KEYS>
+int launch_side(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* status, cudaStream_t stream) {
+  static std::atomic<bool> ready[64];
+  const int tokens = KEYS ? a.Sk : a.Sq, others = KEYS ? a.Sq : a.Sk;
+  if (tokens == 0) return 0;
+  const int64_t all = (int64_t)a.B * (KEYS ? a.Hk : a.Hq);
+  p.tiles = (tokens + HA_BLOCK - 1) / HA_BLOCK;
+  if (all * p.tiles > 0x7fffff00) return (int)cudaErrorInvalidValue;
+  p.total = (int)(all * p.tiles);
+  // what passes by (K and V of a key head, or Q and dO of its query heads) stays in L2 for a group of heads: 32 MiB, as in the
+  // forward pass
+  const int64_t fit = (32ll << 20) / ((int64_t)(others > 0 ? others : 1) * a.D * 4), heads = KEYS ? fit / a.group : fit * a.group, least = KEYS ? 1 : a.group;
+  p.group_heads = (int)(heads < least ? (least < all ? least : all) : heads > all ? all : heads);
+  // longer sequences than a list of units covers walk all of theirs, and compare in each
+  p.ranges = a.documents && (others + GRAD_UNIT - 1) / GRAD_UNIT <= HA_MASK_WORDS * 32 ? ranges : nullptr;
+  const uint32_t format = EL == EL_BF16 ? 1u : 0u;
+  p.idesc_s = sm100::make_idesc(format, false, false, HA_BLOCK, GRAD_UNIT);
+  p.idesc_acc = sm100::make_idesc(format, false, true, HA_BLOCK, D);
+  CUtensorMap t0, t1, u0, u1;
+  const uint32_t q_rows = KEYS ? GRAD_UNIT : HA_BLOCK, k_rows = KEYS ? HA_BLOCK : GRAD_UNIT;
+  CUtensorMap &q = KEYS ? u0 : t0, &d = KEYS ? u1 : t1, &k = KEYS ? t0 : u0, &v = KEYS ? t1 : u1;
+  if (a.Sq > 0 && (!ha_encode(&q, EL, a.q, a.qs, a.B, a.Hq, a.Sq, a.D, q_rows) || !ha_encode(&d, EL, a.dout, a.dos, a.B, a.Hq, a.Sq, a.D, q_rows))) return (int)cudaErrorInvalidValue;
+  if (a.Sk > 0 && (!ha_encode(&k, EL, a.k, a.ks, a.B, a.Hk, a.Sk, a.D, k_rows) || !ha_encode(&v, EL, a.v, a.vs, a.B, a.Hk, a.Sk, a.D, k_rows))) return (int)cudaErrorInvalidValue;
+  if (others == 0) { u0 = t0; u1 = t1; }      // nothing is loaded
+  auto kern = k_attention_gradient<D, EL, KEYS>;
+  using SM = GradSmem<D>;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev < 0 || dev >= 64 || !ready[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::TOTAL);
     if (e != cudaSuccess) return (int)e;
-    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+    if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)ctas), dim3(384), smem, stream, args...);
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(384), SM::TOTAL, stream, t0, t1, u0, u1, p, sched_slot(stream), status);
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();
 }
-
 template <int D, int EL>
-int launch_gradient(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* status, cudaStream_t stream) {
-  static std::atomic<bool> dq_ready[64], dkv_ready[64];
-  const int elem = EL;
-  const uint32_t format = EL == EL_BF16 ? 1u : 0u;
-  int32_t* sched = sched_slot(stream);
-  CUtensorMap q, d, k, v;
-  // K and V of a group of heads stay in L2 together (dQ), or Q and dO (dK, dV): 32 MiB, as in the forward pass
-  if (a.Sq > 0) {
-    p.tiles = p.rows / HA_BLOCK;
-    const int64_t kv = (32ll << 20) / ((int64_t)(a.Sk > 0 ? a.Sk : 1) * a.D * 4), heads = kv < 1 ? a.group : kv * a.group, all = (int64_t)a.B * a.Hq;
-    p.group_heads = (int)(heads > all ? all : heads);
-    if (all * p.tiles > 0x7fffff00) return (int)cudaErrorInvalidValue;
-    p.total = (int)(all * p.tiles);
-    p.ranges = a.documents && p.key_blocks <= HA_MASK_WORDS * 32 ? ranges : nullptr;
-    p.idesc_s = sm100::make_idesc(format, false, false, HA_BLOCK, HA_BLOCK);
-    p.idesc_acc = sm100::make_idesc(format, false, true, HA_BLOCK, D);
-    if (!ha_encode(&q, elem, a.q, a.qs, a.B, a.Hq, a.Sq, a.D) || !ha_encode(&d, elem, a.dout, a.dos, a.B, a.Hq, a.Sq, a.D)) return (int)cudaErrorInvalidValue;
-    if (a.Sk == 0) k = v = q;      // nothing is loaded
-    else if (!ha_encode(&k, elem, a.k, a.ks, a.B, a.Hk, a.Sk, a.D) || !ha_encode(&v, elem, a.v, a.vs, a.B, a.Hk, a.Sk, a.D)) return (int)cudaErrorInvalidValue;
-    const int rc = grad_launch(k_attention_dq<D, EL>, dq_ready, DqSmem<D>::TOTAL, p.total < kNumSms ? p.total : kNumSms, stream, q, d, k, v, p, sched, status);
-    if (rc) return rc;
-  }
-  if (a.Sk > 0) {
-    p.tiles = p.key_blocks;
-    const int64_t fit = (32ll << 20) / ((int64_t)(a.Sq > 0 ? a.Sq : 1) * a.D * 4 * a.group), all = (int64_t)a.B * a.Hk;
-    p.group_heads = (int)(fit < 1 ? 1 : fit > all ? all : fit);
-    if (all * p.tiles > 0x7fffff00) return (int)cudaErrorInvalidValue;
-    p.total = (int)(all * p.tiles);
-    p.ranges = a.documents && (a.Sq + DKV_UNIT - 1) / DKV_UNIT <= HA_MASK_WORDS * 32 ? ranges : nullptr;
-    p.idesc_s = sm100::make_idesc(format, false, false, HA_BLOCK, DKV_UNIT);
-    p.idesc_acc = sm100::make_idesc(format, false, true, HA_BLOCK, D);
-    if (!ha_encode(&k, elem, a.k, a.ks, a.B, a.Hk, a.Sk, a.D) || !ha_encode(&v, elem, a.v, a.vs, a.B, a.Hk, a.Sk, a.D)) return (int)cudaErrorInvalidValue;
-    if (a.Sq == 0) q = d = k;
-    else if (!ha_encode(&q, elem, a.q, a.qs, a.B, a.Hq, a.Sq, a.D, DKV_UNIT) || !ha_encode(&d, elem, a.dout, a.dos, a.B, a.Hq, a.Sq, a.D, DKV_UNIT)) return (int)cudaErrorInvalidValue;
-    return grad_launch(k_attention_dkv<D, EL>, dkv_ready, DkvSmem<D>::TOTAL, p.total < kNumSms ? p.total : kNumSms, stream, q, d, k, v, p, sched, status);
-  }
-  return 0;
+int launch_gradient(const HeadAttn& a, const GradParams& p, const int2* ranges, int32_t* status, cudaStream_t stream) {
+  const int rc = launch_side<D, EL, false>(a, p, ranges, status, stream);
+  return rc ? rc : launch_side<D, EL, true>(a, p, ranges, status, stream);
 }
 
 int grad_rows(int64_t Sq) { return (int)((Sq + HA_BLOCK - 1) / HA_BLOCK * HA_BLOCK); }
