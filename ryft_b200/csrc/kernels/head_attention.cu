@@ -4,7 +4,8 @@
 // Gradient: P = exp(s - lse), dP = dO V^T, delta = sum(dO * O), dS = P (dP - delta) (1 - tanh^2) scale; dQ = dS K, dK = dS^T Q,
 // dV = P^T dO, the last two over all query heads that share the key head.  Sums, statistics and scores in f32.
 //
-// The entry points; the kernels are in head_attention_tc.cu (forward) and head_attention_gradient.cu.
+// The entry points; the kernels are in head_attention_tc.cu (forward), head_attention_token.cu (few queries) and
+// head_attention_gradient.cu.
 #include <cmath>
 
 #include "head_attention_tc.cuh"
@@ -19,7 +20,7 @@ bool ha_rows(const void* p, const B2xHeadStrides& s, int64_t B, int64_t H, int64
 bool ha_valid(const B2xHeadAttentionArgs* a) {
   return ha_rows(a->q, a->qs, a->B, a->Hq, a->Sq) && ha_rows(a->k, a->ks, a->B, a->Hk, a->Sk) && ha_rows(a->v, a->vs, a->B, a->Hk, a->Sk) &&
          ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 &&
-         (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) && (a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e6f)) && std::fabs(a->scale) <= 1e6f &&
+         (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) && a->B * a->Hk < (1ll << 31) && (a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e6f)) && std::fabs(a->scale) <= 1e6f &&
          a->Sq < (1ll << 30) && a->Sk < (1ll << 30) && a->query_offset >= 0 && a->query_offset < (1ll << 30) && (!a->queries_at_end || a->lengths);
 }
 
@@ -43,18 +44,24 @@ HeadAttn ha_params(const B2xHeadAttentionArgs* a) {
 
 extern "C" int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* a, int gradient) {
   const int64_t ranges = a->documents ? a->B * ((a->Sk + b2x::HA_BLOCK - 1) / b2x::HA_BLOCK) * 8 : 0;
-  return gradient ? b2x::ha_gradient_scratch(a) + ranges : ranges;
+  if (gradient) return b2x::ha_gradient_scratch(a) + ranges;
+  const b2x::HeadAttn p = b2x::ha_params(a);
+  return b2x::ha_token_takes(p) ? b2x::ha_token_scratch(p) : ranges;
 }
 
 extern "C" int b2x_head_attention_launches(const B2xHeadAttentionArgs* a, int gradient) {
   const int q = a->B * a->Hq * a->Sq > 0, k = a->B * a->Hk * a->Sk > 0, ranges = k && a->documents;
-  return gradient ? ranges + 2 * q + k : q + (q ? ranges : 0);
+  if (gradient) return ranges + 2 * q + k;
+  const b2x::HeadAttn p = b2x::ha_params(a);
+  return !q ? 0 : b2x::ha_token_takes(p) ? b2x::ha_token_launches(p) : 1 + ranges;
 }
 
 extern "C" int b2x_launch_head_attention(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
   if (!ha_valid(a) || (b2x_head_attention_scratch_bytes(a, 0) > 0 && !a->scratch)) return (int)cudaErrorInvalidValue;
-  return ha_launch_forward(ha_params(a), a->elem, (int2*)a->scratch, status, (cudaStream_t)stream);
+  const HeadAttn p = ha_params(a);
+  if (ha_token_takes(p)) return ha_launch_token(p, a->elem, a->scratch, (cudaStream_t)stream);
+  return ha_launch_forward(p, a->elem, (int2*)a->scratch, status, (cudaStream_t)stream);
 }
 
 extern "C" int b2x_launch_head_attention_gradient(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {

@@ -164,6 +164,10 @@ int32_t* sched_slot(cudaStream_t stream);   // gemm_tc.cu: a (tile counter, fini
 
 // Blocks of 128 tokens and the launches of the entry points.
 int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream);
+bool ha_token_takes(const HeadAttn& p);
+int64_t ha_token_scratch(const HeadAttn& p);
+int ha_token_launches(const HeadAttn& p);
+int ha_launch_token(const HeadAttn& p, int elem, void* scratch, cudaStream_t stream);
 int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a);
 int ha_launch_gradient(const HeadAttn& p, int elem, void* scratch, int32_t* status, cudaStream_t stream);
 int ha_launch_forward(const HeadAttn& p, int elem, int2* ranges, int32_t* status, cudaStream_t stream);
