@@ -2,28 +2,28 @@
 //
 // Bound by HBM: keys and values are read once, 4 * rows flops for every 2 bytes of them.  The query heads that share a key head are
 // the rows of one tile of 16, so that a cache line serves all of them.  The keys of a sequence are cut into chunks, a CTA of four
-// warps each, whatever the batch: long sequences spread over the chip, chunks behind a short one's end leave at once.  A warp takes
-// 16 keys at a time from memory straight into the fragments of m16n8k16 products, the next 16 in flight meanwhile; nothing passes
-// through shared memory and no warp waits for another before the end.  (The 128-row tiles of tcgen05 would be empty but for a few
-// rows; the products here are a fifth of the time that the loads take.)
-//
-// 16-byte loads without shuffles: a product over d does not depend on the order of d, so four neighbouring lanes take 8 adjacent
-// elements each of a key's row (and of a query's) for two k-steps; and the columns of a result may come in any order, so eight
-// lanes take 8 adjacent elements each of a value's row, element i of each belonging to product i.  A lane ends up with 16 adjacent
-// elements of its two rows.
+// warps each, whatever the batch: long sequences spread over the chip, chunks behind a short one's end leave at once.  A warp walks
+// steps of 16 keys through a ring of its own in shared memory, filled two steps ahead by asynchronous copies of 16 bytes (keys
+// behind the sequence's end are filled with zeros, so that nothing that lies there meets a product), and multiplies with m16n8k16
+// from there; no warp waits for another before the end.  (The 128-row tiles of tcgen05 would be empty but for a few rows; the
+// products here are a fifth of the time that the loads take.)  Straight into registers, with one step in flight, the loads
+// reached 3.2 TB/s: their latency showed, and 520 instructions per step went into placing them.
 //
 // Each warp keeps its own maximum (raised only when a score passes it by 2^8), sum and accumulator; the four meet in shared memory,
 // chunks in a second launch that weighs them by their maxima.  Order of sums: fixed.
+#include <atomic>
+
 #include "head_attention_tc.cuh"
 
 namespace b2x {
 namespace {
 
-constexpr int TOKEN_ROWS = 16, TOKEN_WARPS = 4;
+constexpr int TOKEN_ROWS = 16, TOKEN_WARPS = 4, TOKEN_STAGES = 3;
 
 struct TokenParams {
   HeadAttn a;
   int32_t rows, row_tiles;     // of a key head: Sq * group, and tiles of 16
+  int32_t tiles;               // of all key heads and sequences
   int32_t chunk, chunks;       // keys per CTA; CTAs per tile
   float mult;                  // scale * log2(e)
   float cap, cap_in;           // cap * log2(e) and the exponent 2 * scale / cap * log2(e); 0: none
@@ -39,8 +39,17 @@ template <int EL> __device__ __forceinline__ void token_mma(float (&d)[4], const
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t token_low(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x5410); }
-__device__ __forceinline__ uint32_t token_high(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }
+__device__ __forceinline__ void token_ldsm(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void token_ldsm_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes to shared memory, or zeros
+__device__ __forceinline__ void token_copy(uint32_t dst, const char* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(on ? 16 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void token_arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // row of a tile -> query head and query
 struct TokenRow { int h, i; bool there; };
@@ -50,15 +59,25 @@ __device__ __forceinline__ TokenRow token_row(const TokenParams& p, int u, int r
   return {u * p.a.group + (there ? row - i * p.a.group : 0), i, there};
 }
 
+template <int D> struct TokenSmem {
+  static constexpr int STEP_BYTES = 2 * 16 * D * 2;            // 16 keys and their values
+  static constexpr int RING_BYTES = TOKEN_STAGES * STEP_BYTES; // of a warp
+  static constexpr int ROW = D + 4;                            // floats per row where the warps meet (in the rings' place)
+  static constexpr int MEET_BYTES = TOKEN_WARPS * TOKEN_ROWS * ROW * 4 + TOKEN_WARPS * TOKEN_ROWS * 8;
+  static constexpr int TOTAL = TOKEN_WARPS * RING_BYTES > MEET_BYTES ? TOKEN_WARPS * RING_BYTES : MEET_BYTES;
+};
+
 template <int D, int EL>
 __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const __grid_constant__ TokenParams p) {
-  constexpr int KJ = D / 32, VJ = D / 64;
-  __shared__ float so[TOKEN_WARPS][TOKEN_ROWS][D + 4];
-  __shared__ float2 sml[TOKEN_WARPS][TOKEN_ROWS];
+  using SM = TokenSmem<D>;
+  constexpr int PIECES = D / 8;                // 16-byte pieces of a row
+  constexpr int LOADS = 16 * PIECES / 32;      // copies of a lane for 16 rows
+  extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const int tile = (int)(blockIdx.x / (unsigned)p.chunks), chunk = (int)(blockIdx.x - (unsigned)tile * (unsigned)p.chunks);
+  // chunks of all heads and sequences in turn: heads that lie side by side in memory are read at the same time
+  const int tile = (int)(blockIdx.x % (unsigned)p.tiles), chunk = (int)(blockIdx.x / (unsigned)p.tiles);
   const int rt = tile % p.row_tiles, bu = tile / p.row_tiles, b = bu / p.a.Hk, u = bu - b * p.a.Hk;
   const HeadSequence seq = head_sequence(p.a, b);
   const int r0 = rt * TOKEN_ROWS, r_last = min(r0 + TOKEN_ROWS, p.rows) - 1;
@@ -66,94 +85,119 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
   const int k_begin = chunk * p.chunk, k_end = min(k_begin + p.chunk, end);
   const bool work = k_begin < k_end;
   if (work || p.chunks == 1) {
+    const uint32_t ring = sm100::smem_u32(smem) + (uint32_t)warp * SM::RING_BYTES;
+    // copies: this lane's pieces are rows (lane / PIECES) + i * (32 / PIECES), swizzled within groups of eight pieces
+    const int piece = lane % PIECES, row_in = lane / PIECES;
+    const bool wide = piece * 8 < p.a.D;
+    const char* kp = p.a.k + 2 * ((int64_t)b * p.a.ks.batch + (int64_t)u * p.a.ks.head + piece * 8);
+    const char* vp = p.a.v + 2 * ((int64_t)b * p.a.vs.batch + (int64_t)u * p.a.vs.head + piece * 8);
+    auto fill = [&](int stage, int k0) {       // the 16 keys from k0 on; always one group, of nothing behind the chunk
+      if (k0 < k_end) {
+        const uint32_t at = ring + (uint32_t)stage * SM::STEP_BYTES;
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+          const int row = row_in + i * (32 / PIECES), key = k0 + row;
+          const uint32_t dst = at + (uint32_t)(row * D * 2 + (piece & ~7) * 16 + (((piece ^ row) & 7) << 4));
+          const bool on = wide && key < k_end;
+          const int64_t from = on ? key : k_begin;
+          token_copy(dst, kp + (wide ? 2 * from * p.a.ks.token : 0), on);
+          token_copy(dst + 16 * D * 2, vp + (wide ? 2 * from * p.a.vs.token : 0), on);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int k0 = k_begin + warp * 16;
+#pragma unroll
+    for (int st = 0; st < TOKEN_STAGES - 1; st++) fill(st, k0 + st * TOKEN_WARPS * 16);
+
     // this lane's rows r and r + 8
     TokenRow row[2];
     int lim[2], doc[2];
     float slope[2], pos[2];
-    uint32_t qf[2 * KJ][4];
+    uint32_t qf[D / 16][4];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
       row[x] = token_row(p, u, r0 + r + 8 * x);
       const int at = seq.first + row[x].i;
-      lim[x] = row[x].there ? head_limit(p.a, seq, at) : 0;
+      lim[x] = row[x].there ? head_limit(p.a, seq, at) : 0x7fffffff;    // a row that is not there may see what it likes
       doc[x] = 0;
       if (p.a.documents) {
         if (at >= 0 && at < p.a.Sk) doc[x] = (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + at);
-        else lim[x] = 0;
+        else if (row[x].there) lim[x] = 0;
       }
       slope[x] = p.a.slopes ? ld_global(p.a.slopes + row[x].h) * kLog2e : 0.f;
       pos[x] = (float)at;
       const char* q = p.a.q + 2 * ((int64_t)b * p.a.qs.batch + (int64_t)row[x].h * p.a.qs.head + (int64_t)row[x].i * p.a.qs.token);
 #pragma unroll
-      for (int j = 0; j < KJ; j++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row[x].there && 32 * j + 8 * c < p.a.D) v = ld_global((const uint4*)(q + 2 * (32 * j + 8 * c)));
-        qf[2 * j][x] = v.x; qf[2 * j][2 + x] = v.y; qf[2 * j + 1][x] = v.z; qf[2 * j + 1][2 + x] = v.w;
-      }
+      for (int k = 0; k < D / 16; k++)
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const int d = 16 * k + 8 * y + 2 * c;
+          qf[k][x + 2 * y] = row[x].there && d < p.a.D ? ld_global((const uint32_t*)(q + 2 * d)) : 0u;
+        }
     }
-    const char* kp = p.a.k + 2 * ((int64_t)b * p.a.ks.batch + (int64_t)u * p.a.ks.head);
-    const char* vp = p.a.v + 2 * ((int64_t)b * p.a.vs.batch + (int64_t)u * p.a.vs.head);
-    uint4 kf[2][KJ], vf[4][VJ];
-    auto load_k = [&](int k0) {
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-        const int key = k0 + 8 * m + r;
-#pragma unroll
-        for (int j = 0; j < KJ; j++) {
-          kf[m][j] = make_uint4(0, 0, 0, 0);
-          if (key < k_end && 32 * j + 8 * c < p.a.D) kf[m][j] = ld_global((const uint4*)(kp + 2 * ((int64_t)key * p.a.ks.token + 32 * j + 8 * c)));
-        }
-      }
-    };
-    auto load_v = [&](int k0) {
-#pragma unroll
-      for (int m = 0; m < 4; m++) {
-        const int key = k0 + 2 * c + (m & 1) + 8 * (m >> 1);
-#pragma unroll
-        for (int j = 0; j < VJ; j++) {
-          vf[m][j] = make_uint4(0, 0, 0, 0);
-          if (key < k_end && 64 * j + 8 * r < p.a.D) vf[m][j] = ld_global((const uint4*)(vp + 2 * ((int64_t)key * p.a.vs.token + 64 * j + 8 * r)));
-        }
-      }
-    };
-    float acc[8 * VJ][4], m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    // keys below `open` are seen by every row
+    const int open = !p.a.slopes && !p.a.documents ? __reduce_min_sync(0xffffffffu, min(lim[0], lim[1])) : 0;
+    float acc[PIECES][4], m_used[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     bool poisoned[2] = {false, false};
 #pragma unroll
-    for (int i = 0; i < 8 * VJ; i++)
+    for (int i = 0; i < PIECES; i++)
 #pragma unroll
       for (int x = 0; x < 4; x++) acc[i][x] = 0.f;
-    int k0 = k_begin + warp * 16;
-    if (k0 < k_end) { load_k(k0); load_v(k0); }
+    // fragments: keys as they lie (matrix lane / 8 of a load: pieces 4 q + lane / 8 of eight keys), values turned (keys 8 * (bit 3 of the
+    // lane), piece 2 q + (bit 4))
+    const uint32_t k_row = (uint32_t)(lane & 7), v_row = (uint32_t)((lane & 7) + (lane & 8));
+    int stage = 0;
     for (; k0 < k_end; k0 += TOKEN_WARPS * 16) {
-      const int next = k0 + TOKEN_WARPS * 16;
+      token_arrived<TOKEN_STAGES - 2>();
+      __syncwarp();
+      // the stage that the previous step read
+      fill(stage == 0 ? TOKEN_STAGES - 1 : stage - 1, k0 + (TOKEN_STAGES - 1) * TOKEN_WARPS * 16);
+      const uint32_t at = ring + (uint32_t)stage * SM::STEP_BYTES, vat = at + 16 * D * 2;
+      stage = stage == TOKEN_STAGES - 1 ? 0 : stage + 1;
       float s[2][4];
-#pragma unroll
-      for (int m = 0; m < 2; m++) {
-#pragma unroll
-        for (int x = 0; x < 4; x++) s[m][x] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KJ; j++) {
-          token_mma<EL>(s[m], qf[2 * j], kf[m][j].x, kf[m][j].y);
-          token_mma<EL>(s[m], qf[2 * j + 1], kf[m][j].z, kf[m][j].w);
-        }
-      }
-      if (next < k_end) load_k(next);
-      // element x of s[m]: row x >> 1, key k0 + 8 m + 2 c + (x & 1)
-      float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int m = 0; m < 2; m++)
 #pragma unroll
-        for (int x = 0; x < 4; x++) {
-          const int key = k0 + 8 * m + 2 * c + (x & 1), w = x >> 1;
-          float v = s[m][x];
-          if (p.cap > 0.f) v = p.cap - 2.f * p.cap * fast_rcp(1.f + fast_exp2(v * p.cap_in));
-          else v *= p.mult;
-          if (p.a.slopes) v = fmaf(fabsf(pos[w] - (float)key), -slope[w], v);
-          bool see = key < lim[w];
-          if (p.a.documents) see = see && (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + min(key, p.a.Sk - 1)) == doc[w];
-          s[m][x] = see ? v : -INFINITY;
-          most[w] = max3(most[w], s[m][x], -INFINITY);
+        for (int x = 0; x < 4; x++) s[m][x] = 0.f;
+#pragma unroll
+      for (int q = 0; q < D / 32; q++)
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          uint32_t f[4];
+          const uint32_t pc = (uint32_t)(4 * q) + (uint32_t)(lane >> 3);
+          token_ldsm(at + (k_row + 8 * m) * (D * 2) + (pc & ~7u) * 16 + (((pc ^ k_row) & 7) << 4), f);
+          token_mma<EL>(s[m], qf[2 * q], f[0], f[1]);
+          token_mma<EL>(s[m], qf[2 * q + 1], f[2], f[3]);
         }
+      // element x of s[m]: row x >> 1, key k0 + 8 m + 2 c + (x & 1)
+      if (p.cap > 0.f) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) s[m][x] = fmaf(-2.f * p.cap, fast_rcp(1.f + fast_exp2(s[m][x] * p.cap_in)), p.cap);
+      } else {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) s[m][x] *= p.mult;
+      }
+      if (k0 + 16 > open) {
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const int key = k0 + 8 * m + 2 * c + (x & 1), w = x >> 1;
+            float v = s[m][x];
+            if (p.a.slopes) v = fmaf(fabsf(pos[w] - (float)key), -slope[w], v);
+            bool see = key < lim[w] && key < k_end;
+            if (p.a.documents) see = see && (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + min(key, p.a.Sk - 1)) == doc[w];
+            s[m][x] = see ? v : -INFINITY;
+          }
+      }
+      float most[2];
+#pragma unroll
+      for (int w = 0; w < 2; w++) most[w] = max3(max3(s[0][2 * w], s[0][2 * w + 1], s[1][2 * w]), s[1][2 * w + 1], -INFINITY);
       // a NaN score makes its row NaN: noted here, kept out of the arithmetic
 #pragma unroll
       for (int w = 0; w < 2; w++) if (most[w] != most[w]) { poisoned[w] = true; most[w] = 0.f; }
@@ -169,7 +213,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
           m_used[w] = m;
         }
 #pragma unroll
-        for (int i = 0; i < 8 * VJ; i++) { acc[i][0] *= f[0]; acc[i][1] *= f[0]; acc[i][2] *= f[1]; acc[i][3] *= f[1]; }
+        for (int i = 0; i < PIECES; i++) { acc[i][0] *= f[0]; acc[i][1] *= f[0]; acc[i][2] *= f[1]; acc[i][3] *= f[1]; }
       }
       uint32_t pf[4];
       {
@@ -183,18 +227,19 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
         pf[2] = ha_pack<EL>(e[1][0], e[1][1]); pf[3] = ha_pack<EL>(e[1][2], e[1][3]);
       }
 #pragma unroll
-      for (int j = 0; j < VJ; j++) {
-        const uint32_t v0[4] = {vf[0][j].x, vf[0][j].y, vf[0][j].z, vf[0][j].w}, v1[4] = {vf[1][j].x, vf[1][j].y, vf[1][j].z, vf[1][j].w};
-        const uint32_t v2[4] = {vf[2][j].x, vf[2][j].y, vf[2][j].z, vf[2][j].w}, v3[4] = {vf[3][j].x, vf[3][j].y, vf[3][j].z, vf[3][j].w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          token_mma<EL>(acc[8 * j + 2 * i], pf, token_low(v0[i], v1[i]), token_low(v2[i], v3[i]));
-          token_mma<EL>(acc[8 * j + 2 * i + 1], pf, token_high(v0[i], v1[i]), token_high(v2[i], v3[i]));
-        }
+      for (int q = 0; q < PIECES / 2; q++) {
+        uint32_t f[4];
+        const uint32_t pc = (uint32_t)(2 * q) + (uint32_t)(lane >> 4);
+        token_ldsm_t(vat + v_row * (D * 2) + (pc & ~7u) * 16 + (((pc ^ v_row) & 7) << 4), f);
+        token_mma<EL>(acc[2 * q], pf, f[0], f[1]);
+        token_mma<EL>(acc[2 * q + 1], pf, f[2], f[3]);
       }
-      if (next < k_end) load_v(next);
     }
-    // ---- the four warps meet ----
+    // ---- the four warps meet, in the rings' place ----
+    token_arrived<0>();
+    __syncthreads();
+    float (*so)[TOKEN_ROWS][SM::ROW] = (float (*)[TOKEN_ROWS][SM::ROW])smem;
+    float2 (*sml)[TOKEN_ROWS] = (float2 (*)[TOKEN_ROWS])(smem + TOKEN_WARPS * TOKEN_ROWS * SM::ROW * 4);
 #pragma unroll
     for (int w = 0; w < 2; w++) {
       if (poisoned[w]) l[w] = __int_as_float(0x7fc00000);
@@ -212,13 +257,11 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
       f[w] = m_used[w] == -INFINITY ? 0.f : fast_exp2(m_used[w] - most);
     }
 #pragma unroll
-    for (int j = 0; j < VJ; j++)
+    for (int i = 0; i < PIECES; i++)
 #pragma unroll
-      for (int i = 0; i < 8; i++)
-#pragma unroll
-        for (int x = 0; x < 4; x++) so[warp][r + 8 * (x >> 1)][64 * j + 16 * c + 8 * (x & 1) + i] = acc[8 * j + i][x] * f[x >> 1];
+      for (int w = 0; w < 2; w++) *(float2*)&so[warp][r + 8 * w][8 * i + 2 * c] = make_float2(acc[i][2 * w] * f[w], acc[i][2 * w + 1] * f[w]);
     __syncthreads();
-    // thread: row, and every eighth element of it
+    // eight threads per row, two adjacent elements of every sixteen each
     const int orow = threadIdx.x >> 3;
     const TokenRow o = token_row(p, u, r0 + orow);
     if (o.there) {
@@ -233,7 +276,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
       for (int d = (threadIdx.x & 7) * 2; d < p.a.D; d += 16) {
         float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-        for (int k = 0; k < TOKEN_WARPS; k++) { v0 += so[k][orow][d]; v1 += so[k][orow][d + 1]; }
+        for (int k = 0; k < TOKEN_WARPS; k++) { const float2 v = *(const float2*)&so[k][orow][d]; v0 += v.x; v1 += v.y; }
         if (p.chunks > 1) *(float2*)(part + d) = make_float2(v0, v1);
         else *(uint32_t*)(out + 2 * d) = ha_pack<EL>(rl != rl ? rl : v0 * inv, rl != rl ? rl : v1 * inv);
       }
@@ -297,6 +340,7 @@ void token_shape(const HeadAttn& a, TokenParams* p) {
   p->rows = a.Sq * a.group;
   p->row_tiles = (p->rows + TOKEN_ROWS - 1) / TOKEN_ROWS;
   const int64_t tiles = (int64_t)a.B * a.Hk * p->row_tiles;
+  p->tiles = (int)tiles;
   // about eight CTAs per SM where the keys allow (two run at a time: sequences of different lengths even out), one step of the four
   // warps at least, and at most the 128 chunks that are joined
   int64_t chunk = tiles * a.Sk / (kNumSms * 8);
@@ -312,7 +356,16 @@ template <int D, int EL>
 int launch_token(const TokenParams& p, cudaStream_t stream) {
   const int64_t tiles = (int64_t)p.a.B * p.a.Hk * p.row_tiles, ctas = tiles * p.chunks, rows = (int64_t)p.a.B * p.a.Hk * p.rows;
   if (ctas > 0x7fffffff || rows > 0x7fffffff) return (int)cudaErrorInvalidValue;
-  cudaError_t e = launch_overlapped(k_attention_token<D, EL>, dim3((unsigned)ctas), dim3(TOKEN_WARPS * 32), 0, stream, p);
+  auto kern = k_attention_token<D, EL>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static std::atomic<bool> configured[64];
+  if (dev < 0 || dev >= 64 || !configured[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, TokenSmem<D>::TOTAL);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
+  }
+  cudaError_t e = launch_overlapped(kern, dim3((unsigned)ctas), dim3(TOKEN_WARPS * 32), TokenSmem<D>::TOTAL, stream, p);
   if (e != cudaSuccess) return (int)e;
   count_launch();
   if (p.chunks > 1) {
