@@ -23,7 +23,7 @@ namespace b2x {
 namespace {
 
 constexpr int kRotaryWarps = 8;
-constexpr int kRotaryRows = 2;       // heads of a lane in flight: 64 bytes of loads per thread at 128 elements of 16 bits
+constexpr int kRotaryRows = 4;       // heads of a lane in flight: 128 bytes of loads per thread at 128 elements of 16 bits
 
 struct RotaryParams {
   const char* x[2];
@@ -56,17 +56,21 @@ template <int EL> __device__ __forceinline__ uint32_t rot_pack(float a, float b)
   else { __half2 t = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&t); }
 }
 
-// V elements at `p` as floats
-template <int EL, int V> __device__ __forceinline__ void rot_load(const char* p, float (&v)[V]) {
-  constexpr int BYTES = V * (EL == EL_F32 ? 4 : 2);
+// V elements as they lie in memory, and as floats
+template <int EL, int V> struct RotRaw {
+  static constexpr int BYTES = V * (EL == EL_F32 ? 4 : 2);
   uint32_t w[(BYTES + 3) / 4];
-  if constexpr (BYTES == 16) { const uint4 q = ld_global((const uint4*)p); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
-  else if constexpr (BYTES == 8) { const uint2 q = ld_global((const uint2*)p); w[0] = q.x; w[1] = q.y; }
-  else if constexpr (BYTES == 4) w[0] = ld_global((const uint32_t*)p);
-  else w[0] = ld_global((const uint16_t*)p);
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (BYTES == 16) { const uint4 q = ld_global((const uint4*)p); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
+    else if constexpr (BYTES == 8) { const uint2 q = ld_global((const uint2*)p); w[0] = q.x; w[1] = q.y; }
+    else if constexpr (BYTES == 4) w[0] = ld_global((const uint32_t*)p);
+    else w[0] = ld_global((const uint16_t*)p);
+  }
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < V; i++) v[i] = rot_get<EL>(w, i);
-}
+    for (int i = 0; i < (BYTES + 3) / 4; i++) w[i] = 0;
+  }
+};
 template <int EL, int V> __device__ __forceinline__ void rot_store(char* p, const float (&v)[V]) {
   if constexpr (EL == EL_F32) {
     if constexpr (V == 4) *(float4*)p = make_float4(v[0], v[1], v[2], v[3]);
@@ -80,10 +84,12 @@ template <int EL, int V> __device__ __forceinline__ void rot_store(char* p, cons
   }
 }
 
-// NU units per lane; a unit is two pieces of V elements that start at e0 and e1 (-1: none)
+// NU units per lane; a unit is two pieces of V elements that start at e[u][0] and e[u][1] (-1: none)
 template <int EL, int V, int NU> struct RotLane {
   static constexpr int ES = EL == EL_F32 ? 4 : 2;
+  using Raw = RotRaw<EL, V>;
   int e[NU][2];
+  int turns[NU];                   // pairs of the unit that turn: the first so many, the others pass
   float cs[NU][V], sn[NU][V];      // of pair j: half layout (a_j, b_j); interleaved pairs of piece 0, then of piece 1
   float w[NU][2][V];
 
@@ -91,24 +97,15 @@ template <int EL, int V, int NU> struct RotLane {
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       const int unit = lane + u * p.lanes;
-      int a = -1, b = -1;
+      int a = -1, b = -1, t = 0;
       if (unit < p.units) {
-        if (p.interleaved) { a = 2 * unit * V; b = a + V; }
-        else if (unit < p.pair_units) { a = unit * V; b = a + p.R / 2; }
+        if (p.interleaved) { a = 2 * unit * V; b = a + V; t = min(max(p.R / 2 - unit * V, 0), V); }
+        else if (unit < p.pair_units) { a = unit * V; b = a + p.R / 2; t = V; }
         else { a = p.R + 2 * (unit - p.pair_units) * V; b = a + V; }
         if (b >= p.D) b = -1;
       }
-      e[u][0] = a; e[u][1] = b;
+      e[u][0] = a; e[u][1] = b; turns[u] = t;
     }
-  }
-  // which pair number j is, -1 for elements that pass
-  __device__ __forceinline__ int pair(const RotaryParams& p, int u, int j) const {
-    if (e[u][0] < 0) return -1;
-    int i;
-    if (!p.interleaved) i = e[u][0] < p.R / 2 ? e[u][0] + j : -1;
-    else if constexpr (V == 1) i = e[u][0] / 2;
-    else i = j < V / 2 ? e[u][0] / 2 + j : e[u][0] / 2 + V / 2 + (j - V / 2);
-    return i < p.R / 2 ? i : -1;
   }
   // cosines and sines of the warp's token
   __device__ __forceinline__ void angles(const RotaryParams& p, int token, float2* table) {
@@ -127,8 +124,8 @@ template <int EL, int V, int NU> struct RotLane {
     for (int u = 0; u < NU; u++)
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const int i = pair(p, u, j);
-        const float2 t = i >= 0 ? table[i] : make_float2(1.f, 0.f);
+        // the unit's first pair: both layouts count pairs from half the first element on, or from the element itself
+        const float2 t = j < turns[u] ? table[(p.interleaved ? e[u][0] / 2 : e[u][0]) + j] : make_float2(1.f, 0.f);
         cs[u][j] = t.x; sn[u][j] = t.y;
       }
   }
@@ -149,17 +146,22 @@ template <int EL, int V, int NU> struct RotLane {
           }
         }
   }
-  __device__ __forceinline__ void load(const char* row, bool on, float (&v)[NU][2][V]) const {
+  __device__ __forceinline__ void load(const char* row, bool on, Raw (&v)[NU][2]) const {
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        if (on && e[u][s] >= 0) rot_load<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
-        else {
-#pragma unroll
-          for (int j = 0; j < V; j++) v[u][s][j] = 0.f;
-        }
+        if (on && e[u][s] >= 0) v[u][s].load(row + (int64_t)e[u][s] * ES);
+        else v[u][s].zero();
       }
+  }
+  static __device__ __forceinline__ void floats(const Raw (&r)[NU][2], float (&v)[NU][2][V]) {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int j = 0; j < V; j++) v[u][s][j] = rot_get<EL>(r[u][s].w, j);
   }
   __device__ __forceinline__ void store(char* row, const float (&v)[NU][2][V]) const {
 #pragma unroll
@@ -168,38 +170,38 @@ template <int EL, int V, int NU> struct RotLane {
       for (int s = 0; s < 2; s++)
         if (e[u][s] >= 0) rot_store<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
   }
+  // pairs that pass are left alone: with a cosine of 1 and a sine of 0 an infinity in one element would make the other NaN
   __device__ __forceinline__ void turn(const RotaryParams& p, float (&v)[NU][2][V]) const {
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       if (V == 1 || !p.interleaved) {
+        if (turns[u] > 0) {
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-          const float a = v[u][0][j], b = v[u][1][j];
-          // a pair that passes has cos 1 and sin 0; without the test an infinity in one half would make the other NaN
-          if (sn[u][j] != 0.f || cs[u][j] != 1.f) { v[u][0][j] = a * cs[u][j] - b * sn[u][j]; v[u][1][j] = b * cs[u][j] + a * sn[u][j]; }
+          for (int j = 0; j < V; j++) {
+            const float a = v[u][0][j], b = v[u][1][j];
+            v[u][0][j] = a * cs[u][j] - b * sn[u][j];
+            v[u][1][j] = b * cs[u][j] + a * sn[u][j];
+          }
         }
       } else if constexpr (V > 1) {
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-          for (int j = 0; j < V / 2; j++) {
-            const int k = s * (V / 2) + j;
-            const float a = v[u][s][2 * j], b = v[u][s][2 * j + 1];
-            if (sn[u][k] != 0.f || cs[u][k] != 1.f) { v[u][s][2 * j] = a * cs[u][k] - b * sn[u][k]; v[u][s][2 * j + 1] = b * cs[u][k] + a * sn[u][k]; }
-          }
+        for (int k = 0; k < V; k++) {
+          float &x = v[u][k / (V / 2)][2 * (k % (V / 2))], &y = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
+          const float a = x, b = y;
+          if (k < turns[u]) { x = a * cs[u][k] - b * sn[u][k]; y = b * cs[u][k] + a * sn[u][k]; }
+        }
       }
     }
   }
   static __device__ __forceinline__ float dot(const float (&a)[NU][2][V], const float (&b)[NU][2][V], int lanes) {
-    float s = 0.f;
+    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
-      for (int k = 0; k < 2; k++)
-#pragma unroll
-        for (int j = 0; j < V; j++) s = fmaf(a[u][k][j], b[u][k][j], s);
-    for (int off = lanes >> 1; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    return s;
+      for (int j = 0; j < V; j++) { s[0] = fmaf(a[u][0][j], b[u][0][j], s[0]); s[1] = fmaf(a[u][1][j], b[u][1][j], s[1]); }
+    float t = s[0] + s[1];
+    for (int off = lanes >> 1; off > 0; off >>= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
+    return t;
   }
 };
 
@@ -213,9 +215,10 @@ __device__ __forceinline__ RotJob rot_job(const RotaryParams& p, int job) {
 __device__ __forceinline__ int64_t rot_at(const B2xHeadStrides& s, int b, int h, int t) { return (int64_t)b * s.batch + (int64_t)h * s.head + (int64_t)t * s.token; }
 
 template <int EL, int V, int NU>
-__global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary(const __grid_constant__ RotaryParams p) {
   __shared__ float2 table[kRotaryWarps][128];
   constexpr int ES = EL == EL_F32 ? 4 : 2;
+  constexpr int ROWS = NU == 1 ? kRotaryRows : 1;
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -228,36 +231,40 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary(const __grid_const
   const int slots = 32 / p.lanes, slot = lane / p.lanes;
   RotLane<EL, V, NU> me;
   me.pieces(p, lane & (p.lanes - 1));
+  const char* in = p.x[job.ti] + rot_at(p.xs[job.ti], b, 0, t) * ES;
+  char* out = p.y[job.ti] + rot_at(p.ys[job.ti], b, 0, t) * ES;
+  const int64_t in_head = p.xs[job.ti].head * ES, out_head = p.ys[job.ti].head * ES;
+  typename RotLane<EL, V, NU>::Raw raw[ROWS][NU][2];
+  // the first heads are on their way while the angles are worked out
+#pragma unroll
+  for (int r = 0; r < ROWS; r++) { const int h = job.h0 + r * slots + slot; me.load(in + h * in_head, h < job.h1, raw[r]); }
   me.angles(p, token, table[warp]);
   me.weights(p, job.ti);
-  for (int h0 = job.h0; h0 < job.h1; h0 += kRotaryRows * slots) {
-    float v[kRotaryRows][NU][2][V];
+  for (int h0 = job.h0; h0 < job.h1; h0 += ROWS * slots) {
 #pragma unroll
-    for (int r = 0; r < kRotaryRows; r++) {
-      const int h = h0 + r * slots + slot;
-      me.load(p.x[job.ti] + rot_at(p.xs[job.ti], b, h, t) * ES, h < job.h1, v[r]);
-    }
-#pragma unroll
-    for (int r = 0; r < kRotaryRows; r++) {
-      const int h = h0 + r * slots + slot;
+    for (int r = 0; r < ROWS; r++) {
+      const int h = h0 + r * slots + slot, next = h + ROWS * slots;
+      float v[NU][2][V];
+      me.floats(raw[r], v);
+      me.load(in + next * in_head, next < job.h1, raw[r]);
       if (p.norm) {
-        const float f = rsqrtf(me.dot(v[r], v[r], p.lanes) * p.inv_d + p.epsilon);
+        const float f = rsqrtf(me.dot(v, v, p.lanes) * p.inv_d + p.epsilon);
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
           for (int s = 0; s < 2; s++)
 #pragma unroll
-            for (int j = 0; j < V; j++) v[r][u][s][j] *= f * me.w[u][s][j];
+            for (int j = 0; j < V; j++) v[u][s][j] *= f * me.w[u][s][j];
       }
-      me.turn(p, v[r]);
-      if (h < job.h1) me.store(p.y[job.ti] + rot_at(p.ys[job.ti], b, h, t) * ES, v[r]);
+      me.turn(p, v);
+      if (h < job.h1) me.store(out + h * out_head, v);
     }
   }
 }
 
 // Gradient with norms: tensor blockIdx.y; a warp walks tokens in steps of the grid and keeps its elements' share of dw
 template <int EL, int V, int NU>
-__global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary_gradient(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const __grid_constant__ RotaryParams p) {
   __shared__ float2 table[kRotaryWarps][128];
   __shared__ float sums[kRotaryWarps][256];
   constexpr int ES = EL == EL_F32 ? 4 : 2;
@@ -280,12 +287,21 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary_gradient(const __g
     const int token = (int)(id / p.jobs[ti]);
     const int first = (int)(id - (int64_t)token * p.jobs[ti]) * p.job_heads, last = min(first + p.job_heads, p.heads[ti]);
     const int b = token / p.S, t = token - b * p.S;
+    const char* in = p.x[ti] + rot_at(p.xs[ti], b, 0, t) * ES;
+    const char* din = p.dy[ti] + rot_at(p.dys[ti], b, 0, t) * ES;
+    char* out = p.y[ti] + rot_at(p.ys[ti], b, 0, t) * ES;
+    const int64_t in_head = p.xs[ti].head * ES, din_head = p.dys[ti].head * ES, out_head = p.ys[ti].head * ES;
+    typename RotLane<EL, V, NU>::Raw rx[NU][2], rg[NU][2];
+    me.load(in + (first + slot) * in_head, first + slot < last, rx);
+    me.load(din + (first + slot) * din_head, first + slot < last, rg);
     me.angles(p, token, table[warp]);
     for (int h0 = first; h0 < last; h0 += slots) {
-      const int h = h0 + slot;
+      const int h = h0 + slot, next = h + slots;
       float x[NU][2][V], g[NU][2][V];
-      me.load(p.x[ti] + rot_at(p.xs[ti], b, h, t) * ES, h < last, x);
-      me.load(p.dy[ti] + rot_at(p.dys[ti], b, h, t) * ES, h < last, g);
+      me.floats(rx, x);
+      me.floats(rg, g);
+      me.load(in + next * in_head, next < last, rx);
+      me.load(din + next * din_head, next < last, rg);
       me.turn(p, g);
       const float f = rsqrtf(me.dot(x, x, p.lanes) * p.inv_d + p.epsilon);
 #pragma unroll
@@ -305,7 +321,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32) k_rotary_gradient(const __g
         for (int s = 0; s < 2; s++)
 #pragma unroll
           for (int j = 0; j < V; j++) g[u][s][j] = f * (g[u][s][j] - x[u][s][j] * m);
-      if (h < last) me.store(p.y[ti] + rot_at(p.ys[ti], b, h, t) * ES, g);
+      if (h < last) me.store(out + h * out_head, g);
     }
   }
   // the warp's slots, then the CTA's warps, in a fixed order
