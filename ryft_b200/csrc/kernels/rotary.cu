@@ -34,9 +34,8 @@ struct RotaryParams {
   const int32_t* positions;
   const uint64_t* turns;
   float* partial;              // gradient with norms: [tensor][CTA][D]
-  int64_t warps;               // warps with work
   int32_t tokens, S, D, R;
-  int32_t heads[2], jobs[2];   // a token's heads are cut into jobs of `job_heads`
+  int32_t heads[2];            // a token's heads are cut into jobs of `job_heads`: of both tensors together, in a gradient of each
   int32_t job_heads, lanes, units;
   int32_t pair_units;          // half layout: units whose two pieces are partners
   float epsilon, inv_d, sine;  // sine: 1, or -1 to turn back
@@ -92,6 +91,7 @@ template <int EL, int V, int NU> struct RotLane {
   int turns[NU];                   // pairs of the unit that turn: the first so many, the others pass
   float cs[NU][V], sn[NU][V];      // of pair j: half layout (a_j, b_j); interleaved pairs of piece 0, then of piece 1
   float w[NU][2][V];
+  float ca[NU][V], sa[NU][V], cb[NU][V], sb[NU][V];
 
   __device__ __forceinline__ void pieces(const RotaryParams& p, int lane) {
 #pragma unroll
@@ -120,6 +120,8 @@ template <int EL, int V, int NU> struct RotLane {
       table[i] = make_float2(c, s * p.sine);
     }
     __syncwarp();
+  }
+  __device__ __forceinline__ void take(const RotaryParams& p, const float2* table) {
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
@@ -170,6 +172,38 @@ template <int EL, int V, int NU> struct RotLane {
       for (int s = 0; s < 2; s++)
         if (e[u][s] >= 0) rot_store<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
   }
+  // w (of the elements) times cos and sin: x turns to f (x[a] ca - x[b] sb), ...
+  __device__ __forceinline__ void fold(const RotaryParams& p, const float2* table) {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float2 t = k < turns[u] ? table[(p.interleaved ? e[u][0] / 2 : e[u][0]) + k] : make_float2(1.f, 0.f);
+        const bool across = V == 1 || !p.interleaved;
+        const float wa = across ? w[u][0][k] : w[u][k / ((V + 1) / 2)][(2 * k) % V], wb = across ? w[u][1][k] : w[u][k / ((V + 1) / 2)][(2 * k + 1) % V];
+        ca[u][k] = t.x * wa; sa[u][k] = t.y * wa; cb[u][k] = t.x * wb; sb[u][k] = t.y * wb;
+      }
+  }
+  __device__ __forceinline__ void turn_weighted(const RotaryParams& p, float (&v)[NU][2][V], float f) const {
+#pragma unroll
+    for (int u = 0; u < NU; u++)
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const bool across = V == 1 || !p.interleaved;
+        if (across) {
+          const float a = v[u][0][k] * f, b = v[u][1][k] * f;
+          float x = a * ca[u][k], y = b * cb[u][k];
+          if (turns[u] > 0) { x = fmaf(-b, sb[u][k], x); y = fmaf(a, sa[u][k], y); }
+          v[u][0][k] = x; v[u][1][k] = y;
+        } else if constexpr (V > 1) {
+          float &px = v[u][k / (V / 2)][2 * (k % (V / 2))], &py = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
+          const float a = px * f, b = py * f;
+          float x = a * ca[u][k], y = b * cb[u][k];
+          if (k < turns[u]) { x = fmaf(-b, sb[u][k], x); y = fmaf(a, sa[u][k], y); }
+          px = x; py = y;
+        }
+      }
+  }
   // pairs that pass are left alone: with a cosine of 1 and a sine of 0 an infinity in one element would make the other NaN
   __device__ __forceinline__ void turn(const RotaryParams& p, float (&v)[NU][2][V]) const {
 #pragma unroll
@@ -205,59 +239,54 @@ template <int EL, int V, int NU> struct RotLane {
   }
 };
 
-// The head's rows of a job: tensor, first head and the head behind the last
-struct RotJob { int ti, h0, h1; };
-__device__ __forceinline__ RotJob rot_job(const RotaryParams& p, int job) {
-  const int ti = job >= p.jobs[0] ? 1 : 0;
-  const int h0 = (job - (ti ? p.jobs[0] : 0)) * p.job_heads;
-  return {ti, h0, min(h0 + p.job_heads, p.heads[ti])};
-}
 __device__ __forceinline__ int64_t rot_at(const B2xHeadStrides& s, int b, int h, int t) { return (int64_t)b * s.batch + (int64_t)h * s.head + (int64_t)t * s.token; }
 
+// A warp: one token (of this CTA's eight), and the heads of share blockIdx.y of all its heads
 template <int EL, int V, int NU>
 __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary(const __grid_constant__ RotaryParams p) {
   __shared__ float2 table[kRotaryWarps][128];
   constexpr int ES = EL == EL_F32 ? 4 : 2;
   constexpr int ROWS = NU == 1 ? kRotaryRows : 1;
+  using Lane = RotLane<EL, V, NU>;
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * kRotaryWarps + warp;
-  if (id >= p.warps) return;
-  const int all = p.jobs[0] + p.jobs[1];
-  const int token = (int)(id / all);
-  const RotJob job = rot_job(p, (int)(id - (int64_t)token * all));
-  const int b = token / p.S, t = token - b * p.S;
+  const uint32_t token = blockIdx.x * kRotaryWarps + warp;
+  if (token >= (uint32_t)p.tokens) return;
+  const int b = (int)(token / (uint32_t)p.S), t = (int)(token - (uint32_t)b * (uint32_t)p.S);
   const int slots = 32 / p.lanes, slot = lane / p.lanes;
-  RotLane<EL, V, NU> me;
+  Lane me;
   me.pieces(p, lane & (p.lanes - 1));
-  const char* in = p.x[job.ti] + rot_at(p.xs[job.ti], b, 0, t) * ES;
-  char* out = p.y[job.ti] + rot_at(p.ys[job.ti], b, 0, t) * ES;
-  const int64_t in_head = p.xs[job.ti].head * ES, out_head = p.ys[job.ti].head * ES;
-  typename RotLane<EL, V, NU>::Raw raw[ROWS][NU][2];
-  // the first heads are on their way while the angles are worked out
+  bool angles = false;
+#pragma unroll 1
+  for (int ti = 0; ti < 2; ti++) {
+    // this share's heads of the tensor
+    const int h_begin = max((int)blockIdx.y * p.job_heads - (ti ? p.heads[0] : 0), 0), h_end = min(((int)blockIdx.y + 1) * p.job_heads - (ti ? p.heads[0] : 0), p.heads[ti]);
+    if (h_begin >= h_end) continue;
+    const char* in = p.x[ti] + rot_at(p.xs[ti], b, h_begin + slot, t) * ES;
+    char* out = p.y[ti] + rot_at(p.ys[ti], b, h_begin + slot, t) * ES;
+    const int64_t in_step = p.xs[ti].head * ES * slots, out_step = p.ys[ti].head * ES * slots;
+    int left = h_end - h_begin - slot;             // heads from this slot's next on
+    typename Lane::Raw raw[ROWS][NU][2];
+    // the first heads are on their way while the angles are worked out
 #pragma unroll
-  for (int r = 0; r < ROWS; r++) { const int h = job.h0 + r * slots + slot; me.load(in + h * in_head, h < job.h1, raw[r]); }
-  me.angles(p, token, table[warp]);
-  me.weights(p, job.ti);
-  for (int h0 = job.h0; h0 < job.h1; h0 += ROWS * slots) {
+    for (int r = 0; r < ROWS; r++) { me.load(in, left > r * slots, raw[r]); in += in_step; }
+    if (!angles) { me.angles(p, (int)token, table[warp]); angles = true; }
+    me.weights(p, ti);
+    me.fold(p, table[warp]);
+    for (int n = h_begin; n < h_end; n += ROWS * slots) {
 #pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-      const int h = h0 + r * slots + slot, next = h + ROWS * slots;
-      float v[NU][2][V];
-      me.floats(raw[r], v);
-      me.load(in + next * in_head, next < job.h1, raw[r]);
-      if (p.norm) {
-        const float f = rsqrtf(me.dot(v, v, p.lanes) * p.inv_d + p.epsilon);
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-          for (int s = 0; s < 2; s++)
-#pragma unroll
-            for (int j = 0; j < V; j++) v[u][s][j] *= f * me.w[u][s][j];
+      for (int r = 0; r < ROWS; r++) {
+        float v[NU][2][V];
+        Lane::floats(raw[r], v);
+        me.load(in, left > ROWS * slots, raw[r]);
+        in += in_step;
+        const float f = p.norm ? rsqrtf(Lane::dot(v, v, p.lanes) * p.inv_d + p.epsilon) : 1.f;
+        me.turn_weighted(p, v, f);
+        if (left > 0) me.store(out, v);
+        out += out_step;
+        left -= slots;
       }
-      me.turn(p, v);
-      if (h < job.h1) me.store(out + h * out_head, v);
     }
   }
 }
@@ -282,11 +311,11 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
     for (int s = 0; s < 2; s++)
 #pragma unroll
       for (int j = 0; j < V; j++) dw[u][s][j] = 0.f;
-  const int64_t work = (int64_t)p.tokens * p.jobs[ti];
-  for (int64_t id = (int64_t)blockIdx.x * kRotaryWarps + warp; id < work; id += (int64_t)gridDim.x * kRotaryWarps) {
-    const int token = (int)(id / p.jobs[ti]);
-    const int first = (int)(id - (int64_t)token * p.jobs[ti]) * p.job_heads, last = min(first + p.job_heads, p.heads[ti]);
-    const int b = token / p.S, t = token - b * p.S;
+  const uint32_t jobs = (uint32_t)((p.heads[ti] + p.job_heads - 1) / p.job_heads), work = (uint32_t)p.tokens * jobs;
+  for (uint32_t id = blockIdx.x * kRotaryWarps + warp; id < work; id += gridDim.x * kRotaryWarps) {
+    const int token = (int)(jobs == 1 ? id : id / jobs);
+    const int first = (int)(id - (uint32_t)token * jobs) * p.job_heads, last = min(first + p.job_heads, p.heads[ti]);
+    const int b = (int)((uint32_t)token / (uint32_t)p.S), t = token - b * p.S;
     const char* in = p.x[ti] + rot_at(p.xs[ti], b, 0, t) * ES;
     const char* din = p.dy[ti] + rot_at(p.dys[ti], b, 0, t) * ES;
     char* out = p.y[ti] + rot_at(p.ys[ti], b, 0, t) * ES;
@@ -295,6 +324,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
     me.load(in + (first + slot) * in_head, first + slot < last, rx);
     me.load(din + (first + slot) * din_head, first + slot < last, rg);
     me.angles(p, token, table[warp]);
+    me.take(p, table[warp]);
     for (int h0 = first; h0 < last; h0 += slots) {
       const int h = h0 + slot, next = h + slots;
       float x[NU][2][V], g[NU][2][V];
@@ -388,7 +418,7 @@ int rot_piece(const B2xRotaryArgs* a, bool gradient) {
   return 1;
 }
 
-RotaryParams rot_params(const B2xRotaryArgs* a, int V) {
+RotaryParams rot_params(const B2xRotaryArgs* a, int V, bool each) {
   RotaryParams p{};
   p.positions = a->positions; p.turns = a->turns;
   p.tokens = (int32_t)(a->B * a->S); p.S = (int32_t)a->S; p.D = (int32_t)a->D; p.R = (int32_t)a->R;
@@ -408,19 +438,16 @@ RotaryParams rot_params(const B2xRotaryArgs* a, int V) {
   }
   // a warp walks all heads of its token, unless that leaves SMs without work: then as few as one round of its slots
   const int slots = 32 / p.lanes;
-  int most = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+  const int most = each ? (p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1]) : p.heads[0] + p.heads[1];
   p.job_heads = (most + slots - 1) / slots * slots;
   if (p.job_heads < slots) p.job_heads = slots;
-  while (p.job_heads > slots && (int64_t)p.tokens * ((p.heads[0] + p.job_heads - 1) / p.job_heads + (p.heads[1] + p.job_heads - 1) / p.job_heads) < (int64_t)kNumSms * 32)
-    p.job_heads = (p.job_heads / 2 + slots - 1) / slots * slots;
-  for (int i = 0; i < 2; i++) p.jobs[i] = (p.heads[i] + p.job_heads - 1) / p.job_heads;
-  p.warps = (int64_t)p.tokens * (p.jobs[0] + p.jobs[1]);
+  while (p.job_heads > slots && (int64_t)p.tokens * ((most + p.job_heads - 1) / p.job_heads) < (int64_t)kNumSms * 16) p.job_heads = (p.job_heads / 2 + slots - 1) / slots * slots;
   return p;
 }
 
 int rot_gradient_ctas(const RotaryParams& p) {
-  const int64_t jobs = p.jobs[0] > p.jobs[1] ? p.jobs[0] : p.jobs[1];
-  const int64_t ctas = ((int64_t)p.tokens * jobs + kRotaryWarps - 1) / kRotaryWarps;
+  const int most = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
+  const int64_t ctas = ((int64_t)p.tokens * ((most + p.job_heads - 1) / p.job_heads) + kRotaryWarps - 1) / kRotaryWarps;
   return (int)(ctas < 1 ? 1 : ctas > kNumSms * 3 ? kNumSms * 3 : ctas);
 }
 
@@ -428,7 +455,10 @@ template <int EL, int V, int NU>
 int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, bool norm_gradient, cudaStream_t stream) {
   cudaError_t e;
   if (norm_gradient) e = launch_overlapped(k_rotary_gradient<EL, V, NU>, dim3((unsigned)rot_gradient_ctas(p), a->n), dim3(kRotaryWarps * 32), 0, stream, p);
-  else e = launch_overlapped(k_rotary<EL, V, NU>, dim3((unsigned)((p.warps + kRotaryWarps - 1) / kRotaryWarps)), dim3(kRotaryWarps * 32), 0, stream, p);
+  else {
+    const unsigned jobs = (unsigned)((p.heads[0] + p.heads[1] + p.job_heads - 1) / p.job_heads);
+    e = launch_overlapped(k_rotary<EL, V, NU>, dim3((unsigned)((p.tokens + kRotaryWarps - 1) / kRotaryWarps), jobs), dim3(kRotaryWarps * 32), 0, stream, p);
+  }
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();
@@ -457,8 +487,8 @@ extern "C" int b2x_launch_rotary(const B2xRotaryArgs* a, b2x_stream_t stream) {
   if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
   if (a->D == 0) return 0;
   const int V = rot_piece(a, false);
-  const RotaryParams p = rot_params(a, V);
-  if (p.warps == 0) return 0;
+  const RotaryParams p = rot_params(a, V, false);
+  if (p.tokens == 0 || p.heads[0] + p.heads[1] == 0) return 0;
   return launch_rot(a, p, V, false, (cudaStream_t)stream);
 }
 
@@ -478,12 +508,12 @@ extern "C" int b2x_launch_rotary_gradient(const B2xRotaryArgs* a, b2x_stream_t s
   if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
   if (a->D == 0) return 0;
   const int V = rot_piece(a, true);
-  RotaryParams p = rot_params(a, V);
+  RotaryParams p = rot_params(a, V, a->norm);
   p.sine = -1.f;
   if (!a->norm) {
     // the rotation's transpose: the same kernel, turned the other way
     for (int i = 0; i < a->n; i++) { p.x[i] = p.dy[i]; p.xs[i] = p.dys[i]; }
-    if (p.warps == 0) return 0;
+    if (p.tokens == 0 || p.heads[0] + p.heads[1] == 0) return 0;
     return launch_rot(a, p, V, false, (cudaStream_t)stream);
   }
   if (!a->scratch) return (int)cudaErrorInvalidValue;
