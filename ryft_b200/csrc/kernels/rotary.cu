@@ -39,7 +39,7 @@ struct RotaryParams {
   int32_t job_heads, lanes, units;
   int32_t pair_units;          // half layout: units whose two pieces are partners
   float epsilon, inv_d, sine;  // sine: 1, or -1 to turn back
-  uint8_t interleaved, norm, weight_f32;
+  uint8_t interleaved, norm, weight_f32, weight_wide;   // wide: weights start on 16 bytes
 };
 
 template <int EL> __device__ __forceinline__ float rot_get(const uint32_t* w, int i) {
@@ -59,15 +59,18 @@ template <int EL> __device__ __forceinline__ uint32_t rot_pack(float a, float b)
 template <int EL, int V> struct RotRaw {
   static constexpr int BYTES = V * (EL == EL_F32 ? 4 : 2);
   uint32_t w[(BYTES + 3) / 4];
-  __device__ __forceinline__ void load(const char* p) {
-    if constexpr (BYTES == 16) { const uint4 q = ld_global((const uint4*)p); w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w; }
-    else if constexpr (BYTES == 8) { const uint2 q = ld_global((const uint2*)p); w[0] = q.x; w[1] = q.y; }
-    else if constexpr (BYTES == 4) w[0] = ld_global((const uint32_t*)p);
-    else w[0] = ld_global((const uint16_t*)p);
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < (BYTES + 3) / 4; i++) w[i] = 0;
+  // zeros where there is nothing, without a branch
+  __device__ __forceinline__ void load(const char* p, bool on) {
+    const int q = on;
+    if constexpr (BYTES == 16)
+      asm volatile("{\n .reg .pred q;\n setp.ne.s32 q, %5, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n mov.b32 %2, 0;\n mov.b32 %3, 0;\n @q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+                   : "=&r"(w[0]), "=&r"(w[1]), "=&r"(w[2]), "=&r"(w[3]) : "l"(__cvta_generic_to_global(p)), "r"(q));
+    else if constexpr (BYTES == 8)
+      asm volatile("{\n .reg .pred q;\n setp.ne.s32 q, %3, 0;\n mov.b32 %0, 0;\n mov.b32 %1, 0;\n @q ld.global.v2.u32 {%0, %1}, [%2];\n}"
+                   : "=&r"(w[0]), "=&r"(w[1]) : "l"(__cvta_generic_to_global(p)), "r"(q));
+    else if constexpr (BYTES == 4)
+      asm volatile("{\n .reg .pred q;\n setp.ne.s32 q, %2, 0;\n mov.b32 %0, 0;\n @q ld.global.u32 %0, [%1];\n}" : "=&r"(w[0]) : "l"(__cvta_generic_to_global(p)), "r"(q));
+    else w[0] = on ? ld_global((const uint16_t*)p) : 0u;
   }
 };
 template <int EL, int V> __device__ __forceinline__ void rot_store(char* p, const float (&v)[V]) {
@@ -135,7 +138,26 @@ template <int EL, int V, int NU> struct RotLane {
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
-      for (int s = 0; s < 2; s++)
+      for (int s = 0; s < 2; s++) {
+        if constexpr (V > 1) {
+          if (p.norm && p.weight_wide) {
+            if (p.weight_f32) {
+#pragma unroll
+              for (int j = 0; j < V; j += 4) {
+                RotRaw<EL_F32, 4> q;
+                q.load(p.weight[ti] + (int64_t)(e[u][s] + j) * 4, e[u][s] >= 0);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[u][s][j + i] = __uint_as_float(q.w[i]);
+              }
+            } else {
+              Raw q;
+              q.load(p.weight[ti] + (int64_t)e[u][s] * ES, e[u][s] >= 0);
+#pragma unroll
+              for (int j = 0; j < V; j++) w[u][s][j] = rot_get<EL>(q.w, j);
+            }
+            continue;
+          }
+        }
 #pragma unroll
         for (int j = 0; j < V; j++) {
           w[u][s][j] = 1.f;
@@ -147,14 +169,14 @@ template <int EL, int V, int NU> struct RotLane {
             }
           }
         }
+      }
   }
   __device__ __forceinline__ void load(const char* row, bool on, Raw (&v)[NU][2]) const {
 #pragma unroll
     for (int u = 0; u < NU; u++)
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        if (on && e[u][s] >= 0) v[u][s].load(row + (int64_t)e[u][s] * ES);
-        else v[u][s].zero();
+        v[u][s].load(row + (int64_t)e[u][s] * ES, on && e[u][s] >= 0);
       }
   }
   static __device__ __forceinline__ void floats(const Raw (&r)[NU][2], float (&v)[NU][2][V]) {
@@ -186,16 +208,23 @@ template <int EL, int V, int NU> struct RotLane {
   }
   __device__ __forceinline__ void turn_weighted(const RotaryParams& p, float (&v)[NU][2][V], float f) const {
 #pragma unroll
-    for (int u = 0; u < NU; u++)
+    for (int u = 0; u < NU; u++) {
+      if (V == 1 || !p.interleaved) {
+        // pieces turn as a whole or pass as a whole
+        if (turns[u] > 0) {
 #pragma unroll
-      for (int k = 0; k < V; k++) {
-        const bool across = V == 1 || !p.interleaved;
-        if (across) {
-          const float a = v[u][0][k] * f, b = v[u][1][k] * f;
-          float x = a * ca[u][k], y = b * cb[u][k];
-          if (turns[u] > 0) { x = fmaf(-b, sb[u][k], x); y = fmaf(a, sa[u][k], y); }
-          v[u][0][k] = x; v[u][1][k] = y;
-        } else if constexpr (V > 1) {
+          for (int k = 0; k < V; k++) {
+            const float a = v[u][0][k] * f, b = v[u][1][k] * f;
+            v[u][0][k] = fmaf(-b, sb[u][k], a * ca[u][k]);
+            v[u][1][k] = fmaf(a, sa[u][k], b * cb[u][k]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; k++) { v[u][0][k] *= f * ca[u][k]; v[u][1][k] *= f * cb[u][k]; }
+        }
+      } else if constexpr (V > 1) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
           float &px = v[u][k / (V / 2)][2 * (k % (V / 2))], &py = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
           const float a = px * f, b = py * f;
           float x = a * ca[u][k], y = b * cb[u][k];
@@ -203,6 +232,7 @@ template <int EL, int V, int NU> struct RotLane {
           px = x; py = y;
         }
       }
+    }
   }
   // pairs that pass are left alone: with a cosine of 1 and a sine of 0 an infinity in one element would make the other NaN
   __device__ __forceinline__ void turn(const RotaryParams& p, float (&v)[NU][2][V]) const {
@@ -234,7 +264,8 @@ template <int EL, int V, int NU> struct RotLane {
 #pragma unroll
       for (int j = 0; j < V; j++) { s[0] = fmaf(a[u][0][j], b[u][0][j], s[0]); s[1] = fmaf(a[u][1][j], b[u][1][j], s[1]); }
     float t = s[0] + s[1];
-    for (int off = lanes >> 1; off > 0; off >>= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) if (off < lanes) t += __shfl_xor_sync(0xffffffffu, t, off);
     return t;
   }
 };
@@ -381,8 +412,15 @@ __global__ void __launch_bounds__(1024) k_rotary_fold(const float* partial, floa
   pdl_wait();
   const int c = blockIdx.x * 32 + (threadIdx.x & 31), r = threadIdx.x >> 5;
   const float* src = partial + (int64_t)blockIdx.y * rows * D;
+  // sixteen loads of a thread in flight: the CTAs are few
   float s = 0.f;
-  if (c < D) for (int i = r; i < rows; i += 32) s += ld_global(src + (int64_t)i * D + c);
+  for (int i = r; i < rows; i += 32 * 16) {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; k++) v[k] = c < D && i + 32 * k < rows ? ld_global(src + (int64_t)(i + 32 * k) * D + c) : 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; k++) s += v[k];
+  }
   part[r][threadIdx.x & 31] = s;
   __syncthreads();
   if (r == 0 && c < D) {
@@ -424,6 +462,8 @@ RotaryParams rot_params(const B2xRotaryArgs* a, int V, bool each) {
   p.tokens = (int32_t)(a->B * a->S); p.S = (int32_t)a->S; p.D = (int32_t)a->D; p.R = (int32_t)a->R;
   p.epsilon = a->epsilon; p.inv_d = 1.0f / (float)a->D; p.sine = 1.f;
   p.interleaved = a->interleaved; p.norm = a->norm; p.weight_f32 = a->weight_elem == EL_F32;
+  p.weight_wide = 1;
+  for (int i = 0; i < a->n; i++) if ((uintptr_t)a->weight[i] % 16 != 0) p.weight_wide = 0;
   const int pieces = (p.D + V - 1) / V;
   p.pair_units = a->interleaved ? 0 : p.R / 2 / V;
   p.units = a->interleaved ? (pieces + 1) / 2 : p.pair_units + (pieces - 2 * p.pair_units + 1) / 2;
