@@ -194,7 +194,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     uint32_t uc = 0, nt = 0;       // units loaded, tiles with work
     int fixed = (int)blockIdx.x;
     for (int n = 0;; n++) {
-      const bool free = n < 2 || mbar_wait(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 61);
+      const bool free = n < 2 || ha_barrier(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 61);
       if (!__all_sync(0xffffffffu, free)) break;
       int t = 0;
       if (sched) {
@@ -263,7 +263,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       if (t < 0) break;
       if (units == 0) continue;
       if (elect_one()) {
-        bool ok = nt == 0 || mbar_wait(bar_tu, (nt - 1) & 1, abort_flag, status, 62);
+        bool ok = nt == 0 || ha_barrier(bar_tu, (nt - 1) & 1, abort_flag, status, 62);
         if (ok) {
           mbar_expect_tx(bar_tl, 2 * SM::T_BYTES);
 #pragma unroll
@@ -278,7 +278,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
             walk.start(s, listed);
             for (int it = 0; it < units; it++, k++) {
               const uint32_t st = k % GRAD_STAGES, turn = k / GRAD_STAGES;
-              if (turn > 0 && !mbar_wait(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
+              if (turn > 0 && !ha_barrier(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
               mbar_expect_tx(bar_uf + 8 * st, 2 * SM::U_BYTES);
               const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES;
 #pragma unroll
@@ -305,7 +305,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       auto issue_scores = [&](bool last_of_tile) -> bool {
         const uint32_t st = sc % GRAD_STAGES, g = sc & 1;
         const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
-        if (!mbar_wait(bar_uf + 8 * st, (sc / GRAD_STAGES) & 1, abort_flag, status, 71)) return false;
+        if (!ha_barrier(bar_uf + 8 * st, (sc / GRAD_STAGES) & 1, abort_flag, status, 71)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
@@ -323,19 +323,19 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         return true;
       };
       for (int n = 0; ok; n++) {
-        if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 72)) { ok = false; break; }
+        if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 72)) { ok = false; break; }
         const int t = slots[n & 1].tile, total = slots[n & 1].blocks * repeat;
         mbar_arrive(bar_te + 8 * (n & 1));
         if (t < 0) break;
         if (total == 0) continue;
-        if (!mbar_wait(bar_tl, nt & 1, abort_flag, status, 73)) { ok = false; break; }
+        if (!ha_barrier(bar_tl, nt & 1, abort_flag, status, 73)) { ok = false; break; }
         for (int it = 0; it < 2 && it < total && ok; it++) ok = issue_scores(it + 1 == total);
         for (int it = 0; it < total && ok; it++) {
           const uint32_t st = uc % GRAD_STAGES, g = uc & 1;
           const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
-          if (!mbar_wait(bar_pf + 8 * g, (uc >> 1) & 1, abort_flag, status, 74)) { ok = false; break; }
+          if (!ha_barrier(bar_pf + 8 * g, (uc >> 1) & 1, abort_flag, status, 74)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulators
-          if (it == 0 && nt > 0 && !mbar_wait(bar_of, (nt - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
+          if (it == 0 && nt > 0 && !ha_barrier(bar_of, (nt - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
           tc_fence_after();
           // A = P or dS from TMEM: 16 of the unit are 8 columns; B = the unit's rows (MN-major: chunks of 64 of the width are U_CHUNK apart)
           if constexpr (KEYS) {
@@ -357,7 +357,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       }
       // everything this thread issued must retire before TMEM is released
       tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, abort_flag, nullptr, 0);
+      ha_barrier(bar_drain, 0, abort_flag, nullptr, 0);
     }
   } else if (warp >= 4) {
     // ---------------------------------------------- P and dS --------------------------------------------------------
@@ -368,7 +368,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     uint32_t uc = 0, mine = 0, nt = 0;            // units of all groups before this tile, this group's units, tiles with work
     bool ok = true;
     for (int n = 0; ok; n++) {
-      if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
+      if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
       const int t = s->tile, units = s->blocks, b = s->b, th = s->h, at = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
@@ -423,8 +423,8 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         advance();
         if (k - 1 < total) { advance(); if (KEYS && k < total) ahead = fetch(hh, walk.j); }
         // the group's four warps have stored theirs (and read those of two units ago)
-        if (KEYS && !mbar_wait(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
-        if (!mbar_wait(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
+        if (KEYS && !ha_barrier(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
+        if (!ha_barrier(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
         tc_fence_after();
         const int u0 = unit * GRAD_UNIT;           // the unit's first key or query
         const float slope = p.a.slopes ? ld_global(p.a.slopes + head) * kLog2e : 0.f;
@@ -509,7 +509,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1));   // the tile's list has been walked
       if (total > 0) {
-        if (!mbar_wait(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
+        if (!ha_barrier(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
         tc_fence_after();
         nt++;
       }

@@ -97,7 +97,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     int fixed = (int)blockIdx.x * 2 + w;   // without a counter: every worker takes tiles in steps of all workers
     for (int n = 0;; n++) {
       // the slot's previous tile has been read by the issuer and the four softmax warps (all lanes wait: they leave together)
-      const bool free = n < 2 || mbar_wait(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21);
+      const bool free = n < 2 || ha_barrier(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21);
       if (!__all_sync(0xffffffffu, free)) break;
       int t = 0;
       if (sched) {
@@ -159,7 +159,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (elect_one()) {
         const int b = bh / p.a.Hq, h = bh - b * p.a.Hq, u = h / p.a.group;
         // Q is free once the previous tile's last Q K^T has retired
-        if (nq > 0 && !mbar_wait(bar_qe, (nq - 1) & 1, abort_flag, status, 22)) ok = false;
+        if (nq > 0 && !ha_barrier(bar_qe, (nq - 1) & 1, abort_flag, status, 22)) ok = false;
         if (ok) {
           mbar_expect_tx(bar_qf, SM::Q_BYTES);
 #pragma unroll
@@ -207,9 +207,9 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const uint32_t qa = wbase + SM::Q_OFF, ka = wbase + SM::K_OFF, va = wbase + SM::V_OFF, pa = wbase + SM::P_OFF;
       bool ok = true;
       auto issue_qk = [&](bool last_of_tile) -> bool {
-        if (!mbar_wait(bar_kf, kc & 1, abort_flag, status, 13)) return false;
+        if (!ha_barrier(bar_kf, kc & 1, abort_flag, status, 13)) return false;
         // the worker's softmax has copied the previous block's scores into registers
-        if (kc > 0 && !mbar_wait(bar_se, (kc - 1) & 1, abort_flag, status, 14)) return false;
+        if (kc > 0 && !ha_barrier(bar_se, (kc - 1) & 1, abort_flag, status, 14)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
@@ -223,23 +223,23 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         return true;
       };
       for (int n = 0; ok; n++) {
-        if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 23)) { ok = false; break; }
+        if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 23)) { ok = false; break; }
         const int t = slots[n & 1].tile, blocks = slots[n & 1].blocks;
         mbar_arrive(bar_te + 8 * (n & 1));
         if (t < 0) break;
         if (blocks == 0) continue;
-        if (!mbar_wait(bar_qf, nq & 1, abort_flag, status, 12)) { ok = false; break; }
+        if (!ha_barrier(bar_qf, nq & 1, abort_flag, status, 12)) { ok = false; break; }
         if (!issue_qk(blocks == 1)) { ok = false; break; }
         for (int it = 0; it < blocks && ok; it++) {
           // the block's scores are in the softmax warps' registers early: the next score block goes ahead of this
           // block's products
           if (it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
-          if (!mbar_wait(bar_vf, vc & 1, abort_flag, status, 15)) { ok = false; break; }
+          if (!ha_barrier(bar_vf, vc & 1, abort_flag, status, 15)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulator
-          if (it == 0 && nq > 0 && !mbar_wait(bar_of, (nq - 1) & 1, abort_flag, status, 24)) { ok = false; break; }
+          if (it == 0 && nq > 0 && !ha_barrier(bar_of, (nq - 1) & 1, abort_flag, status, 24)) { ok = false; break; }
 #pragma unroll
           for (int h = 0; h < 2; h++) {
-            if (!mbar_wait(bar_pf, hc & 1, abort_flag, status, 16)) { ok = false; break; }
+            if (!ha_barrier(bar_pf, hc & 1, abort_flag, status, 16)) { ok = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -259,7 +259,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       // everything this thread issued must retire before TMEM is released
       tc_commit(bar_drain);
-      mbar_wait(bar_drain, 0, abort_flag, nullptr, 0);
+      ha_barrier(bar_drain, 0, abort_flag, nullptr, 0);
     }
   } else {
     // ---------------------------------------------- softmax ---------------------------------------------------------
@@ -299,7 +299,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       hc++;
     };
     for (int n = 0; ok; n++) {
-      if (!mbar_wait(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
+      if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
       const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
@@ -322,7 +322,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const bool compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
         if (it + 1 < blocks) walk.next();
         else if (listed) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
-        if (!mbar_wait(bar_sf, sc & 1, abort_flag, status, 17)) { ok = false; break; }
+        if (!ha_barrier(bar_sf, sc & 1, abort_flag, status, 17)) { ok = false; break; }
         tc_fence_after();
         // keys of this block that this row sees: [0, lim], and among them those of its document
         const int lim = end - 1 - j * HA_BLOCK;
@@ -393,7 +393,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         else if ((mx - m_used) * p.mult > 8.0f) { alpha = fast_exp2((m_used - mx) * p.mult); l *= alpha; m_used = mx; rescale = true; }
         if (it > 0) {
           // the previous block's second half-product has retired: the buffer of weights is free and the accumulator at rest
-          if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) { ok = false; break; }
+          if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) { ok = false; break; }
           tc_fence_after();
           if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
@@ -410,7 +410,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         if (p.a.lengths && seq.length < p.a.Sk && seq.length < (j + 1) * HA_BLOCK) {
           // values behind the sequence's end: zero before they meet their weights of zero
-          if (!mbar_wait(bar_vf, (sc - 1) & 1, abort_flag, status, 26)) { ok = false; break; }
+          if (!ha_barrier(bar_vf, (sc - 1) & 1, abort_flag, status, 26)) { ok = false; break; }
           if (j * HA_BLOCK + row >= seq.length) {
 #pragma unroll 1
             for (int c = 0; c < DC; c++)
@@ -431,7 +431,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // the second half: its first 32 keys are exponentiated while the first half multiplies
           uint32_t pw[16];
           exps(r[2], mn2, ps2, pw);
-          if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
+          if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
           store(0, pw);
           exps(r[3], mn2, ps2, pw); store(1, pw);
         }
@@ -445,7 +445,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!ok) break;
       // ---- the tile's last product has retired: normalise and write the rows ----
       if (blocks > 0) {
-        if (!mbar_wait(bar_pv, (hc - 1) & 1, abort_flag, status, 20)) { ok = false; break; }
+        if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 20)) { ok = false; break; }
         tc_fence_after();
       }
       if (poisoned) l = __int_as_float(0x7fc00000);

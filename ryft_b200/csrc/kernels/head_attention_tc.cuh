@@ -110,15 +110,16 @@ inline HeadCap ha_cap(float softcap, float scale) {
   h.out2 = ha_pair(h.cap); h.twice2 = ha_pair(-2.0f * h.cap);
   return h;
 }
-// cap * tanh(x) of a pair
-__device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t x) {
+// cap * tanh(x) of a pair, and the same plus something
+__device__ __forceinline__ uint64_t cap_share(const HeadCap& h, uint64_t x) {
   const uint64_t y = mul2(x, x);
   uint64_t c = fma2(y, h.c4, h.c3);
   c = fma2(y, c, h.c2);
   c = fma2(y, c, h.c1);
-  c = fma2(y, c, h.c0);
-  return mul2(x, c);
+  return fma2(y, c, h.c0);
 }
+__device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t x) { return mul2(x, cap_share(h, x)); }
+__device__ __forceinline__ uint64_t cap_small_plus(const HeadCap& h, uint64_t x, uint64_t plus) { return fma2(x, cap_share(h, x), plus); }
 // q = 1 / (1 + e^2x)
 __device__ __forceinline__ uint64_t cap_rest(uint64_t x) {
   uint32_t a0, a1;
@@ -126,12 +127,50 @@ __device__ __forceinline__ uint64_t cap_rest(uint64_t x) {
   unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), splat2(1.f)), a0, a1);
   return pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
 }
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Waits for a TMEM load; naming its registers keeps their uses behind the wait.
+__device__ __forceinline__ void ha_wait(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+  asm volatile("" : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]),
+                    "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
 // Largest magnitude of 32 products, NaN if one is
 __device__ __forceinline__ float ha_largest(const uint32_t (&r)[32]) {
   float m[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 16; i++) m[i & 1] = max3(m[i & 1], fabsf(__uint_as_float(r[2 * i])), fabsf(__uint_as_float(r[2 * i + 1])));
   return max3(m[0], m[1], 0.f);
+}
+
+// sm100::mbar_wait with the thread asleep in between: most of a CTA's warps wait most of the time here, and what they poll with
+// is taken from the warps that compute.
+__device__ __forceinline__ bool ha_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(2000u)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool ha_barrier(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
+  for (uint32_t i = 0; i < (1u << 21); i++) {
+    if (ha_try_wait(bar, parity)) return true;
+    if (i > 4 && *abort_flag) return false;
+  }
+  *abort_flag = 1;
+  if (status) atomicCAS(status, 0, code);
+  return false;
 }
 
 // A tile as its loading warp publishes it.
