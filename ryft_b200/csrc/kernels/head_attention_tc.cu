@@ -46,12 +46,17 @@ template <int D> struct TileSmem {
   static constexpr int TOTAL = SLOT_OFF + 4 * (int)sizeof(TileSlot) + 1024;
 };
 
-template <int D, int EL>
+// What a kernel can do beside causal, prefix and length masks.  One kernel for everything left the warps of a plain problem waiting
+// for instructions and its registers spilled (2 x 16 heads of 4096 x 128, causal: 199 us where the plain form takes PLAIN_US).
+enum TileMode { TILE_PLAIN, TILE_CAP, TILE_DOCUMENTS, TILE_ANY };
+
+template <int D, int EL, int MODE>
 __global__ void __launch_bounds__(384, 1)
 k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const __grid_constant__ TileParams p, int32_t* sched, int32_t* status) {
   using namespace sm100;
   using SM = TileSmem<D>;
+  constexpr bool CAP = MODE == TILE_CAP || MODE == TILE_ANY, SLOPES = MODE == TILE_ANY, DOCUMENTS = MODE == TILE_DOCUMENTS || MODE == TILE_ANY;
   constexpr int DC = D / 64;
   constexpr uint32_t TMEM_COLS = 512;          // S0 [0,128), S1 [128,256), O0 [256, 256 + D), O1 [256 + D, 256 + 2 D)
 
@@ -69,7 +74,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  bar_se = wb + 56, bar_pf = wb + 64, bar_pv = wb + 72, bar_of = wb + 80, bar_tf = wb + 88 /* [2] */, bar_te = wb + 104 /* [2] */,
                  bar_drain = wb + 120;
   const uint32_t wbase = sbase + (uint32_t)w * SM::W_BYTES;
-  const bool listed = p.ranges != nullptr;
+  const bool listed = DOCUMENTS && p.ranges != nullptr;
 
   if (threadIdx.x == 0) {
     for (int v = 0; v < 2; v++) {
@@ -301,17 +306,22 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int n = 0; ok; n++) {
       if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
-      const int t = s->tile, blocks = s->blocks, b = s->b, h = s->h, q0 = s->at;
-      const HeadSequence seq{s->length, s->first, s->prefix};
-      // the blocks' bits stay this warp's to read until it has walked them
-      if (!listed || t < 0 || blocks == 0) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
+      const int t = s->tile, blocks = s->blocks;
       if (t < 0) break;
-      const int qrow = q0 + row, pos = seq.first + qrow;
-      const float slope = p.a.slopes ? ld_global(p.a.slopes + h) * kLog2e : 0.f;
-      int doc = 0, end = head_limit(p.a, seq, pos);
-      if (p.a.documents) {
-        if (pos >= 0 && pos < p.a.Sk) doc = (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos);
-        else end = 0;
+      // what is needed again at the tile's end is read again there: the slot stays this tile's until then
+      int pos = 0, end, doc = 0;
+      float slope = 0.f;
+      {
+        const HeadSequence seq{s->length, s->first, s->prefix};
+        pos = seq.first + s->at + row;
+        end = head_limit(p.a, seq, pos);
+        if constexpr (SLOPES) slope = p.a.slopes ? ld_global(p.a.slopes + s->h) * kLog2e : 0.f;
+        if constexpr (DOCUMENTS) {
+          if (p.a.documents) {
+            if (pos >= 0 && pos < p.a.Sk) doc = (int)ld_global((const uint32_t*)p.a.documents + (int64_t)s->b * p.a.Sk + pos);
+            else end = 0;
+          }
+        }
       }
       float m_used = -INFINITY, l = 0.f;
       bool poisoned = false;
@@ -319,9 +329,9 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (blocks > 0) walk.start(s, listed);
       for (int it = 0; it < blocks && ok; it++) {
         const int j = walk.j;
-        const bool compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
+        bool compare = false;
+        if constexpr (DOCUMENTS) compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
         if (it + 1 < blocks) walk.next();
-        else if (listed) { __syncwarp(); if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1)); }
         if (!ha_barrier(bar_sf, sc & 1, abort_flag, status, 17)) { ok = false; break; }
         tc_fence_after();
         // keys of this block that this row sees: [0, lim], and among them those of its document
@@ -335,7 +345,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_se);
         sc++;
-        if (p.cap.cap > 0.f) {
+        if (CAP && p.cap.cap > 0.f) {
           const float largest = max3(max3(ha_largest(r[0]), ha_largest(r[1]), 0.f), ha_largest(r[2]), ha_largest(r[3]));
           if (__all_sync(0xffffffffu, largest <= p.cap.small)) {
 #pragma unroll
@@ -350,13 +360,13 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               for (int i = 0; i < 16; i++)
                 unpack2(fma2(cap_rest(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), p.cap.twice2, p.cap.out2), r[c][2 * i], r[c][2 * i + 1]);
           }
-        } else if (p.scaled) {
+        } else if (MODE == TILE_ANY && p.scaled) {
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.in2), r[c][2 * i], r[c][2 * i + 1]);
         }
-        if (p.a.slopes) {
+        if (SLOPES && p.a.slopes) {
           const float far = (float)(pos - j * HA_BLOCK);
 #pragma unroll
           for (int c = 0; c < 4; c++)
@@ -367,9 +377,9 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 4; c++) {
             uint32_t bits = ha_bits(lim - c * 32);
-            if (compare) {
+            if (DOCUMENTS && compare) {
               const int key = j * HA_BLOCK + c * 32 + lane;
-              const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + key) : 0;
+              const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)s->b * p.a.Sk + key) : 0;
               bits &= ha_same_document(doc, theirs, key < p.a.Sk);
             }
 #pragma unroll
@@ -408,10 +418,10 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             tc_wait_st();
           }
         }
-        if (p.a.lengths && seq.length < p.a.Sk && seq.length < (j + 1) * HA_BLOCK) {
+        if (p.a.lengths && s->length < p.a.Sk && s->length < (j + 1) * HA_BLOCK) {
           // values behind the sequence's end: zero before they meet their weights of zero
           if (!ha_barrier(bar_vf, (sc - 1) & 1, abort_flag, status, 26)) { ok = false; break; }
-          if (j * HA_BLOCK + row >= seq.length) {
+          if (j * HA_BLOCK + row >= s->length) {
 #pragma unroll 1
             for (int c = 0; c < DC; c++)
 #pragma unroll
@@ -450,6 +460,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       if (poisoned) l = __int_as_float(0x7fc00000);
       const float inv = !(l <= 0.f) ? 1.0f / l : 0.f;   // a NaN sum stays NaN
+      const int b = s->b, h = s->h, qrow = s->at + row;
       char* orow = p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)h * p.a.os.head + (int64_t)qrow * p.a.os.token);
 #pragma unroll 1
       for (int c = 0; c < D / 16; c++) {
@@ -479,7 +490,10 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         p.a.lse[((int64_t)b * p.a.Hq + h) * p.a.Sq + qrow] = l == 0.f ? -INFINITY : (m_used * p.mult + fast_log2(l)) * 0.6931471805599453f;
       tc_fence_before();
       __syncwarp();
-      if (blocks > 0 && lane == 0) mbar_arrive(bar_of);
+      if (lane == 0) {
+        mbar_arrive(bar_te + 8 * (n & 1));
+        if (blocks > 0) mbar_arrive(bar_of);
+      }
     }
   }
 
@@ -510,10 +524,10 @@ __global__ void __launch_bounds__(256) k_document_ranges(const int32_t* document
   }
 }
 
-template <int D, int EL>
+template <int D, int EL, int MODE>
 int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileParams& p, int32_t* sched, int32_t* status, cudaStream_t stream) {
   using SM = TileSmem<D>;
-  auto kern = k_head_attention<D, EL>;
+  auto kern = k_head_attention<D, EL, MODE>;
   int dev = 0;
   cudaGetDevice(&dev);
   static std::atomic<bool> configured[64];
@@ -527,6 +541,15 @@ int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& 
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();
+}
+
+template <int D, int EL>
+int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileParams& p, int32_t* sched, int32_t* status, cudaStream_t stream) {
+  const bool cap = p.cap.cap > 0.f;
+  if (p.a.slopes || !(p.a.scale > 0.f) || (cap && p.a.documents)) return launch_tiles<D, EL, TILE_ANY>(q, k, v, p, sched, status, stream);
+  if (cap) return launch_tiles<D, EL, TILE_CAP>(q, k, v, p, sched, status, stream);
+  if (p.a.documents) return launch_tiles<D, EL, TILE_DOCUMENTS>(q, k, v, p, sched, status, stream);
+  return launch_tiles<D, EL, TILE_PLAIN>(q, k, v, p, sched, status, stream);
 }
 
 }  // namespace
