@@ -15,6 +15,7 @@
 // Rows of V behind a sequence's length are set to zero in shared memory before they meet their zero weights: a product of 0 and
 // what happens to lie there might be NaN.
 #include <atomic>
+#include <type_traits>
 
 #include "head_attention_tc.cuh"
 
@@ -56,6 +57,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                  const __grid_constant__ TileParams p, int32_t* sched, int32_t* status) {
   using namespace sm100;
   using SM = TileSmem<D>;
+  constexpr bool TWO_PASS = MODE == TILE_CAP;   // how the softmax warps go over a block
   constexpr bool CAP = MODE == TILE_CAP || MODE == TILE_ANY, SLOPES = MODE == TILE_ANY, DOCUMENTS = MODE == TILE_DOCUMENTS || MODE == TILE_ANY;
   constexpr int DC = D / 64;
   constexpr uint32_t TMEM_COLS = 512;          // S0 [0,128), S1 [128,256), O0 [256, 256 + D), O1 [256 + D, 256 + 2 D)
@@ -237,8 +239,8 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!issue_qk(blocks == 1)) { ok = false; break; }
         for (int it = 0; it < blocks && ok; it++) {
           // the block's scores are in the softmax warps' registers early: the next score block goes ahead of this
-          // block's products
-          if (it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
+          // block's products.  In two passes they are read to the end only while the first half multiplies: it goes between.
+          if (!TWO_PASS && it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
           if (!ha_barrier(bar_vf, vc & 1, abort_flag, status, 15)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulator
           if (it == 0 && nq > 0 && !ha_barrier(bar_of, (nq - 1) & 1, abort_flag, status, 24)) { ok = false; break; }
@@ -255,6 +257,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             tc_commit(bar_pv);     // the half's weights have been read; the accumulator holds them
             hc++;
+            if (h == 0 && TWO_PASS && it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
           }
           if (!ok) break;
           tc_commit(bar_ve);
@@ -325,6 +328,39 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       float m_used = -INFINITY, l = 0.f;
       bool poisoned = false;
+      // the previous block's second half-product has retired: the buffer of weights is free and the accumulator at rest
+      auto settle = [&](int it, bool rescale, float alpha) -> bool {
+        if (it == 0) return true;
+        if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) return false;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t o[16];
+            tmem_ld_32x16(o_addr + (uint32_t)(c * 16), o);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x16(o_addr + (uint32_t)(c * 16), o);
+          }
+          tc_wait_st();
+        }
+        return true;
+      };
+      // values behind the sequence's end: zero before they meet their weights of zero
+      uint32_t vc = sc;                           // the tile's first V block; its count goes with the score blocks
+      auto clear_tail = [&](int j) -> bool {
+        const uint32_t turn = vc++;
+        if (!p.a.lengths || s->length >= p.a.Sk || s->length >= (j + 1) * HA_BLOCK) return true;
+        if (!ha_barrier(bar_vf, turn & 1, abort_flag, status, 26)) return false;
+        if (j * HA_BLOCK + row >= s->length) {
+#pragma unroll 1
+          for (int c = 0; c < DC; c++)
+#pragma unroll
+            for (int q = 0; q < 8; q++) sts_v4(wbase + (uint32_t)(SM::V_OFF + c * HA_CHUNK + row * 128 + q * 16), 0, 0, 0, 0);
+        }
+        return true;
+      };
       BlockWalk walk;
       if (blocks > 0) walk.start(s, listed);
       for (int it = 0; it < blocks && ok; it++) {
@@ -337,6 +373,102 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         // keys of this block that this row sees: [0, lim], and among them those of its document
         const int lim = end - 1 - j * HA_BLOCK;
         const bool need_mask = compare || __any_sync(0xffffffffu, lim < HA_BLOCK - 1);
+        if constexpr (TWO_PASS) {
+          // Capped scores: the cap is monotonic, so a first pass finds the row's maximum among the products, a second caps, weighs and
+          // stores 32 columns at a time, a loop of a few registers and little code.  The score buffer is handed back late, which
+          // this much arithmetic hides.  (With all 128 scores in registers, as below: 263 us where this takes 2xx.)
+          uint32_t seen[4];
+          float hi = -INFINITY, lo = INFINITY;
+          if (need_mask) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+              seen[c] = ha_bits(lim - c * 32);
+              if (DOCUMENTS && compare) {
+                const int key = j * HA_BLOCK + c * 32 + lane;
+                const int theirs = key < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)s->b * p.a.Sk + key) : 0;
+                seen[c] &= ha_same_document(doc, theirs, key < p.a.Sk);
+              }
+            }
+          }
+#pragma unroll 1
+          for (int c = 0; c < 4; c++) {
+            uint32_t r[32];
+            tmem_ld_32x32(s_addr + (uint32_t)(c * 32), r);
+            ha_wait(r);
+            if (need_mask) {
+              const uint32_t bits = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+#pragma unroll
+              for (int i = 0; i < 32; i++)
+                if ((bits >> i) & 1u) { hi = max3(hi, __uint_as_float(r[i]), hi); lo = min3(lo, __uint_as_float(r[i]), lo); }
+            } else {
+              float h2[2] = {hi, hi}, l2[2] = {lo, lo};
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                h2[i & 1] = max3(h2[i & 1], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+                l2[i & 1] = min3(l2[i & 1], __uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+              }
+              hi = max3(h2[0], h2[1], h2[0]); lo = min3(l2[0], l2[1], l2[0]);
+            }
+          }
+          const bool small = __all_sync(0xffffffffu, hi <= p.cap.small && lo >= -p.cap.small);
+          float mx = -INFINITY;
+          if (hi != -INFINITY) {
+            const uint64_t x = mul2(splat2(hi), p.cap.in2);
+            uint32_t v0, v1;
+            unpack2(small ? cap_small(p.cap, x) : fma2(cap_rest(x), p.cap.twice2, p.cap.out2), v0, v1);
+            mx = __uint_as_float(v0);
+          }
+          if (hi != hi || lo != lo) { poisoned = true; mx = 0.f; }
+          float alpha = 1.f;
+          bool rescale = false;
+          if (it == 0) m_used = mx;
+          else if (mx - m_used > 8.0f) { alpha = fast_exp2(m_used - mx); l *= alpha; m_used = mx; rescale = true; }
+          if (!settle(it, rescale, alpha) || !clear_tail(j)) { ok = false; break; }
+          const uint64_t mn2 = splat2(m_used == -INFINITY ? 0.f : -m_used);
+          uint64_t ps2[2] = {0ull, 0ull};
+          auto chunks = [&](auto SMALL, auto MASK) {
+#pragma unroll 1
+            for (int c = 0; c < 4; c++) {
+              uint32_t r[32], pw[16];
+              tmem_ld_32x32(s_addr + (uint32_t)(c * 32), r);
+              ha_wait(r);
+              if (c == 3) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_se);
+              }
+              const uint32_t bits = c == 0 ? seen[0] : c == 1 ? seen[1] : c == 2 ? seen[2] : seen[3];
+#pragma unroll
+              for (int h2 = 0; h2 < 16; h2++) {
+                const uint64_t x = mul2(pack2(r[2 * h2], r[2 * h2 + 1]), p.cap.in2);
+                uint64_t y;
+                if constexpr (decltype(SMALL)::value) y = cap_small_plus(p.cap, x, mn2);
+                else y = add2(fma2(cap_rest(x), p.cap.twice2, p.cap.out2), mn2);
+                uint32_t t0, t1;
+                unpack2(y, t0, t1);
+                if constexpr (decltype(MASK)::value) {
+                  if (!((bits >> (2 * h2)) & 1u)) t0 = 0xff800000u;
+                  if (!((bits >> (2 * h2 + 1)) & 1u)) t1 = 0xff800000u;
+                }
+                const float e0 = fast_exp2(__uint_as_float(t0)), e1 = fast_exp2(__uint_as_float(t1));
+                ps2[h2 & 1] = add2(ps2[h2 & 1], pack2(__float_as_uint(e0), __float_as_uint(e1)));
+                pw[h2] = ha_pack<EL>(e0, e1);
+              }
+              // the first half's product has retired: its buffer takes the second half
+              if (c == 2 && !ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
+              store(c & 1, pw);
+              if (c & 1) publish();
+            }
+          };
+          using std::bool_constant;
+          if (small) { if (need_mask) chunks(bool_constant<true>{}, bool_constant<true>{}); else chunks(bool_constant<true>{}, bool_constant<false>{}); }
+          else { if (need_mask) chunks(bool_constant<false>{}, bool_constant<true>{}); else chunks(bool_constant<false>{}, bool_constant<false>{}); }
+          sc++;
+          if (!ok) break;
+          uint32_t a0, a1, b0, b1;
+          unpack2(ps2[0], a0, a1); unpack2(ps2[1], b0, b1);
+          l += (__uint_as_float(a0) + __uint_as_float(a1)) + (__uint_as_float(b0) + __uint_as_float(b1));
+        } else {
         uint32_t r[4][32];
 #pragma unroll
         for (int c = 0; c < 4; c++) tmem_ld_32x32(s_addr + (uint32_t)(c * 32), r[c]);
@@ -401,33 +533,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         bool rescale = false;
         if (it == 0) m_used = mx;
         else if ((mx - m_used) * p.mult > 8.0f) { alpha = fast_exp2((m_used - mx) * p.mult); l *= alpha; m_used = mx; rescale = true; }
-        if (it > 0) {
-          // the previous block's second half-product has retired: the buffer of weights is free and the accumulator at rest
-          if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) { ok = false; break; }
-          tc_fence_after();
-          if (__any_sync(0xffffffffu, rescale)) {
-#pragma unroll 1
-            for (int c = 0; c < D / 16; c++) {
-              uint32_t o[16];
-              tmem_ld_32x16(o_addr + (uint32_t)(c * 16), o);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-              tmem_st_32x16(o_addr + (uint32_t)(c * 16), o);
-            }
-            tc_wait_st();
-          }
-        }
-        if (p.a.lengths && s->length < p.a.Sk && s->length < (j + 1) * HA_BLOCK) {
-          // values behind the sequence's end: zero before they meet their weights of zero
-          if (!ha_barrier(bar_vf, (sc - 1) & 1, abort_flag, status, 26)) { ok = false; break; }
-          if (j * HA_BLOCK + row >= s->length) {
-#pragma unroll 1
-            for (int c = 0; c < DC; c++)
-#pragma unroll
-              for (int q = 0; q < 8; q++) sts_v4(wbase + (uint32_t)(SM::V_OFF + c * HA_CHUNK + row * 128 + q * 16), 0, 0, 0, 0);
-          }
-        }
+        if (!settle(it, rescale, alpha) || !clear_tail(j)) { ok = false; break; }
         const float mneg = (m_used == -INFINITY) ? 0.f : -m_used * p.mult;
         const uint64_t mn2 = splat2(mneg);
         uint64_t ps2[2] = {0ull, 0ull};
@@ -450,6 +556,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           uint32_t a0, a1, b0, b1;
           unpack2(ps2[0], a0, a1); unpack2(ps2[1], b0, b1);
           l += (__uint_as_float(a0) + __uint_as_float(a1)) + (__uint_as_float(b0) + __uint_as_float(b1));
+        }
         }
       }
       if (!ok) break;
