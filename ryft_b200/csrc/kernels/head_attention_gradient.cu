@@ -27,7 +27,6 @@ namespace b2x {
 namespace {
 
 constexpr int GRAD_UNIT = 64;         // keys (dQ) or queries (dK, dV) per step
-constexpr int GRAD_STAGES = 4;
 
 struct GradParams {
   HeadAttn a;
@@ -141,12 +140,13 @@ __device__ __forceinline__ void grad_write_row(uint32_t taddr, char* row, bool t
 template <int D> struct GradSmem {
   static constexpr int T_BYTES = HA_BLOCK * D * 2;         // the tile's Q and dO, or K and V
   static constexpr int U_BYTES = GRAD_UNIT * D * 2;        // a unit's K and V, or Q and dO
+  static constexpr int STAGES = D == 64 ? 8 : 5;           // what fits; with four at a width of 128 the products waited 530 cycles of 2270 per unit for loads
   static constexpr int T0_OFF = 0, T1_OFF = T_BYTES;
-  static constexpr int U_OFF = 2 * T_BYTES;                // GRAD_STAGES x 2
-  static constexpr int ROW_OFF = U_OFF + GRAD_STAGES * 2 * U_BYTES;   // row constants: 2 groups x 2 turns x (64 + 64) floats
+  static constexpr int U_OFF = 2 * T_BYTES;                // STAGES x 2
+  static constexpr int ROW_OFF = U_OFF + STAGES * 2 * U_BYTES;   // row constants: 2 groups x 2 turns x (64 + 64) floats
   static constexpr int BAR_OFF = ROW_OFF + 2 * 2 * 512;
-  static constexpr int SLOT_OFF = BAR_OFF + 256;
-  static constexpr int TOTAL = SLOT_OFF + 2 * (int)sizeof(TileSlot) + 1024;
+  static constexpr int SLOT_OFF = BAR_OFF + 264;            // 15 + 2 x STAGES barriers, TMEM slot, abort flag
+  static constexpr int TOTAL = SLOT_OFF + 2 * (int)sizeof(TileSlot);
 };
 
 // KEYS: tiles of keys (dK, dV); else tiles of queries (dQ).  t0, t1: Q and dO, or K and V; u0, u1: K and V, or Q and dO.
@@ -156,17 +156,17 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
                      const __grid_constant__ CUtensorMap tmU1, const __grid_constant__ GradParams p, int32_t* sched, int32_t* status) {
   using namespace sm100;
   using SM = GradSmem<D>;
-  constexpr int DC = D / 64;
+  constexpr int DC = D / 64, STAGES = SM::STAGES;
   constexpr uint32_t U_CHUNK = GRAD_UNIT * 128;            // one [64 rows x 128 bytes] swizzled sub-tile
   constexpr uint32_t TMEM_COLS = 512;          // pair g: S [128 g, +64), dP [128 g + 64, +64); dQ or dV [256, 256 + D), dK [256 + D, 256 + 2 D)
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  // swizzled tiles start on 1024 bytes; there is no room to round up to them
+  extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const uint32_t b0 = sbase + SM::BAR_OFF;
-  const uint32_t bar_tl = b0, bar_tu = b0 + 8 /* tile loaded, tile used */, bar_uf = b0 + 16 /* [4] */, bar_ue = b0 + 48 /* [4] */, bar_sf = b0 + 80 /* [2] */,
-                 bar_pf = b0 + 96 /* [2] */, bar_end = b0 + 112, bar_of = b0 + 120, bar_tf = b0 + 128 /* [2] */, bar_te = b0 + 144 /* [2] */, bar_drain = b0 + 160,
-                 bar_rf = b0 + 168 /* [2] */;
-  uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 192);
+  const uint32_t bar_tl = b0, bar_tu = b0 + 8 /* tile loaded, tile used */, bar_sf = b0 + 16 /* [2] */, bar_pf = b0 + 32 /* [2] */, bar_end = b0 + 48, bar_of = b0 + 56,
+                 bar_tf = b0 + 64 /* [2] */, bar_te = b0 + 80 /* [2] */, bar_drain = b0 + 96, bar_rf = b0 + 104 /* [2] */, bar_uf = b0 + 120 /* [STAGES] */,
+                 bar_ue = bar_uf + 8 * STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 248);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile TileSlot* slots = (volatile TileSlot*)(smem + SM::SLOT_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -175,7 +175,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
 
   if (threadIdx.x == 0) {
     mbar_init(bar_tl, 1); mbar_init(bar_tu, 1); mbar_init(bar_end, 1); mbar_init(bar_of, 8); mbar_init(bar_drain, 1);
-    for (uint32_t s = 0; s < 8 * GRAD_STAGES; s += 8) { mbar_init(bar_uf + s, 1); mbar_init(bar_ue + s, 1); }
+    for (uint32_t s = 0; s < 8 * STAGES; s += 8) { mbar_init(bar_uf + s, 1); mbar_init(bar_ue + s, 1); }
     for (uint32_t s = 0; s < 16; s += 8) { mbar_init(bar_sf + s, 1); mbar_init(bar_pf + s, 4); mbar_init(bar_rf + s, 4); mbar_init(bar_tf + s, 1); mbar_init(bar_te + s, 9); }
     *abort_flag = 0;
     mbar_fence_init();
@@ -201,6 +201,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         if (lane == 0) t = atomicAdd(sched, 1);
         t = __shfl_sync(0xffffffffu, t, 0);
       } else { t = fixed; fixed += (int)gridDim.x; }
+      if ((sbase & 1023u) != 0) { t = -1; if (lane == 0 && status) atomicCAS(status, 0, 60); }   // nothing is touched
       if (t >= p.total) t = -1;
       volatile TileSlot* s = slots + (n & 1);
       int b = 0, h = 0, at = 0, begin = 0, units = 0;
@@ -277,7 +278,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
             BlockWalk walk;
             walk.start(s, listed);
             for (int it = 0; it < units; it++, k++) {
-              const uint32_t st = k % GRAD_STAGES, turn = k / GRAD_STAGES;
+              const uint32_t st = k % STAGES, turn = k / STAGES;
               if (turn > 0 && !ha_barrier(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
               mbar_expect_tx(bar_uf + 8 * st, 2 * SM::U_BYTES);
               const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES;
@@ -303,9 +304,9 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       const uint32_t ta = sbase + SM::T0_OFF, tb = sbase + SM::T1_OFF;
       bool ok = true;
       auto issue_scores = [&](bool last_of_tile) -> bool {
-        const uint32_t st = sc % GRAD_STAGES, g = sc & 1;
+        const uint32_t st = sc % STAGES, g = sc & 1;
         const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
-        if (!ha_barrier(bar_uf + 8 * st, (sc / GRAD_STAGES) & 1, abort_flag, status, 71)) return false;
+        if (!ha_barrier(bar_uf + 8 * st, (sc / STAGES) & 1, abort_flag, status, 71)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
@@ -331,7 +332,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         if (!ha_barrier(bar_tl, nt & 1, abort_flag, status, 73)) { ok = false; break; }
         for (int it = 0; it < 2 && it < total && ok; it++) ok = issue_scores(it + 1 == total);
         for (int it = 0; it < total && ok; it++) {
-          const uint32_t st = uc % GRAD_STAGES, g = uc & 1;
+          const uint32_t st = uc % STAGES, g = uc & 1;
           const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
           if (!ha_barrier(bar_pf + 8 * g, (uc >> 1) & 1, abort_flag, status, 74)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulators
@@ -411,7 +412,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       }
       while (k < total && ok) {
         const int unit = walk.j, head = KEYS ? th * p.a.group + hh : th;
-        const uint32_t stage = (uc + (uint32_t)k) % GRAD_STAGES;
+        const uint32_t stage = (uc + (uint32_t)k) % STAGES;
         const bool compare = listed ? (s->compare[unit >> 5] >> (unit & 31)) & 1 : p.a.documents != nullptr;
         const uint32_t rows_at = sbase + (uint32_t)(SM::ROW_OFF + (g * 2 + (int)(mine & 1)) * 512);
         if constexpr (KEYS) {
