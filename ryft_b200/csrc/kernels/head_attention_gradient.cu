@@ -115,58 +115,62 @@ __device__ __forceinline__ void grad_wait(uint32_t (&a)[16], uint32_t (&b)[16]) 
 // Lets the loads in flight land before shared memory goes away.
 __device__ __forceinline__ void grad_linger() { for (uint32_t i = 0; i < 4096; i++) __nanosleep(256); }
 
-// A row of an accumulator times `f`, as 16-bit values
-template <int EL, int D>
-__device__ __forceinline__ void grad_write_row(uint32_t taddr, char* row, bool there, int width, float f, bool zero) {
-#pragma unroll 1
-  for (int c = 0; c < D / 16; c++) {
-    uint32_t x[16];
-    if (!zero) { sm100::tmem_ld_32x16(taddr + (uint32_t)(c * 16), x); sm100::tc_wait_ld(); }
-    else {
+// Sixteen columns of a row of an accumulator times `f`, as 16-bit values; `width` of them exist
+template <int EL>
+__device__ __forceinline__ void grad_write(uint32_t taddr, char* row, bool there, int width, float f, bool zero) {
+  uint32_t x[16];
+  if (!zero) { sm100::tmem_ld_32x16(taddr, x); sm100::tc_wait_ld(); }
+  else {
 #pragma unroll
-      for (int i = 0; i < 16; i++) x[i] = 0;
-    }
+    for (int i = 0; i < 16; i++) x[i] = 0;
+  }
 #pragma unroll
-    for (int q = 0; q < 2; q++) {
-      uint32_t wd[4];
+  for (int q = 0; q < 2; q++) {
+    uint32_t wd[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) wd[k] = ha_pack<EL>(__uint_as_float(x[q * 8 + 2 * k]) * f, __uint_as_float(x[q * 8 + 2 * k + 1]) * f);
-      if (there && c * 16 + q * 8 < width) *reinterpret_cast<uint4*>(row + 2 * (c * 16 + q * 8)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
-    }
+    for (int k = 0; k < 4; k++) wd[k] = ha_pack<EL>(__uint_as_float(x[q * 8 + 2 * k]) * f, __uint_as_float(x[q * 8 + 2 * k + 1]) * f);
+    if (there && q * 8 < width) *reinterpret_cast<uint4*>(row + 2 * (q * 8)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
   }
 }
 
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------
+// Pairs of score buffers in TMEM, each with four warps of its own: as many as the accumulators leave room for
+template <int D, bool KEYS> struct GradShape {
+  static constexpr int GROUPS = KEYS && D == 128 ? 2 : 3;
+  static constexpr int THREADS = 128 + 128 * GROUPS;
+};
+
 template <int D> struct GradSmem {
   static constexpr int T_BYTES = HA_BLOCK * D * 2;         // the tile's Q and dO, or K and V
   static constexpr int U_BYTES = GRAD_UNIT * D * 2;        // a unit's K and V, or Q and dO
   static constexpr int STAGES = D == 64 ? 8 : 5;           // what fits; with four at a width of 128 the products waited 530 cycles of 2270 per unit for loads
   static constexpr int T0_OFF = 0, T1_OFF = T_BYTES;
   static constexpr int U_OFF = 2 * T_BYTES;                // STAGES x 2
-  static constexpr int ROW_OFF = U_OFF + STAGES * 2 * U_BYTES;   // row constants: 2 groups x 2 turns x (64 + 64) floats
-  static constexpr int BAR_OFF = ROW_OFF + 2 * 2 * 512;
-  static constexpr int SLOT_OFF = BAR_OFF + 264;            // 15 + 2 x STAGES barriers, TMEM slot, abort flag
+  static constexpr int ROW_OFF = U_OFF + STAGES * 2 * U_BYTES;   // row constants of keys' tiles: groups x 2 turns x (64 + 64) floats
+  static constexpr int BAR_OFF = ROW_OFF + GradShape<D, true>::GROUPS * 2 * 512;
+  static constexpr int SLOT_OFF = BAR_OFF + 288;            // 18 + 2 x STAGES barriers, TMEM slot, abort flag
   static constexpr int TOTAL = SLOT_OFF + 2 * (int)sizeof(TileSlot);
 };
 
 // KEYS: tiles of keys (dK, dV); else tiles of queries (dQ).  t0, t1: Q and dO, or K and V; u0, u1: K and V, or Q and dO.
 template <int D, int EL, bool KEYS>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(GradShape<D, KEYS>::THREADS, 1)
 k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_constant__ CUtensorMap tmT1, const __grid_constant__ CUtensorMap tmU0,
                      const __grid_constant__ CUtensorMap tmU1, const __grid_constant__ GradParams p, int32_t* sched, int32_t* status) {
   using namespace sm100;
   using SM = GradSmem<D>;
-  constexpr int DC = D / 64, STAGES = SM::STAGES;
+  constexpr int DC = D / 64, STAGES = SM::STAGES, GROUPS = GradShape<D, KEYS>::GROUPS;
   constexpr uint32_t U_CHUNK = GRAD_UNIT * 128;            // one [64 rows x 128 bytes] swizzled sub-tile
-  constexpr uint32_t TMEM_COLS = 512;          // pair g: S [128 g, +64), dP [128 g + 64, +64); dQ or dV [256, 256 + D), dK [256 + D, 256 + 2 D)
+  constexpr uint32_t TMEM_COLS = 512;          // pair g: S [128 g, +64), dP [128 g + 64, +64); behind the pairs dQ, or dV and dK
+  constexpr uint32_t ACC = GROUPS * 128;
   // swizzled tiles start on 1024 bytes; there is no room to round up to them
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
   const uint32_t b0 = sbase + SM::BAR_OFF;
-  const uint32_t bar_tl = b0, bar_tu = b0 + 8 /* tile loaded, tile used */, bar_sf = b0 + 16 /* [2] */, bar_pf = b0 + 32 /* [2] */, bar_end = b0 + 48, bar_of = b0 + 56,
-                 bar_tf = b0 + 64 /* [2] */, bar_te = b0 + 80 /* [2] */, bar_drain = b0 + 96, bar_rf = b0 + 104 /* [2] */, bar_uf = b0 + 120 /* [STAGES] */,
+  const uint32_t bar_tl = b0, bar_tu = b0 + 8 /* tile loaded, tile used */, bar_end = b0 + 16, bar_of = b0 + 24, bar_tf = b0 + 32 /* [2] */, bar_te = b0 + 48 /* [2] */,
+                 bar_drain = b0 + 64, bar_sf = b0 + 72 /* [3] */, bar_pf = b0 + 96 /* [3] */, bar_rf = b0 + 120 /* [3] */, bar_uf = b0 + 144 /* [STAGES] */,
                  bar_ue = bar_uf + 8 * STAGES;
-  uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 248);
+  uint32_t* tmem_slot = (uint32_t*)(smem + SM::BAR_OFF + 272);
   volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
   volatile TileSlot* slots = (volatile TileSlot*)(smem + SM::SLOT_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -174,9 +178,10 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
   const int repeat = KEYS ? p.a.group : 1;     // heads that pass by a tile
 
   if (threadIdx.x == 0) {
-    mbar_init(bar_tl, 1); mbar_init(bar_tu, 1); mbar_init(bar_end, 1); mbar_init(bar_of, 8); mbar_init(bar_drain, 1);
+    mbar_init(bar_tl, 1); mbar_init(bar_tu, 1); mbar_init(bar_end, 1); mbar_init(bar_of, 4 * GROUPS); mbar_init(bar_drain, 1);
     for (uint32_t s = 0; s < 8 * STAGES; s += 8) { mbar_init(bar_uf + s, 1); mbar_init(bar_ue + s, 1); }
-    for (uint32_t s = 0; s < 16; s += 8) { mbar_init(bar_sf + s, 1); mbar_init(bar_pf + s, 4); mbar_init(bar_rf + s, 4); mbar_init(bar_tf + s, 1); mbar_init(bar_te + s, 9); }
+    for (uint32_t s = 0; s < 8 * GROUPS; s += 8) { mbar_init(bar_sf + s, 1); mbar_init(bar_pf + s, 4); mbar_init(bar_rf + s, 4); }
+    for (uint32_t s = 0; s < 16; s += 8) { mbar_init(bar_tf + s, 1); mbar_init(bar_te + s, 1 + 4 * GROUPS); }
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmT0); tma_prefetch_desc(&tmT1); tma_prefetch_desc(&tmU0); tma_prefetch_desc(&tmU1);
@@ -304,7 +309,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       const uint32_t ta = sbase + SM::T0_OFF, tb = sbase + SM::T1_OFF;
       bool ok = true;
       auto issue_scores = [&](bool last_of_tile) -> bool {
-        const uint32_t st = sc % STAGES, g = sc & 1;
+        const uint32_t st = sc % STAGES, g = sc % GROUPS;
         const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
         if (!ha_barrier(bar_uf + 8 * st, (sc / STAGES) & 1, abort_flag, status, 71)) return false;
         tc_fence_after();
@@ -330,11 +335,11 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         if (t < 0) break;
         if (total == 0) continue;
         if (!ha_barrier(bar_tl, nt & 1, abort_flag, status, 73)) { ok = false; break; }
-        for (int it = 0; it < 2 && it < total && ok; it++) ok = issue_scores(it + 1 == total);
+        for (int it = 0; it < GROUPS && it < total && ok; it++) ok = issue_scores(it + 1 == total);
         for (int it = 0; it < total && ok; it++) {
-          const uint32_t st = uc % STAGES, g = uc & 1;
+          const uint32_t st = uc % STAGES, g = uc % GROUPS;
           const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
-          if (!ha_barrier(bar_pf + 8 * g, (uc >> 1) & 1, abort_flag, status, 74)) { ok = false; break; }
+          if (!ha_barrier(bar_pf + 8 * g, (uc / GROUPS) & 1, abort_flag, status, 74)) { ok = false; break; }
           // the previous tile's rows have been read out of the accumulators
           if (it == 0 && nt > 0 && !ha_barrier(bar_of, (nt - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
           tc_fence_after();
@@ -342,17 +347,17 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
           if constexpr (KEYS) {
 #pragma unroll
             for (int k = 0; k < GRAD_UNIT / 16; k++)
-              umma_ts_f16(tmem_base + 256u, tmem_base + g * 128u + (uint32_t)(k * 8), make_smem_desc(ub + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+              umma_ts_f16(tmem_base + ACC, tmem_base + g * 128u + (uint32_t)(k * 8), make_smem_desc(ub + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
           }
 #pragma unroll
           for (int k = 0; k < GRAD_UNIT / 16; k++)
-            umma_ts_f16(tmem_base + 256u + (KEYS ? (uint32_t)D : 0u), tmem_base + g * 128u + 64u + (uint32_t)(k * 8), make_smem_desc(ua + (uint32_t)k * 2048, U_CHUNK, 1024),
+            umma_ts_f16(tmem_base + ACC + (KEYS ? (uint32_t)D : 0u), tmem_base + g * 128u + 64u + (uint32_t)(k * 8), make_smem_desc(ua + (uint32_t)k * 2048, U_CHUNK, 1024),
                         p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
           tc_commit(bar_ue + 8 * st);
           if (it + 1 == total) tc_commit(bar_end);
           uc++;
           // the tensor pipe keeps this thread's order: the pair's next scores come after the products that read it
-          if (it + 2 < total && !issue_scores(it + 3 == total)) { ok = false; break; }
+          if (it + GROUPS < total && !issue_scores(it + GROUPS + 1 == total)) { ok = false; break; }
         }
         nt++;
       }
@@ -362,7 +367,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     }
   } else if (warp >= 4) {
     // ---------------------------------------------- P and dS --------------------------------------------------------
-    const int g = (warp - 4) >> 2;                // this group's pair of buffers: units of this parity
+    const int g = (warp - 4) >> 2;                // this group's pair of buffers: every GROUPS-th unit
     const int quad = warp & 3, row = quad * 32 + lane, tid = (int)threadIdx.x - 128 - g * 128;
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(g * 128);
@@ -407,7 +412,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       float ahead = 0.f;
       if (total > 0) {
         walk.start(s, listed);
-        if ((uc & 1) != (uint32_t)g) { k++; advance(); }
+        for (uint32_t first = ((uint32_t)g + GROUPS - uc % GROUPS) % GROUPS; k < (int)first && k < total; k++) advance();
         if (KEYS && k < total) ahead = fetch(hh, walk.j);
       }
       while (k < total && ok) {
@@ -420,9 +425,8 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_rf + 8 * g);
         }
-        k += 2;
-        advance();
-        if (k - 1 < total) { advance(); if (KEYS && k < total) ahead = fetch(hh, walk.j); }
+        for (int i = 0; i < GROUPS && k < total; i++, k++) advance();
+        if (KEYS && k < total) ahead = fetch(hh, walk.j);
         // the group's four warps have stored theirs (and read those of two units ago)
         if (KEYS && !ha_barrier(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
         if (!ha_barrier(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
@@ -514,15 +518,14 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         tc_fence_after();
         nt++;
       }
-      if constexpr (KEYS) {
-        // one group writes dV, the other dK
-        const B2xHeadStrides& o = g == 0 ? p.a.dvs : p.a.dks;
-        char* out = (g == 0 ? p.a.dv : p.a.dk) + 2 * ((int64_t)b * o.batch + (int64_t)th * o.head + (int64_t)self * o.token);
-        grad_write_row<EL, D>(tmem_base + lane_addr + 256u + (uint32_t)(g * D), out, self < p.a.Sk, p.a.D, g == 0 ? 1.f : p.scale, total == 0);
-      } else {
-        // each group writes half of the width
-        char* out = p.a.dq + 2 * ((int64_t)b * p.a.dqs.batch + (int64_t)th * p.a.dqs.head + (int64_t)self * p.a.dqs.token + g * (D / 2));
-        grad_write_row<EL, D / 2>(tmem_base + lane_addr + 256u + (uint32_t)(g * (D / 2)), out, self < p.a.Sq, p.a.D - g * (D / 2), p.scale, total == 0);
+      // sixteen columns at a time, the groups in turn: dQ, or dV and then dK
+#pragma unroll 1
+      for (int c = g; c < (KEYS ? 2 : 1) * (D / 16); c += GROUPS) {
+        const bool second = c >= D / 16;
+        const int first = (second ? c - D / 16 : c) * 16;
+        const B2xHeadStrides& o = !KEYS ? p.a.dqs : second ? p.a.dks : p.a.dvs;
+        char* out = (!KEYS ? p.a.dq : second ? p.a.dk : p.a.dv) + 2 * ((int64_t)b * o.batch + (int64_t)th * o.head + (int64_t)self * o.token + first);
+        grad_write<EL>(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), out, self < (KEYS ? p.a.Sk : p.a.Sq), p.a.D - first, KEYS && !second ? 1.f : p.scale, total == 0);
       }
       tc_fence_before();
       __syncwarp();
@@ -607,7 +610,7 @@ int launch_side(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* st
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(384), SM::TOTAL, stream, t0, t1, u0, u1, p, sched_slot(stream), status);
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(GradShape<D, KEYS>::THREADS), SM::TOTAL, stream, t0, t1, u0, u1, p, sched_slot(stream), status);
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();
