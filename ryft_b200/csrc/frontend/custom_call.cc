@@ -148,7 +148,7 @@ RotarySpec describe_rotary(Reader& r, bool gradient) {
     }
   }
   if (s.positions >= 0) r.same(r.in(s.positions), type_of(DType::S32, {s.B, s.S}), "the positions");
-  r.limit(s.B * s.S < (1ll << 31) && s.heads[0] + s.heads[1] < (1 << 20), "too many tokens or heads");
+  r.limit(s.B < (1ll << 31) && s.S < (1ll << 31) && s.B * s.S < (1ll << 31) && s.heads[0] < (1 << 20) && s.heads[1] < (1 << 20), "too many tokens or heads");
   return s;
 }
 

@@ -610,7 +610,7 @@ int launch_side(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* st
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) ready[dev].store(true, std::memory_order_release);
   }
-  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(GradShape<D, KEYS>::THREADS), SM::TOTAL, stream, t0, t1, u0, u1, p, sched_slot(stream), status);
+  const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(GradShape<D, KEYS>::THREADS), SM::TOTAL, stream, t0, t1, u0, u1, p, ha_sched(stream), status);
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();

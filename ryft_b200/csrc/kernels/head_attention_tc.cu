@@ -701,7 +701,7 @@ int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status
   if (!ha_encode(&q, elem, a.q, a.qs, a.B, a.Hq, a.Sq, a.D)) return (int)cudaErrorInvalidValue;
   if (a.Sk == 0) k = v = q;      // nothing is loaded
   else if (!ha_encode(&k, elem, a.k, a.ks, a.B, a.Hk, a.Sk, a.D) || !ha_encode(&v, elem, a.v, a.vs, a.B, a.Hk, a.Sk, a.D)) return (int)cudaErrorInvalidValue;
-  int32_t* sched = sched_slot(stream);
+  int32_t* sched = ha_sched(stream);
   if (D == 64) return elem == EL_BF16 ? launch_tiles<64, EL_BF16>(q, k, v, p, sched, status, stream) : launch_tiles<64, EL_F16>(q, k, v, p, sched, status, stream);
   return elem == EL_BF16 ? launch_tiles<128, EL_BF16>(q, k, v, p, sched, status, stream) : launch_tiles<128, EL_F16>(q, k, v, p, sched, status, stream);
 }

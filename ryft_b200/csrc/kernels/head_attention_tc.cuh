@@ -200,6 +200,13 @@ struct BlockWalk {
 
 
 int32_t* sched_slot(cudaStream_t stream);   // gemm_tc.cu: a (tile counter, finished CTAs) pair per stream
+// The same, or nullptr (tiles dealt out in a fixed order) while the stream is captured: graphs of one stream may later run side by
+// side, and would share the counter.
+inline int32_t* ha_sched(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) return nullptr;
+  return sched_slot(stream);
+}
 
 // Blocks of 128 tokens and the launches of the entry points.
 int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream);
