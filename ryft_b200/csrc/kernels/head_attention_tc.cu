@@ -48,8 +48,9 @@ template <int D> struct TileSmem {
 };
 
 // What a kernel can do beside causal, prefix and length masks.  One kernel for everything left the warps of a plain problem waiting
-// for instructions and its registers spilled (2 x 16 heads of 4096 x 128, causal: 199 us where the plain form takes PLAIN_US).
-enum TileMode { TILE_PLAIN, TILE_CAP, TILE_DOCUMENTS, TILE_ANY };
+// for instructions and its registers spilled (2 x 16 heads of 4096 x 128, causal: 199 us where the
+// plain form takes 157).
+enum TileMode { TILE_PLAIN, TILE_CAP /* and documents */, TILE_DOCUMENTS, TILE_ANY /* a bias by distance, scales that are not positive */ };
 
 template <int D, int EL, int MODE>
 __global__ void __launch_bounds__(384, 1)
@@ -58,7 +59,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   using namespace sm100;
   using SM = TileSmem<D>;
   constexpr bool TWO_PASS = MODE == TILE_CAP;   // how the softmax warps go over a block
-  constexpr bool CAP = MODE == TILE_CAP || MODE == TILE_ANY, SLOPES = MODE == TILE_ANY, DOCUMENTS = MODE == TILE_DOCUMENTS || MODE == TILE_ANY;
+  constexpr bool CAP = MODE == TILE_CAP || MODE == TILE_ANY, SLOPES = MODE == TILE_ANY, DOCUMENTS = MODE != TILE_PLAIN;
   constexpr int DC = D / 64;
   constexpr uint32_t TMEM_COLS = 512;          // S0 [0,128), S1 [128,256), O0 [256, 256 + D), O1 [256 + D, 256 + 2 D)
 
@@ -376,7 +377,8 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if constexpr (TWO_PASS) {
           // Capped scores: the cap is monotonic, so a first pass finds the row's maximum among the products, a second caps, weighs and
           // stores 32 columns at a time, a loop of a few registers and little code.  The score buffer is handed back late, which
-          // this much arithmetic hides.  (With all 128 scores in registers, as below: 263 us where this takes 2xx.)
+          // this much arithmetic hides.  (With all 128 scores in registers, as below, 235 us
+          // where this takes 220; with two warps for every 32 queries, a half of the keys each, 282.)
           uint32_t seen[4];
           float hi = -INFINITY, lo = INFINITY;
           if (need_mask) {
@@ -478,32 +480,44 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (lane == 0) mbar_arrive(bar_se);
         sc++;
         if (CAP && p.cap.cap > 0.f) {
-          const float largest = max3(max3(ha_largest(r[0]), ha_largest(r[1]), 0.f), ha_largest(r[2]), ha_largest(r[3]));
-          if (__all_sync(0xffffffffu, largest <= p.cap.small)) {
 #pragma unroll
-            for (int c = 0; c < 4; c++)
+          for (int c = 0; c < 4; c++)
 #pragma unroll
-              for (int i = 0; i < 16; i++)
-                unpack2(cap_small(p.cap, mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), r[c][2 * i], r[c][2 * i + 1]);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 4; c++)
-#pragma unroll
-              for (int i = 0; i < 16; i++)
-                unpack2(fma2(cap_rest(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), p.cap.twice2, p.cap.out2), r[c][2 * i], r[c][2 * i + 1]);
-          }
-        } else if (MODE == TILE_ANY && p.scaled) {
+            for (int i = 0; i < 16; i++)
+              unpack2(fma2(cap_rest(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), p.cap.twice2, p.cap.out2), r[c][2 * i], r[c][2 * i + 1]);
+        } else if (MODE == TILE_ANY && !p.a.slopes) {
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.in2), r[c][2 * i], r[c][2 * i + 1]);
         }
         if (SLOPES && p.a.slopes) {
-          const float far = (float)(pos - j * HA_BLOCK);
+          const int far = pos - j * HA_BLOCK;
+          const uint64_t m2 = p.cap.cap > 0.f ? splat2(1.f) : p.in2;
+          const bool before = __all_sync(0xffffffffu, far >= HA_BLOCK - 1), behind = __all_sync(0xffffffffu, far <= 0);
+          if (before || behind) {
+            // all keys on one side of all the warp's queries: the bias grows by the slope from key to key, anew every 32 of them
+            const float grow = before ? slope : -slope;
+            const uint64_t step2 = splat2(2.f * grow);
 #pragma unroll
-          for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 4; c++) {
+              const float first = (float)(c * 32 - far) * grow;
+              uint64_t bias2 = pack2(__float_as_uint(first), __float_as_uint(first + grow));
 #pragma unroll
-            for (int i = 0; i < 32; i++) r[c][i] = __float_as_uint(fmaf(fabsf(far - (float)(c * 32 + i)), -slope, __uint_as_float(r[c][i])));
+              for (int i = 0; i < 16; i++) {
+                unpack2(fma2(pack2(r[c][2 * i], r[c][2 * i + 1]), m2, bias2), r[c][2 * i], r[c][2 * i + 1]);
+                bias2 = add2(bias2, step2);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 16; i++) {
+                const float d0 = -slope * fabsf((float)(far - c * 32 - 2 * i)), d1 = -slope * fabsf((float)(far - c * 32 - 2 * i - 1));
+                unpack2(fma2(pack2(r[c][2 * i], r[c][2 * i + 1]), m2, pack2(__float_as_uint(d0), __float_as_uint(d1))), r[c][2 * i], r[c][2 * i + 1]);
+              }
+          }
         }
         if (need_mask) {
 #pragma unroll
@@ -653,7 +667,7 @@ int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& 
 template <int D, int EL>
 int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const TileParams& p, int32_t* sched, int32_t* status, cudaStream_t stream) {
   const bool cap = p.cap.cap > 0.f;
-  if (p.a.slopes || !(p.a.scale > 0.f) || (cap && p.a.documents)) return launch_tiles<D, EL, TILE_ANY>(q, k, v, p, sched, status, stream);
+  if (p.a.slopes || !(p.a.scale > 0.f)) return launch_tiles<D, EL, TILE_ANY>(q, k, v, p, sched, status, stream);
   if (cap) return launch_tiles<D, EL, TILE_CAP>(q, k, v, p, sched, status, stream);
   if (p.a.documents) return launch_tiles<D, EL, TILE_DOCUMENTS>(q, k, v, p, sched, status, stream);
   return launch_tiles<D, EL, TILE_PLAIN>(q, k, v, p, sched, status, stream);
