@@ -124,13 +124,10 @@ __device__ __forceinline__ void grad_write(uint32_t taddr, char* row, bool there
 #pragma unroll
     for (int i = 0; i < 16; i++) x[i] = 0;
   }
+  uint32_t wd[8];
 #pragma unroll
-  for (int q = 0; q < 2; q++) {
-    uint32_t wd[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) wd[k] = ha_pack<EL>(__uint_as_float(x[q * 8 + 2 * k]) * f, __uint_as_float(x[q * 8 + 2 * k + 1]) * f);
-    if (there && q * 8 < width) *reinterpret_cast<uint4*>(row + 2 * (q * 8)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
-  }
+  for (int k = 0; k < 8; k++) wd[k] = ha_pack<EL>(__uint_as_float(x[2 * k]) * f, __uint_as_float(x[2 * k + 1]) * f);
+  if (there) ha_store_row(row, width, wd);
 }
 
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------

@@ -594,17 +594,11 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int i = 0; i < 16; i++) x[i] = 0;
         }
         if (qrow < p.a.Sq) {
+          uint32_t wd[8];
+          // a row that sees nothing is 0, whatever weights of zero were multiplied with
 #pragma unroll
-          for (int q = 0; q < 2; q++) {
-            uint32_t wd[4];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-              // a row that sees nothing is 0, whatever weights of zero were multiplied with
-              const float f0 = inv == 0.f ? 0.f : __uint_as_float(x[q * 8 + 2 * k]) * inv, f1 = inv == 0.f ? 0.f : __uint_as_float(x[q * 8 + 2 * k + 1]) * inv;
-              wd[k] = ha_pack<EL>(f0, f1);
-            }
-            if (c * 16 + q * 8 < p.a.D) *reinterpret_cast<uint4*>(orow + 2 * (c * 16 + q * 8)) = make_uint4(wd[0], wd[1], wd[2], wd[3]);
-          }
+          for (int k = 0; k < 8; k++) wd[k] = inv == 0.f ? 0u : ha_pack<EL>(__uint_as_float(x[2 * k]) * inv, __uint_as_float(x[2 * k + 1]) * inv);
+          ha_store_row(orow + 2 * (c * 16), p.a.D - c * 16, wd);
         }
       }
       if (p.a.lse && qrow < p.a.Sq)

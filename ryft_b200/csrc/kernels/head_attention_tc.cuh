@@ -152,6 +152,19 @@ __device__ __forceinline__ float ha_largest(const uint32_t (&r)[32]) {
   return max3(m[0], m[1], 0.f);
 }
 
+// Sixteen 16-bit values of a row, `width` of which exist: 32 bytes at once where the row lies on that boundary (a sector in one
+// access, half as many of them), else 16 bytes at a time.
+__device__ __forceinline__ void ha_store_row(char* row, int width, const uint32_t (&w)[8]) {
+  if (width >= 16 && ((uintptr_t)row & 31) == 0) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(__cvta_generic_to_global(row)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+    return;
+  }
+  if (width > 0) *reinterpret_cast<uint4*>(row) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (width > 8) *reinterpret_cast<uint4*>(row + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+}
+
 // sm100::mbar_wait with the thread asleep in between: most of a CTA's warps wait most of the time here, and what they poll with
 // is taken from the warps that compute.
 __device__ __forceinline__ bool ha_try_wait(uint32_t bar, uint32_t parity) {
