@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include "../../../include/b2x_kernels.h"
+#include "attention_math.cuh"
 #include "common.cuh"
 
 namespace b2x {
@@ -83,6 +84,51 @@ template <int EL, int V> __device__ __forceinline__ void rot_store(char* p, cons
     *(uint2*)p = make_uint2(rot_pack<EL>(v[0], v[1]), rot_pack<EL>(v[2], v[3]));
   } else {
     *(uint16_t*)p = (uint16_t)(rot_pack<EL>(v[0], 0.f) & 0xffffu);
+  }
+}
+
+// Two adjacent elements of V at a time where there are two: the kernels are bound by the instructions that they issue as much as by HBM.
+__device__ __forceinline__ uint64_t rot_two(const float* v) { return pack2(__float_as_uint(v[0]), __float_as_uint(v[1])); }
+__device__ __forceinline__ void rot_put(float* v, uint64_t x) {
+  uint32_t a, b;
+  unpack2(x, a, b);
+  v[0] = __uint_as_float(a); v[1] = __uint_as_float(b);
+}
+__device__ __forceinline__ uint64_t rot_mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t rot_neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+// o = a * b, o = a * f, o = a * b + c
+template <int V> __device__ __forceinline__ void rot_mul(float (&o)[V], const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) o[0] = a[0] * b[0];
+  else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) rot_put(o + j, rot_mul2(rot_two(a + j), rot_two(b + j)));
+  }
+}
+template <int V> __device__ __forceinline__ void rot_scale(float (&o)[V], const float (&a)[V], float f) {
+  if constexpr (V == 1) o[0] = a[0] * f;
+  else {
+    const uint64_t f2 = splat2(f);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) rot_put(o + j, rot_mul2(rot_two(a + j), f2));
+  }
+}
+template <int V> __device__ __forceinline__ void rot_fma(float (&o)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V == 1) o[0] = fmaf(a[0], b[0], c[0]);
+  else {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) rot_put(o + j, fma2(rot_two(a + j), rot_two(b + j), rot_two(c + j)));
+  }
+}
+template <int V> __device__ __forceinline__ void rot_fma(float (&o)[V], const float (&a)[V], float f, const float (&c)[V]) {
+  if constexpr (V == 1) o[0] = fmaf(a[0], f, c[0]);
+  else {
+    const uint64_t f2 = splat2(f);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) rot_put(o + j, fma2(rot_two(a + j), f2, rot_two(c + j)));
   }
 }
 
@@ -194,7 +240,7 @@ template <int EL, int V, int NU> struct RotLane {
       for (int s = 0; s < 2; s++)
         if (e[u][s] >= 0) rot_store<EL, V>(row + (int64_t)e[u][s] * ES, v[u][s]);
   }
-  // w (of the elements) times cos and sin: x turns to f (x[a] ca - x[b] sb), ...
+  // w (of the elements) times cos and sin: the pair (a, b) turns to f (a ca + b sb), f (b cb + a sa)
   __device__ __forceinline__ void fold(const RotaryParams& p, const float2* table) {
 #pragma unroll
     for (int u = 0; u < NU; u++)
@@ -203,24 +249,22 @@ template <int EL, int V, int NU> struct RotLane {
         const float2 t = k < turns[u] ? table[(p.interleaved ? e[u][0] / 2 : e[u][0]) + k] : make_float2(1.f, 0.f);
         const bool across = V == 1 || !p.interleaved;
         const float wa = across ? w[u][0][k] : w[u][k / ((V + 1) / 2)][(2 * k) % V], wb = across ? w[u][1][k] : w[u][k / ((V + 1) / 2)][(2 * k + 1) % V];
-        ca[u][k] = t.x * wa; sa[u][k] = t.y * wa; cb[u][k] = t.x * wb; sb[u][k] = t.y * wb;
+        ca[u][k] = t.x * wa; sa[u][k] = t.y * wa; cb[u][k] = t.x * wb; sb[u][k] = -t.y * wb;
       }
   }
   __device__ __forceinline__ void turn_weighted(const RotaryParams& p, float (&v)[NU][2][V], float f) const {
 #pragma unroll
     for (int u = 0; u < NU; u++) {
       if (V == 1 || !p.interleaved) {
-        // pieces turn as a whole or pass as a whole
+        // pieces turn as a whole or pass as a whole; sb carries its sign
+        float a[V], b[V];
+        rot_scale<V>(a, v[u][0], f);
+        rot_scale<V>(b, v[u][1], f);
+        rot_mul<V>(v[u][0], a, ca[u]);
+        rot_mul<V>(v[u][1], b, cb[u]);
         if (turns[u] > 0) {
-#pragma unroll
-          for (int k = 0; k < V; k++) {
-            const float a = v[u][0][k] * f, b = v[u][1][k] * f;
-            v[u][0][k] = fmaf(-b, sb[u][k], a * ca[u][k]);
-            v[u][1][k] = fmaf(a, sa[u][k], b * cb[u][k]);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; k++) { v[u][0][k] *= f * ca[u][k]; v[u][1][k] *= f * cb[u][k]; }
+          rot_fma<V>(v[u][0], b, sb[u], v[u][0]);
+          rot_fma<V>(v[u][1], a, sa[u], v[u][1]);
         }
       } else if constexpr (V > 1) {
 #pragma unroll
@@ -228,7 +272,7 @@ template <int EL, int V, int NU> struct RotLane {
           float &px = v[u][k / (V / 2)][2 * (k % (V / 2))], &py = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
           const float a = px * f, b = py * f;
           float x = a * ca[u][k], y = b * cb[u][k];
-          if (k < turns[u]) { x = fmaf(-b, sb[u][k], x); y = fmaf(a, sa[u][k], y); }
+          if (k < turns[u]) { x = fmaf(b, sb[u][k], x); y = fmaf(a, sa[u][k], y); }
           px = x; py = y;
         }
       }
@@ -240,12 +284,16 @@ template <int EL, int V, int NU> struct RotLane {
     for (int u = 0; u < NU; u++) {
       if (V == 1 || !p.interleaved) {
         if (turns[u] > 0) {
+          float a[V], b[V];
+          rot_mul<V>(a, v[u][1], sn[u]);
+          rot_mul<V>(b, v[u][0], sn[u]);
+          if constexpr (V == 1) a[0] = -a[0];
+          else {
 #pragma unroll
-          for (int j = 0; j < V; j++) {
-            const float a = v[u][0][j], b = v[u][1][j];
-            v[u][0][j] = a * cs[u][j] - b * sn[u][j];
-            v[u][1][j] = b * cs[u][j] + a * sn[u][j];
+            for (int j = 0; j < V; j += 2) rot_put(a + j, rot_neg2(rot_two(a + j)));
           }
+          rot_fma<V>(v[u][0], v[u][0], cs[u], a);
+          rot_fma<V>(v[u][1], v[u][1], cs[u], b);
         }
       } else if constexpr (V > 1) {
 #pragma unroll
@@ -258,12 +306,23 @@ template <int EL, int V, int NU> struct RotLane {
     }
   }
   static __device__ __forceinline__ float dot(const float (&a)[NU][2][V], const float (&b)[NU][2][V], int lanes) {
-    float s[2] = {0.f, 0.f};
+    float s[2][V];
 #pragma unroll
-    for (int u = 0; u < NU; u++)
+    for (int k = 0; k < 2; k++) {
+      rot_mul<V>(s[k], a[0][k], b[0][k]);
 #pragma unroll
-      for (int j = 0; j < V; j++) { s[0] = fmaf(a[u][0][j], b[u][0][j], s[0]); s[1] = fmaf(a[u][1][j], b[u][1][j], s[1]); }
-    float t = s[0] + s[1];
+      for (int u = 1; u < NU; u++) rot_fma<V>(s[k], a[u][k], b[u][k], s[k]);
+    }
+    float t = 0.f;
+    if constexpr (V == 1) t = s[0][0] + s[1][0];
+    else {
+      uint64_t q = add2(rot_two(s[0]), rot_two(s[1]));
+#pragma unroll
+      for (int j = 2; j < V; j += 2) q = add2(q, add2(rot_two(s[0] + j), rot_two(s[1] + j)));
+      uint32_t x, y;
+      unpack2(q, x, y);
+      t = __uint_as_float(x) + __uint_as_float(y);
+    }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) if (off < lanes) t += __shfl_xor_sync(0xffffffffu, t, off);
     return t;
@@ -332,7 +391,8 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ti = blockIdx.y;
   const int slots = 32 / p.lanes, slot = lane / p.lanes;
-  RotLane<EL, V, NU> me;
+  using Lane = RotLane<EL, V, NU>;
+  Lane me;
   me.pieces(p, lane & (p.lanes - 1));
   me.weights(p, ti);
   float dw[NU][2][V];
@@ -364,24 +424,23 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
       me.load(in + next * in_head, next < last, rx);
       me.load(din + next * din_head, next < last, rg);
       me.turn(p, g);
-      const float f = rsqrtf(me.dot(x, x, p.lanes) * p.inv_d + p.epsilon);
+      const float f = rsqrtf(Lane::dot(x, x, p.lanes) * p.inv_d + p.epsilon);
 #pragma unroll
       for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-          for (int j = 0; j < V; j++) {
-            x[u][s][j] *= f;
-            if (h < last) dw[u][s][j] = fmaf(g[u][s][j], x[u][s][j], dw[u][s][j]);
-            g[u][s][j] *= me.w[u][s][j];
-          }
-      const float m = me.dot(x, g, p.lanes) * p.inv_d;
+        for (int s = 0; s < 2; s++) {
+          rot_scale<V>(x[u][s], x[u][s], f);
+          if (h < last) rot_fma<V>(dw[u][s], g[u][s], x[u][s], dw[u][s]);
+          rot_mul<V>(g[u][s], g[u][s], me.w[u][s]);
+        }
+      const float m = Lane::dot(x, g, p.lanes) * p.inv_d;
 #pragma unroll
       for (int u = 0; u < NU; u++)
 #pragma unroll
-        for (int s = 0; s < 2; s++)
-#pragma unroll
-          for (int j = 0; j < V; j++) g[u][s][j] = f * (g[u][s][j] - x[u][s][j] * m);
+        for (int s = 0; s < 2; s++) {
+          rot_fma<V>(g[u][s], x[u][s], -m, g[u][s]);
+          rot_scale<V>(g[u][s], g[u][s], f);
+        }
       if (h < last) me.store(out + h * out_head, g);
     }
   }
