@@ -158,6 +158,27 @@ def test_captured_graphs_replayed_side_by_side(lib, Sq, softcap):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("S", [66_000, 132_000])
+def test_documents_of_more_tokens_than_lists_cover(lib, S):
+    """A row of documents of 500 tokens, each against the same document alone; behind 65536 (gradient) and 131072 (forward) tokens blocks
+    are no longer listed but compared one by one."""
+    D, n = 64, S // 500
+    q, k, v, do = make(5, 1, 1, 1, S, S, D)
+    documents = (torch.arange(S, device="cuda", dtype=torch.int32) // 500)[None].contiguous()
+    o, lse = torch.empty_like(q), torch.empty(1, 1, S, device="cuda")
+    grads = (do, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+    for gradient in (False, True):
+        rc, status = launch(lib, attention_args(lib, q, k, v, o, lse, grads if gradient else None, causal=1, documents=documents), gradient)
+        torch.cuda.synchronize()
+        assert rc == 0 and not status.item()
+    alone = lambda t: t.cpu().reshape(n, 500, 1, D)  # noqa: E731
+    pick = [0, 1, n // 2, n - 2, n - 1]
+    want = ref.attention(*[alone(t)[pick] for t in (q, k, v)], "bf16", "bshd", D ** -0.5, do=alone(do)[pick], causal=True)
+    for name, t in (("o", o), ("dq", grads[1]), ("dk", grads[2]), ("dv", grads[3])):
+        close(alone(t)[pick], *want[name], name)
+    close(lse.cpu().reshape(n, 1, 500)[pick], *want["lse"], "lse")
+
+
 def test_what_cannot_be_addressed_is_refused(lib):
     q, k, v, do = make(3, 1, 2, 2, 40, 40, 64)
     o, lse = torch.zeros_like(q), torch.zeros(1, 2, 40, device="cuda")

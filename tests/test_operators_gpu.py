@@ -207,12 +207,41 @@ ATTENTION = [
     (dict(B=1, Sq=17, Sk=64, Hq=4, Hk=4, D=8, dtype="bf16", layout="bhsd"), dict(scale=0.5)),
     (dict(B=2, Sq=5, Sk=200, Hq=3, Hk=1, D=120, dtype="f16", layout="bshd"), dict(lengths=[3, 200], queries_at_end=True)),
     (dict(B=1, Sq=640, Sk=640, Hq=12, Hk=4, D=128, dtype="bf16", layout="bshd"), dict(causal=True)),
+    (dict(B=1, Sq=1, Sk=37, Hq=40, Hk=1, D=8, dtype="bf16", layout="bhsd"), dict()),                                # rows of a key head over three tiles
+    (dict(B=2, Sq=16, Sk=130, Hq=6, Hk=2, D=24, dtype="f16", layout="bshd"), dict(causal=True, query_offset=114, softcap=10.0, slopes=True)),
+    (dict(B=3, Sq=40, Sk=300, Hq=2, Hk=1, D=64, dtype="bf16", layout="bhsd"), dict(causal=True, queries_at_end=True, lengths=[300, 20, 171], documents=4)),
+    (dict(B=3, Sq=150, Sk=150, Hq=2, Hk=2, D=64, dtype="bf16", layout="bshd"), dict(causal=True, lengths=[-5, 10 ** 6, 150], prefix=[-7, 10 ** 6, 3])),
+    (dict(B=3, Sq=2, Sk=150, Hq=2, Hk=2, D=64, dtype="bf16", layout="bshd"), dict(lengths=[-5, 10 ** 6, 150], queries_at_end=True, causal=True)),
+    (dict(B=1, Sq=200, Sk=200, Hq=2, Hk=1, D=128, dtype="bf16", layout="bhsd"), dict(documents=3, causal=True, softcap=25.0)),
+    (dict(B=1, Sq=140, Sk=140, Hq=2, Hk=1, D=64, dtype="bf16", layout="bhsd"), dict(scale=-0.2, causal=True)),
+    (dict(B=1, Sq=140, Sk=140, Hq=2, Hk=1, D=64, dtype="f16", layout="bhsd"), dict(scale=-0.2, softcap=5.0)),
+    (dict(B=1, Sq=130, Sk=60, Hq=1, Hk=1, D=64, dtype="bf16", layout="bhsd"), dict(scale=0.0)),
+    (dict(B=1, Sq=150, Sk=260, Hq=2, Hk=2, D=64, dtype="bf16", layout="bhsd"), dict(scale=3.0, softcap=30.0, causal=True, query_offset=110)),   # scores far beyond the cap
 ]
 
 
 @pytest.mark.parametrize("sizes,options", ATTENTION, ids=str)
 def test_attention_and_its_gradient(client, sizes, options):
     attention_check(client, **sizes, **options)
+
+
+def test_a_token_against_a_very_long_cache(client):
+    attention_check(client, 1, 1, 200_001, 2, 1, 64, "bf16", "bhsd", gradient=False, causal=True, query_offset=200_000, softcap=30.0)
+
+
+def test_operands_that_the_program_holds_itself(client):
+    """Lengths, slopes and documents as constants and as results of other ops."""
+    B, S, D = 2, 140, 64
+    q, k, v, do, _, _ = attention_case(B, S, S, 2, 2, D, "bf16", "bhsd", 3)
+    b = Builder()
+    args = [b.arg([B, 2, S, D], "bf16") for _ in range(3)]
+    position = b.iota(1, [B, S], "i32")
+    documents = b._emit(position.type, f"stablehlo.divide {position}, {b.constant(50, [B, S], 'i32')} : {position.type}")
+    o = b.attention(*args, causal=True, lengths=b.constant(100, [B], "i32"), slopes=b.constant_array([0.5, 0.25], "f32"), documents=documents)
+    got = run(client, b.build(o), [q, k, v])[0]
+    want = ref.attention(q, k, v, "bf16", "bhsd", D ** -0.5, slopes=torch.tensor([0.5, 0.25]), causal=True, lengths=torch.tensor([100, 100]),
+                         documents=(torch.arange(S) // 50).expand(B, S).contiguous())
+    within(got, *want["o"], "o")
 
 
 def test_attention_of_nothing(client):
