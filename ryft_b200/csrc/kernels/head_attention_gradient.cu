@@ -303,23 +303,18 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     // ---------------------------------------------- MMA issuer ------------------------------------------------------
     if (elect_one()) {
       uint32_t sc = 0, uc = 0, nt = 0;     // units whose scores are issued, units added to the accumulators, tiles with work
-      const uint32_t ta = sbase + SM::T0_OFF, tb = sbase + SM::T1_OFF;
+      const uint32_t dta = ha_desc(sbase + SM::T0_OFF, 16), dtb = ha_desc(sbase + SM::T1_OFF, 16);
       bool ok = true;
       auto issue_scores = [&](bool last_of_tile) -> bool {
         const uint32_t st = sc % STAGES, g = sc % GROUPS;
         const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES, ub = ua + SM::U_BYTES;
         if (!ha_barrier(bar_uf + 8 * st, (sc / STAGES) & 1, abort_flag, status, 71)) return false;
         tc_fence_after();
+        const uint32_t da = ha_desc(ua, 16), db = ha_desc(ub, 16), to = tmem_base + g * 128u;
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t in = (uint32_t)(k & 3) * 32, c = (uint32_t)(k >> 2);
-          umma_ss<false>(tmem_base + g * 128u, make_smem_desc(ta + c * HA_CHUNK + in, 16, 1024), make_smem_desc(ua + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < D / 16; k++) ha_mma(to, dta + ((k >> 2) * HA_CHUNK + (k & 3) * 32) / 16, da + ((k >> 2) * U_CHUNK + (k & 3) * 32) / 16, p.idesc_s, k > 0);
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t in = (uint32_t)(k & 3) * 32, c = (uint32_t)(k >> 2);
-          umma_ss<false>(tmem_base + g * 128u + 64u, make_smem_desc(tb + c * HA_CHUNK + in, 16, 1024), make_smem_desc(ub + c * U_CHUNK + in, 16, 1024), p.idesc_s, k > 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < D / 16; k++) ha_mma(to + 64u, dtb + ((k >> 2) * HA_CHUNK + (k & 3) * 32) / 16, db + ((k >> 2) * U_CHUNK + (k & 3) * 32) / 16, p.idesc_s, k > 0);
         tc_commit(bar_sf + 8 * g);
         if (last_of_tile) tc_commit(bar_tu);
         sc++;
@@ -341,15 +336,13 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
           if (it == 0 && nt > 0 && !ha_barrier(bar_of, (nt - 1) & 1, abort_flag, status, 75)) { ok = false; break; }
           tc_fence_after();
           // A = P or dS from TMEM: 16 of the unit are 8 columns; B = the unit's rows (MN-major: chunks of 64 of the width are U_CHUNK apart)
+          const uint32_t da = ha_desc(ua, U_CHUNK), db = ha_desc(ub, U_CHUNK), from = tmem_base + g * 128u;
           if constexpr (KEYS) {
 #pragma unroll
-            for (int k = 0; k < GRAD_UNIT / 16; k++)
-              umma_ts_f16(tmem_base + ACC, tmem_base + g * 128u + (uint32_t)(k * 8), make_smem_desc(ub + (uint32_t)k * 2048, U_CHUNK, 1024), p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < GRAD_UNIT / 16; k++) ha_mma_ts(tmem_base + ACC, from + (uint32_t)(k * 8), db + k * 128, p.idesc_acc, it > 0 || k > 0);
           }
 #pragma unroll
-          for (int k = 0; k < GRAD_UNIT / 16; k++)
-            umma_ts_f16(tmem_base + ACC + (KEYS ? (uint32_t)D : 0u), tmem_base + g * 128u + 64u + (uint32_t)(k * 8), make_smem_desc(ua + (uint32_t)k * 2048, U_CHUNK, 1024),
-                        p.idesc_acc, (it > 0 || k > 0) ? 1u : 0u);
+          for (int k = 0; k < GRAD_UNIT / 16; k++) ha_mma_ts(tmem_base + ACC + (KEYS ? (uint32_t)D : 0u), from + 64u + (uint32_t)(k * 8), da + k * 128, p.idesc_acc, it > 0 || k > 0);
           tc_commit(bar_ue + 8 * st);
           if (it + 1 == total) tc_commit(bar_end);
           uc++;

@@ -212,7 +212,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (elect_one()) {
       uint32_t kc = 0, vc = 0, hc = 0, nq = 0;     // score blocks issued, V blocks consumed, P V half-steps issued, tiles with work
       const uint32_t s_tmem = tmem_base + (uint32_t)(w * 128), o_tmem = tmem_base + 256u + (uint32_t)(w * D);
-      const uint32_t qa = wbase + SM::Q_OFF, ka = wbase + SM::K_OFF, va = wbase + SM::V_OFF, pa = wbase + SM::P_OFF;
+      const uint32_t dq = ha_desc(wbase + SM::Q_OFF, 16), dk = ha_desc(wbase + SM::K_OFF, 16), dv = ha_desc(wbase + SM::V_OFF, HA_CHUNK), dp = ha_desc(wbase + SM::P_OFF, 16);
       bool ok = true;
       auto issue_qk = [&](bool last_of_tile) -> bool {
         if (!ha_barrier(bar_kf, kc & 1, abort_flag, status, 13)) return false;
@@ -220,10 +220,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (kc > 0 && !ha_barrier(bar_se, (kc - 1) & 1, abort_flag, status, 14)) return false;
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < D / 16; k++) {
-          const uint32_t off = (uint32_t)(k >> 2) * HA_CHUNK + (uint32_t)(k & 3) * 32;
-          umma_ss<false>(s_tmem, make_smem_desc(qa + off, 16, 1024), make_smem_desc(ka + off, 16, 1024), p.idesc_qk, k > 0 ? 1u : 0u);
-        }
+        for (int k = 0; k < D / 16; k++) ha_mma(s_tmem, dq + ((k >> 2) * HA_CHUNK + (k & 3) * 32) / 16, dk + ((k >> 2) * HA_CHUNK + (k & 3) * 32) / 16, p.idesc_qk, k > 0);
         tc_commit(bar_sf);
         tc_commit(bar_ke);
         if (last_of_tile) tc_commit(bar_qe);
@@ -249,13 +246,9 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int h = 0; h < 2; h++) {
             if (!ha_barrier(bar_pf, hc & 1, abort_flag, status, 16)) { ok = false; break; }
             tc_fence_after();
+            // A = P (K-major: 64 keys contiguous per row); B = V (MN-major: head-dim chunks of 64 are HA_CHUNK apart)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-              // A = P (K-major: 64 keys contiguous per row); B = V (MN-major: head-dim chunks of 64 are HA_CHUNK apart)
-              const int kk = 4 * h + k;
-              umma_ss<false>(o_tmem, make_smem_desc(pa + (uint32_t)k * 32, 16, 1024), make_smem_desc(va + (uint32_t)kk * 2048, HA_CHUNK, 1024), p.idesc_pv,
-                             (it > 0 || kk > 0) ? 1u : 0u);
-            }
+            for (int k = 0; k < 4; k++) ha_mma(o_tmem, dp + k * 2, dv + (4 * h + k) * 128, p.idesc_pv, it > 0 || h > 0 || k > 0);
             tc_commit(bar_pv);     // the half's weights have been read; the accumulator holds them
             hc++;
             if (h == 0 && TWO_PASS && it + 1 < blocks && !issue_qk(it + 2 == blocks)) { ok = false; break; }
