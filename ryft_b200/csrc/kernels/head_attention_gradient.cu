@@ -6,8 +6,9 @@
 // of dQ is written and read.
 //
 // Both are one kernel, k_attention_gradient: a tile of 128 rows (queries with their dO; or keys with their values) stays in shared
-// memory, units of 64 of the other side pass by in four stages.  Two products per unit, S and dP (transposed for keys), go into one
-// of two pairs of TMEM buffers of 64 columns, so that four warps turn one pair into P and dS while the tensor pipe works for the other.
+// memory, units of 64 of the other side pass by in five stages (eight at a width of 64).  Two products per unit, S and dP (transposed
+// for keys), go into one of two or three pairs of TMEM buffers of 64 columns, so that four warps turn one pair into P and dS while the
+// tensor pipe works for the others.
 // P and dS are written in place as 16-bit words (a row's words take columns that it has read) and are the left operands of the
 // second products, dQ += dS K, or dV += P^T dO and dK += dS^T Q: they never pass through shared memory, whose bandwidth bounds
 // the products.  Accumulators and buffers fill TMEM at a width of 128.  Query heads that share a key head follow one another into the
@@ -15,9 +16,16 @@
 //
 // The arithmetic of a unit is a loop over 16 columns whose body is one of nine forms (cap, bias, mask), chosen once per unit: with
 // the four steps unrolled, or with the forms' branches inside, the warps waited for instructions more than for anything else
-// (ncu, training_capped's dK and dV: 505 us with branches inside, 416 unrolled, 336 as a loop).
+// (dK and dV of 2 x 16/4 heads, 4096 x 128, causal, capped: 505 us with branches inside, 416 unrolled, 336 as a loop).
 //
-// 384 threads: warp 0 draws tiles and loads (TMA), warp 1 issues the MMAs, warps 4-11 do the arithmetic.
+// What bounds it: a product of 128 x 64 x 16 takes the tensor pipe 48 cycles where both operands come from shared memory (32 would be
+// its arithmetic; the rows of the tile are read again for every unit), so a unit cannot take less than 1003 cycles for dQ and
+// 1259 for dK and dV.  At that size dQ takes 201 us, about 30 % above its products, and dK and dV 273 us, 50 % above: with two
+// pairs a unit's arithmetic is on the way from its scores to its sums.  Capped they take 242 and 313 us: the cap's polynomial and its
+// derivative double the instructions for the FMA pipe.  Both kernels and the row constants: 470 us, 731 TFLOP/s of the gradient's
+// five products; capped 548 us.
+//
+// 384 threads, 512 with three pairs: warp 0 draws tiles and loads (TMA), warp 1 issues the MMAs, warps 4 and up do the arithmetic.
 #include <atomic>
 #include <type_traits>
 
@@ -539,23 +547,31 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
   if (sched && threadIdx.x == 0 && atomicAdd(sched + 1, 1) == (int)gridDim.x - 1) { sched[0] = 0; sched[1] = 0; __threadfence(); }
 }
 
-// ---- row constants: -log sum in log2 units and -delta, two rows per warp; rows behind the last query weigh nothing --------------
+// ---- row constants: -log sum in log2 units and -delta; rows behind the last query weigh nothing ---------------------------------
+// 32 rows of a head per block (`rows` is a multiple of 128), two per half warp, so that a thread has four loads of 16 bytes in flight;
+// a sequence's heads follow one another, for where tokens come before heads their rows are neighbours in memory.  2 x 16 heads of
+// 4096 rows of 128, 67 MB: 16 us with nothing in L2 (18 with one row per half warp, head by head).
 template <int EL>
 __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ HeadAttn p, float* neg_lse, float* neg_delta, int32_t rows) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, part = lane & 15;
-  const int64_t id = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * 2 + (lane >> 4);
-  const int64_t all = (int64_t)p.B * p.Hq * rows;
-  const int i = (int)(id % rows);
-  const int64_t bh = id / rows;
-  const int h = (int)(bh % p.Hq), b = (int)(bh / p.Hq);
-  float d = 0.f;
-  const bool there = id < all && i < p.Sq;
-  if (there && part * 8 < p.D) {
-    const uint4 x = ld_global((const uint4*)(p.o + 2 * ((int64_t)b * p.os.batch + (int64_t)h * p.os.head + (int64_t)i * p.os.token)) + part);
-    const uint4 y = ld_global((const uint4*)(p.dout + 2 * ((int64_t)b * p.dos.batch + (int64_t)h * p.dos.head + (int64_t)i * p.dos.token)) + part);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+  const uint32_t per_head = (uint32_t)rows / 32u, at = blockIdx.x / (uint32_t)p.Hq;
+  const int h = (int)(blockIdx.x - at * (uint32_t)p.Hq), b = (int)(at / per_head), bh = b * p.Hq + h;
+  const int first = (int)(at - (uint32_t)b * per_head) * 32 + ((int)(threadIdx.x >> 5) * 2 + (lane >> 4)) * 2;
+  uint4 x[2], y[2];
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    x[r] = y[r] = make_uint4(0, 0, 0, 0);
+    if (first + r < p.Sq && part * 8 < p.D) {
+      x[r] = ld_global((const uint4*)(p.o + 2 * ((int64_t)b * p.os.batch + (int64_t)h * p.os.head + (int64_t)(first + r) * p.os.token)) + part);
+      y[r] = ld_global((const uint4*)(p.dout + 2 * ((int64_t)b * p.dos.batch + (int64_t)h * p.dos.head + (int64_t)(first + r) * p.dos.token)) + part);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; r++) {
+    const uint32_t xs[4] = {x[r].x, x[r].y, x[r].z, x[r].w}, ys[4] = {y[r].x, y[r].y, y[r].z, y[r].w};
+    float d = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       float2 u, v;
@@ -564,14 +580,16 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
       d = fmaf(u.x, v.x, d);
       d = fmaf(u.y, v.y, d);
     }
-  }
 #pragma unroll
-  for (int off = 8; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
-  if (id < all && part == 0) {
-    // a query that saw nothing has a log sum of -inf: its weights are 0
-    const float l = there ? ld_global(p.lse + bh * p.Sq + i) : -INFINITY;
-    neg_lse[id] = l == -INFINITY ? -INFINITY : -l * kLog2e;
-    neg_delta[id] = there ? -d : 0.f;
+    for (int off = 8; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+    if (part == 0) {
+      // a query that saw nothing has a log sum of -inf: its weights are 0
+      const bool there = first + r < p.Sq;
+      const int64_t id = (int64_t)bh * rows + first + r;
+      const float l = there ? ld_global(p.lse + (int64_t)bh * p.Sq + first + r) : -INFINITY;
+      neg_lse[id] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+      neg_delta[id] = there ? -d : 0.f;
+    }
   }
 }
 
@@ -645,7 +663,7 @@ int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* stat
     if (rc) return rc;
   }
   if (n > 0) {
-    const cudaError_t e = launch_overlapped(elem == EL_BF16 ? k_attention_rows<EL_BF16> : k_attention_rows<EL_F16>, dim3((unsigned)((n + 15) / 16)), dim3(256), 0, stream, a,
+    const cudaError_t e = launch_overlapped(elem == EL_BF16 ? k_attention_rows<EL_BF16> : k_attention_rows<EL_F16>, dim3((unsigned)(n / 32)), dim3(256), 0, stream, a,
                                             const_cast<float*>(p.neg_lse), const_cast<float*>(p.neg_delta), p.rows);
     if (e != cudaSuccess) return (int)e;
     count_launch();
