@@ -313,7 +313,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       // The tensor pipe's queue holds a few products, less work than a wait takes that is over already.  So the questions of the next
       // unit, is the one behind the pairs loaded and are its dS there, are asked in the middle of this one's scores, and their answers
       // are looked at after them; only a no is waited for.  With two pairs the dS are hardly ever there so early, and are not asked
-      // for.  dQ of 2 x 16/4 heads, 4096 x 128, causal: 225 -> 201 us; products alone (without waits and arithmetic) would take 160.
+      // for.  dQ of 2 x 16/4 heads, 4096 x 128, causal: 225 -> 201 us; products alone (without waits and arithmetic) would take 140.
       uint32_t stage = 0, stage_parity = 0, pair = 0;      // of the next unit whose scores are issued
       uint32_t held = 0, from_pair = 0, pair_parity = 0;   // of the next unit added to the accumulators
       uint32_t nt = 0;                                     // tiles with work
