@@ -8,8 +8,9 @@
 // (the smallest power of two that holds it with two 16-byte pieces per lane: 8 lanes for 128 elements of 16 bits), a pair's two
 // elements always in one lane, so the only exchange is the norm's sum over L lanes.  A warp keeps one token, so that the 2R
 // cosines and sines are computed once, a few per lane, shared through shared memory and then held in registers for all the
-// heads that it walks.  8192 tokens of 40 heads of 128 bf16 elements, with norms: 38 us, 4.4 TB/s (54 % of the issue slots: the norm's
-// and the turn's arithmetic in f32); the gradient of 16384 such tokens 117 us, 4.3 TB/s.
+// heads that it walks.  8192 tokens of 40 heads of 128 bf16 elements, with norms: 37 us, 4.5 TB/s (54 % of the issue slots: the norm's
+// and the turn's arithmetic in f32; without norms 33.5 us, 5.0 TB/s); the gradient of 16384 such tokens 115 us, 4.4 TB/s.  Each layout
+// of pairs is a kernel of its own: with both in one, 38 and 118 us.
 //
 // Angles: a position times a frequency in f32 is off by whole turns far into a context.  Frequencies are therefore turns per
 // position as fractions of 2^64, computed in extended precision where the program is compiled; the product with the position
@@ -41,7 +42,7 @@ struct RotaryParams {
   int32_t job_heads, lanes, units;
   int32_t pair_units;          // half layout: units whose two pieces are partners
   float epsilon, inv_d, sine;  // sine: 1, or -1 to turn back
-  uint8_t interleaved, norm, weight_f32, weight_wide;   // wide: weights start on 16 bytes
+  uint8_t norm, weight_f32, weight_wide;   // wide: weights start on 16 bytes
 };
 
 template <int EL> __device__ __forceinline__ float rot_get(const uint32_t* w, int i) {
@@ -133,8 +134,8 @@ template <int V> __device__ __forceinline__ void rot_fma(float (&o)[V], const fl
   }
 }
 
-// NU units per lane; a unit is two pieces of V elements that start at e[u][0] and e[u][1] (-1: none)
-template <int EL, int V, int NU> struct RotLane {
+// PAIRS: interleaved.  NU units per lane; a unit is two pieces of V elements that start at e[u][0] and e[u][1] (-1: none)
+template <int EL, int V, int NU, bool PAIRS> struct RotLane {
   static constexpr int ES = EL == EL_F32 ? 4 : 2;
   using Raw = RotRaw<EL, V>;
   int e[NU][2];
@@ -149,7 +150,7 @@ template <int EL, int V, int NU> struct RotLane {
       const int unit = lane + u * p.lanes;
       int a = -1, b = -1, t = 0;
       if (unit < p.units) {
-        if (p.interleaved) { a = 2 * unit * V; b = a + V; t = min(max(p.R / 2 - unit * V, 0), V); }
+        if constexpr (PAIRS) { a = 2 * unit * V; b = a + V; t = min(max(p.R / 2 - unit * V, 0), V); }
         else if (unit < p.pair_units) { a = unit * V; b = a + p.R / 2; t = V; }
         else { a = p.R + 2 * (unit - p.pair_units) * V; b = a + V; }
         if (b >= p.D) b = -1;
@@ -177,7 +178,7 @@ template <int EL, int V, int NU> struct RotLane {
 #pragma unroll
       for (int j = 0; j < V; j++) {
         // the unit's first pair: both layouts count pairs from half the first element on, or from the element itself
-        const float2 t = j < turns[u] ? table[(p.interleaved ? e[u][0] / 2 : e[u][0]) + j] : make_float2(1.f, 0.f);
+        const float2 t = j < turns[u] ? table[(PAIRS ? e[u][0] / 2 : e[u][0]) + j] : make_float2(1.f, 0.f);
         cs[u][j] = t.x; sn[u][j] = t.y;
       }
   }
@@ -247,8 +248,8 @@ template <int EL, int V, int NU> struct RotLane {
     for (int u = 0; u < NU; u++)
 #pragma unroll
       for (int k = 0; k < V; k++) {
-        const float2 t = k < turns[u] ? table[(p.interleaved ? e[u][0] / 2 : e[u][0]) + k] : make_float2(1.f, 0.f);
-        const bool across = V == 1 || !p.interleaved;
+        const float2 t = k < turns[u] ? table[(PAIRS ? e[u][0] / 2 : e[u][0]) + k] : make_float2(1.f, 0.f);
+        constexpr bool across = V == 1 || !PAIRS;
         const float wa = across ? w[u][0][k] : w[u][k / ((V + 1) / 2)][(2 * k) % V], wb = across ? w[u][1][k] : w[u][k / ((V + 1) / 2)][(2 * k + 1) % V];
         ca[u][k] = t.x * wa; sa[u][k] = t.y * wa; cb[u][k] = t.x * wb; sb[u][k] = -t.y * wb;
       }
@@ -256,7 +257,7 @@ template <int EL, int V, int NU> struct RotLane {
   __device__ __forceinline__ void turn_weighted(const RotaryParams& p, float (&v)[NU][2][V], float f) const {
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-      if (V == 1 || !p.interleaved) {
+      if constexpr (V == 1 || !PAIRS) {
         // pieces turn as a whole or pass as a whole; sb carries its sign
         float a[V], b[V];
         rot_scale<V>(a, v[u][0], f);
@@ -267,7 +268,7 @@ template <int EL, int V, int NU> struct RotLane {
           rot_fma<V>(v[u][0], b, sb[u], v[u][0]);
           rot_fma<V>(v[u][1], a, sa[u], v[u][1]);
         }
-      } else if constexpr (V > 1) {
+      } else {
 #pragma unroll
         for (int k = 0; k < V; k++) {
           float &px = v[u][k / (V / 2)][2 * (k % (V / 2))], &py = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
@@ -283,7 +284,7 @@ template <int EL, int V, int NU> struct RotLane {
   __device__ __forceinline__ void turn(const RotaryParams& p, float (&v)[NU][2][V]) const {
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-      if (V == 1 || !p.interleaved) {
+      if constexpr (V == 1 || !PAIRS) {
         if (turns[u] > 0) {
           float a[V], b[V];
           rot_mul<V>(a, v[u][1], sn[u]);
@@ -296,7 +297,7 @@ template <int EL, int V, int NU> struct RotLane {
           rot_fma<V>(v[u][0], v[u][0], cs[u], a);
           rot_fma<V>(v[u][1], v[u][1], cs[u], b);
         }
-      } else if constexpr (V > 1) {
+      } else {
 #pragma unroll
         for (int k = 0; k < V; k++) {
           float &x = v[u][k / (V / 2)][2 * (k % (V / 2))], &y = v[u][k / (V / 2)][2 * (k % (V / 2)) + 1];
@@ -333,12 +334,12 @@ template <int EL, int V, int NU> struct RotLane {
 __device__ __forceinline__ int64_t rot_at(const B2xHeadStrides& s, int b, int h, int t) { return (int64_t)b * s.batch + (int64_t)h * s.head + (int64_t)t * s.token; }
 
 // A warp: one token (of this CTA's eight), and the heads of share blockIdx.y of all its heads
-template <int EL, int V, int NU>
+template <int EL, int V, int NU, bool PAIRS>
 __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary(const __grid_constant__ RotaryParams p) {
   __shared__ float2 table[kRotaryWarps][128];
   constexpr int ES = EL == EL_F32 ? 4 : 2;
   constexpr int ROWS = NU == 1 ? kRotaryRows : 1;
-  using Lane = RotLane<EL, V, NU>;
+  using Lane = RotLane<EL, V, NU, PAIRS>;
   pdl_trigger();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary(const __grid_co
 }
 
 // Gradient with norms: tensor blockIdx.y; a warp walks tokens in steps of the grid and keeps its elements' share of dw
-template <int EL, int V, int NU>
+template <int EL, int V, int NU, bool PAIRS>
 __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const __grid_constant__ RotaryParams p) {
   __shared__ float2 table[kRotaryWarps][128];
   __shared__ float sums[kRotaryWarps][256];
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ti = blockIdx.y;
   const int slots = 32 / p.lanes, slot = lane / p.lanes;
-  using Lane = RotLane<EL, V, NU>;
+  using Lane = RotLane<EL, V, NU, PAIRS>;
   Lane me;
   me.pieces(p, lane & (p.lanes - 1));
   me.weights(p, ti);
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(kRotaryWarps * 32, 2) k_rotary_gradient(const 
     const char* din = p.dy[ti] + rot_at(p.dys[ti], b, 0, t) * ES;
     char* out = p.y[ti] + rot_at(p.ys[ti], b, 0, t) * ES;
     const int64_t in_head = p.xs[ti].head * ES, din_head = p.dys[ti].head * ES, out_head = p.ys[ti].head * ES;
-    typename RotLane<EL, V, NU>::Raw rx[NU][2], rg[NU][2];
+    typename Lane::Raw rx[NU][2], rg[NU][2];
     me.load(in + (first + slot) * in_head, first + slot < last, rx);
     me.load(din + (first + slot) * din_head, first + slot < last, rg);
     me.angles(p, token, table[warp]);
@@ -521,7 +522,7 @@ RotaryParams rot_params(const B2xRotaryArgs* a, int V, bool each) {
   p.positions = a->positions; p.turns = a->turns;
   p.tokens = (int32_t)(a->B * a->S); p.S = (int32_t)a->S; p.D = (int32_t)a->D; p.R = (int32_t)a->R;
   p.epsilon = a->epsilon; p.inv_d = 1.0f / (float)a->D; p.sine = 1.f;
-  p.interleaved = a->interleaved; p.norm = a->norm; p.weight_f32 = a->weight_elem == EL_F32;
+  p.norm = a->norm; p.weight_f32 = a->weight_elem == EL_F32;
   p.weight_wide = 1;
   for (int i = 0; i < a->n; i++) if ((uintptr_t)a->weight[i] % 16 != 0) p.weight_wide = 0;
   const int pieces = (p.D + V - 1) / V;
@@ -551,17 +552,21 @@ int rot_gradient_ctas(const RotaryParams& p) {
   return (int)(ctas < 1 ? 1 : ctas > kNumSms * 3 ? kNumSms * 3 : ctas);
 }
 
-template <int EL, int V, int NU>
-int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, bool norm_gradient, cudaStream_t stream) {
+template <int EL, int V, int NU, bool PAIRS>
+int launch_rot_as(const B2xRotaryArgs* a, const RotaryParams& p, bool norm_gradient, cudaStream_t stream) {
   cudaError_t e;
-  if (norm_gradient) e = launch_overlapped(k_rotary_gradient<EL, V, NU>, dim3((unsigned)rot_gradient_ctas(p), a->n), dim3(kRotaryWarps * 32), 0, stream, p);
+  if (norm_gradient) e = launch_overlapped(k_rotary_gradient<EL, V, NU, PAIRS>, dim3((unsigned)rot_gradient_ctas(p), a->n), dim3(kRotaryWarps * 32), 0, stream, p);
   else {
     const unsigned jobs = (unsigned)((p.heads[0] + p.heads[1] + p.job_heads - 1) / p.job_heads);
-    e = launch_overlapped(k_rotary<EL, V, NU>, dim3((unsigned)((p.tokens + kRotaryWarps - 1) / kRotaryWarps), jobs), dim3(kRotaryWarps * 32), 0, stream, p);
+    e = launch_overlapped(k_rotary<EL, V, NU, PAIRS>, dim3(((unsigned)p.tokens + kRotaryWarps - 1) / kRotaryWarps, jobs), dim3(kRotaryWarps * 32), 0, stream, p);
   }
   if (e != cudaSuccess) return (int)e;
   count_launch();
   return (int)cudaGetLastError();
+}
+template <int EL, int V, int NU>
+int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, bool norm_gradient, cudaStream_t stream) {
+  return a->interleaved ? launch_rot_as<EL, V, NU, true>(a, p, norm_gradient, stream) : launch_rot_as<EL, V, NU, false>(a, p, norm_gradient, stream);
 }
 template <int EL>
 int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, int V, bool norm_gradient, cudaStream_t stream) {
