@@ -44,14 +44,14 @@ HeadAttn ha_params(const B2xHeadAttentionArgs* a) {
 
 extern "C" int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* a, int gradient) {
   const int64_t ranges = a->documents ? a->B * ((a->Sk + b2x::HA_BLOCK - 1) / b2x::HA_BLOCK) * 8 : 0;
-  if (gradient) return b2x::ha_gradient_scratch(a) + ranges;
+  if (gradient) return b2x::ha_gradient_scratch(a, ranges);
   const b2x::HeadAttn p = b2x::ha_params(a);
   return b2x::ha_token_takes(p) ? b2x::ha_token_scratch(p) : ranges;
 }
 
 extern "C" int b2x_head_attention_launches(const B2xHeadAttentionArgs* a, int gradient) {
   const int q = a->B * a->Hq * a->Sq > 0, k = a->B * a->Hk * a->Sk > 0, ranges = k && a->documents;
-  if (gradient) return ranges + 2 * q + k;
+  if (gradient) return ranges + b2x::ha_gradient_launches(a);
   const b2x::HeadAttn p = b2x::ha_params(a);
   return !q ? 0 : b2x::ha_token_takes(p) ? b2x::ha_token_launches(p) : 1 + ranges;
 }
@@ -66,7 +66,7 @@ extern "C" int b2x_launch_head_attention(const B2xHeadAttentionArgs* a, int32_t*
 
 extern "C" int b2x_launch_head_attention_gradient(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
-  if (!ha_valid(a) || !a->lse || (b2x_head_attention_scratch_bytes(a, 1) > 0 && !a->scratch)) return (int)cudaErrorInvalidValue;
+  if (!ha_valid(a) || !a->lse || (b2x_head_attention_scratch_bytes(a, 1) > 0 && !a->scratch) || ((uintptr_t)a->scratch & 15) != 0) return (int)cudaErrorInvalidValue;
   if (!ha_rows(a->dout, a->dos, a->B, a->Hq, a->Sq) || !ha_rows(a->dq, a->dqs, a->B, a->Hq, a->Sq) || !ha_rows(a->dk, a->dks, a->B, a->Hk, a->Sk) ||
       !ha_rows(a->dv, a->dvs, a->B, a->Hk, a->Sk)) return (int)cudaErrorInvalidValue;
   return ha_launch_gradient(ha_params(a), a->elem, a->scratch, status, (cudaStream_t)stream);

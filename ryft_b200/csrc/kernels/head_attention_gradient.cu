@@ -1,9 +1,11 @@
 // The gradient of attention (head_attention.cu) on the tensor cores.
 //
-// Three launches after the ranges of documents: the row constants (delta = sum dO O, and the log sum in log2 units), dQ per tile of
+// Three launches, or up to five, after the ranges of documents: the row constants (delta = sum dO O, and the log sum in log2 units), dQ per tile of
 // 128 queries, dK and dV per tile of 128 keys.  Both tile kernels compute scores again: seven products of a block of 128 x 128 in
 // all where one kernel that adds dQ in memory would need five, but no sum depends on the order in which CTAs run, and no f32 copy
 // of dQ is written and read.
+//
+// Where there are fewer tiles than SMs (few heads, short sequences) a tile's walk is cut into parts whose sums a further launch joins.
 //
 // Both are one kernel, k_attention_gradient: a tile of 128 rows (queries with their dO; or keys with their values) stays in shared
 // memory, units of 64 of the other side pass by in five stages (eight at a width of 64).  Two products per unit, S and dP (transposed
@@ -42,7 +44,8 @@ struct GradParams {
   const float* neg_lse;               // [B, Hq, rows]: -log sum in log2 units (-inf: nothing seen, or behind the last query)
   const float* neg_delta;             // [B, Hq, rows]
   int32_t rows;                       // queries, rounded up to 128
-  int32_t tiles, group_heads, key_blocks, total;
+  int32_t tiles, group_heads, key_blocks, total, parts;   // total: tiles of all heads, times the parts of each (grad_parts)
+  float* partial;                     // parts' sums: [part][tile][dQ, or dV and dK][128][D]
   uint64_t in2;                       // scale * log2(e)
   HeadCap cap;
   float scale;
@@ -138,6 +141,62 @@ __device__ __forceinline__ void grad_write(uint32_t taddr, char* row, bool there
   if (there) ha_store_row(row, width, wd);
 }
 
+// The same as f32, of a part of the tile's units
+__device__ __forceinline__ void grad_part(uint32_t taddr, float* row, float f, bool zero) {
+  uint32_t x[16];
+  if (!zero) { sm100::tmem_ld_32x16(taddr, x); sm100::tc_wait_ld(); }
+  else {
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[i] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < 16; i += 4)
+    *(float4*)(row + i) = make_float4(__uint_as_float(x[i]) * f, __uint_as_float(x[i + 1]) * f, __uint_as_float(x[i + 2]) * f, __uint_as_float(x[i + 3]) * f);
+}
+
+// Parts that a tile's units are cut into.  Where there are fewer tiles than SMs, the longest walk takes the whole time; parts of nine
+// units and more, as many as fill the SMs (twice under a causal mask, which leaves half of the units), are summed in f32 and joined in
+// their order by k_gradient_join.  Whole gradients, causal: 8 query heads of one key head, 4096 x 128, 534 -> 150 us; 16/4 heads, 2048 x 128,
+// 167 -> 101; 2 heads, 3766 x 80, cap and bias, 151 -> 91.  4 heads, 1024 x 128, without a mask: two parts of eight units 47 us, one 46.
+template <typename Args> int grad_parts(const Args& a, bool keys) {
+  const int64_t tiles = (int64_t)a.B * (keys ? a.Hk : a.Hq) * (((keys ? a.Sk : a.Sq) + HA_BLOCK - 1) / HA_BLOCK);
+  const int64_t units = (((keys ? a.Sq : a.Sk) + GRAD_UNIT - 1) / GRAD_UNIT) * (keys && a.Hk > 0 ? a.Hq / a.Hk : 1);
+  if (tiles <= 0) return 1;
+  int64_t parts = (a.causal ? 2 : 1) * kNumSms / tiles;
+  if (parts > units / 9) parts = units / 9;
+  return parts < 1 ? 1 : (int)(parts < 16 ? parts : 16);
+}
+// bytes of the parts' sums of one side
+template <typename Args> int64_t grad_part_bytes(const Args& a, bool keys) {
+  const int parts = grad_parts(a, keys);
+  return parts == 1 ? 0 : (int64_t)parts * a.B * (keys ? 2 * a.Hk : a.Hq) * (((keys ? a.Sk : a.Sq) + HA_BLOCK - 1) / HA_BLOCK) * HA_BLOCK * (a.D <= 64 ? 64 : 128) * 4;
+}
+
+// One warp per row: the parts' sums in their order, as 16-bit values
+template <int D, int EL, bool KEYS>
+__global__ void __launch_bounds__(256) k_gradient_join(const __grid_constant__ GradParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int col = (threadIdx.x & 31) * 4;
+  const int64_t tiles = p.total / p.parts;
+  const int heads = KEYS ? p.a.Hk : p.a.Hq, tokens = KEYS ? p.a.Sk : p.a.Sq;
+  const int row = (int)(id % HA_BLOCK);
+  const int64_t rest = id / HA_BLOCK, tile = KEYS ? rest >> 1 : rest;
+  const bool second = KEYS && (rest & 1);
+  const int bh = (int)(tile / p.tiles), token = (int)(tile - (int64_t)bh * p.tiles) * HA_BLOCK + row, b = bh / heads, h = bh - b * heads;
+  if (tile < tiles && token < tokens && col < p.a.D) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.parts; k++) {
+      const uint4 x = ld_global((const uint4*)(p.partial + (((k * tiles + tile) * (KEYS ? 2 : 1) + second) * HA_BLOCK + row) * D + col));
+      v.x += __uint_as_float(x.x); v.y += __uint_as_float(x.y); v.z += __uint_as_float(x.z); v.w += __uint_as_float(x.w);
+    }
+    const B2xHeadStrides& o = !KEYS ? p.a.dqs : second ? p.a.dks : p.a.dvs;
+    char* out = (!KEYS ? p.a.dq : second ? p.a.dk : p.a.dv) + 2 * ((int64_t)b * o.batch + (int64_t)h * o.head + (int64_t)token * o.token + col);
+    *(uint2*)out = make_uint2(ha_pack<EL>(v.x, v.y), ha_pack<EL>(v.z, v.w));
+  }
+}
+
 // ---- the tile kernel -------------------------------------------------------------------------------------------------------
 // Pairs of score buffers in TMEM, each with four warps of its own: as many as the accumulators leave room for
 template <int D, bool KEYS> struct GradShape {
@@ -220,7 +279,8 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         // the tiles with the most units first: the last queries, the first keys; inside a group of heads that stay in L2 together
         const int all = KEYS ? p.a.Hk : p.a.Hq;
         const int per_group = p.group_heads * p.tiles;
-        const int g = t / per_group, in = t - g * per_group;
+        const int tile = t / p.parts;
+        const int g = tile / per_group, in = tile - g * per_group;
         const int heads = min(p.group_heads, p.a.B * all - g * p.group_heads);
         const int rank = in / heads, bh = g * p.group_heads + (in - rank * heads);
         b = bh / all; h = bh - b * all;
@@ -265,14 +325,18 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
           units = count;
         }
       }
+      // this part's share of the units
+      const int whole = units * repeat, share = (whole + p.parts - 1) / p.parts, part = t >= 0 ? t % p.parts : 0;
+      const int skip = min(part * share, whole), count = min(share, whole - skip);
       if (lane == 0) {
+        s->skip = skip; s->count = count; s->part = part;
         s->tile = t; s->b = b; s->h = h; s->at = at; s->begin = begin; s->blocks = units;
         s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
         mbar_arrive(bar_tf + 8 * (n & 1));
       }
       __syncwarp();
       if (t < 0) break;
-      if (units == 0) continue;
+      if (count == 0) continue;
       if (elect_one()) {
         bool ok = nt == 0 || ha_barrier(bar_tu, (nt - 1) & 1, abort_flag, status, 62);
         if (ok) {
@@ -282,29 +346,30 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
             tma_load_4d(sbase + SM::T0_OFF + c * HA_CHUNK, &tmT0, bar_tl, c * 64, at, h, b);
             tma_load_4d(sbase + SM::T1_OFF + c * HA_CHUNK, &tmT1, bar_tl, c * 64, at, h, b);
           }
-          uint32_t k = uc;
-          for (int hh = 0; hh < repeat && ok; hh++) {
+          int hh = skip / units, it = skip - hh * units;
+          BlockWalk walk;
+          walk.start(s, listed);
+          for (int i = 0; i < it; i++) walk.next();
+          for (uint32_t k = uc; k < uc + (uint32_t)count; k++) {
+            const uint32_t st = k % STAGES, turn = k / STAGES;
             const int uh = KEYS ? h * p.a.group + hh : h / p.a.group;
-            BlockWalk walk;
-            walk.start(s, listed);
-            for (int it = 0; it < units; it++, k++) {
-              const uint32_t st = k % STAGES, turn = k / STAGES;
-              if (turn > 0 && !ha_barrier(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
-              mbar_expect_tx(bar_uf + 8 * st, 2 * SM::U_BYTES);
-              const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES;
+            if (turn > 0 && !ha_barrier(bar_ue + 8 * st, (turn - 1) & 1, abort_flag, status, 63)) { ok = false; break; }
+            mbar_expect_tx(bar_uf + 8 * st, 2 * SM::U_BYTES);
+            const uint32_t ua = sbase + SM::U_OFF + st * 2 * SM::U_BYTES;
 #pragma unroll
-              for (int c = 0; c < DC; c++) {
-                tma_load_4d(ua + c * U_CHUNK, &tmU0, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
-                tma_load_4d(ua + SM::U_BYTES + c * U_CHUNK, &tmU1, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
-              }
-              if (it + 1 < units) walk.next();
+            for (int c = 0; c < DC; c++) {
+              tma_load_4d(ua + c * U_CHUNK, &tmU0, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
+              tma_load_4d(ua + SM::U_BYTES + c * U_CHUNK, &tmU1, bar_uf + 8 * st, c * 64, walk.j * GRAD_UNIT, uh, b);
             }
+            // the next unit, over the end of a head
+            if (++it < units) walk.next();
+            else { it = 0; hh++; walk.start(s, listed); }
           }
         }
         if (!ok) grad_linger();
       }
       __syncwarp();
-      uc += (uint32_t)(units * repeat); nt++;
+      uc += (uint32_t)count; nt++;
       if (__any_sync(0xffffffffu, *abort_flag != 0)) break;
     }
   } else if (warp == 1) {
@@ -339,7 +404,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       };
       for (int n = 0; ok; n++) {
         if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 72)) { ok = false; break; }
-        const int t = slots[n & 1].tile, total = slots[n & 1].blocks * repeat;
+        const int t = slots[n & 1].tile, total = slots[n & 1].count;
         mbar_arrive(bar_te + 8 * (n & 1));
         if (t < 0) break;
         if (total == 0) continue;
@@ -386,7 +451,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       const int t = s->tile, units = s->blocks, b = s->b, th = s->h, at = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
       if (t < 0) break;
-      const int total = units * repeat, self = at + row;   // this row's query or key
+      const int total = s->count, skip = s->skip, part = s->part, self = at + row;   // this part's units; this row's query or key
       // queries: keys up to `edge` are seen; keys: queries from `edge` on see this key
       const int pos = KEYS ? self : seq.first + self;
       int edge;
@@ -418,7 +483,9 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       int k = 0;
       float ahead = 0.f;
       if (total > 0) {
+        hh = skip / units; it = skip - hh * units;
         walk.start(s, listed);
+        for (int i = 0; i < it; i++) walk.next();
         for (uint32_t first = ((uint32_t)g + GROUPS - uc % GROUPS) % GROUPS; k < (int)first && k < total; k++) advance();
         if (KEYS && k < total) ahead = fetch(hh, walk.j);
       }
@@ -530,6 +597,12 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       for (int c = g; c < (KEYS ? 2 : 1) * (D / 16); c += GROUPS) {
         const bool second = c >= D / 16;
         const int first = (second ? c - D / 16 : c) * 16;
+        if (p.parts > 1) {
+          const int64_t tiles = p.total / p.parts, tile = ((int64_t)b * (KEYS ? p.a.Hk : p.a.Hq) + th) * p.tiles + at / HA_BLOCK;
+          grad_part(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), p.partial + (((part * tiles + tile) * (KEYS ? 2 : 1) + second) * HA_BLOCK + row) * D + first,
+                    KEYS && !second ? 1.f : p.scale, total == 0);
+          continue;
+        }
         const B2xHeadStrides& o = !KEYS ? p.a.dqs : second ? p.a.dks : p.a.dvs;
         char* out = (!KEYS ? p.a.dq : second ? p.a.dk : p.a.dv) + 2 * ((int64_t)b * o.batch + (int64_t)th * o.head + (int64_t)self * o.token + first);
         grad_write<EL>(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), out, self < (KEYS ? p.a.Sk : p.a.Sq), p.a.D - first, KEYS && !second ? 1.f : p.scale, total == 0);
@@ -602,7 +675,8 @@ int launch_side(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* st
   const int64_t all = (int64_t)a.B * (KEYS ? a.Hk : a.Hq);
   p.tiles = (tokens + HA_BLOCK - 1) / HA_BLOCK;
   if (all * p.tiles > 0x7fffff00) return (int)cudaErrorInvalidValue;
-  p.total = (int)(all * p.tiles);
+  p.parts = grad_parts(a, KEYS);
+  p.total = (int)(all * p.tiles) * p.parts;
   // what passes by (K and V of a key head, or Q and dO of its query heads) stays in L2 for a group of heads: 32 MiB, as in the
   // forward pass
   const int64_t fit = (32ll << 20) / ((int64_t)(others > 0 ? others : 1) * a.D * 4), heads = KEYS ? fit / a.group : fit * a.group, least = KEYS ? 1 : a.group;
@@ -630,6 +704,12 @@ int launch_side(const HeadAttn& a, GradParams p, const int2* ranges, int32_t* st
   const cudaError_t e = launch_overlapped(kern, dim3((unsigned)(p.total < kNumSms ? p.total : kNumSms)), dim3(GradShape<D, KEYS>::THREADS), SM::TOTAL, stream, t0, t1, u0, u1, p, ha_sched(stream), status);
   if (e != cudaSuccess) return (int)e;
   count_launch();
+  if (p.parts > 1) {
+    const int64_t rows = (int64_t)(p.total / p.parts) * (KEYS ? 2 : 1) * HA_BLOCK;
+    const cudaError_t f = launch_overlapped(k_gradient_join<D, EL, KEYS>, dim3((unsigned)(rows / 8)), dim3(256), 0, stream, p);
+    if (f != cudaSuccess) return (int)f;
+    count_launch();
+  }
   return (int)cudaGetLastError();
 }
 template <int D, int EL>
@@ -642,9 +722,17 @@ int grad_rows(int64_t Sq) { return (int)((Sq + HA_BLOCK - 1) / HA_BLOCK * HA_BLO
 
 }  // namespace
 
-int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a) { return a->B * a->Hq * (int64_t)grad_rows(a->Sq) * 8; }
+// row constants [2][B, Hq, rows], the documents' ranges, and from a multiple of 16 bytes on the sums of parts, of one side at a time
+int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a, int64_t ranges) {
+  const int64_t head = a->B * a->Hq * (int64_t)grad_rows(a->Sq) * 8 + ranges, q = grad_part_bytes(*a, false), k = grad_part_bytes(*a, true);
+  return q > 0 || k > 0 ? (head + 15) / 16 * 16 + (q > k ? q : k) : head;
+}
+int ha_gradient_launches(const B2xHeadAttentionArgs* a) {
+  const int q = a->B * a->Hq * a->Sq > 0, k = a->B * a->Hk * a->Sk > 0;
+  return (q ? 2 + (grad_parts(*a, false) > 1) : 0) + (k ? 1 + (grad_parts(*a, true) > 1) : 0);
+}
 
-// scratch: row constants [2][B, Hq, rows], then the documents' ranges
+// scratch: ha_gradient_scratch
 int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* status, cudaStream_t stream) {
   if (a.B == 0 || a.Hq == 0) return 0;
   GradParams p{};
@@ -655,6 +743,7 @@ int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* stat
   p.neg_delta = p.neg_lse + n;
   int2* ranges = (int2*)(p.neg_delta + n);
   p.key_blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
+  p.partial = (float*)((char*)scratch + (n * 8 + (a.documents ? (int64_t)a.B * p.key_blocks * 8 : 0) + 15) / 16 * 16);
   p.scale = a.scale;
   p.in2 = ha_pair(a.scale * kLog2e);
   p.cap = ha_cap(a.softcap, a.scale);

@@ -1,10 +1,12 @@
 """The named operators without a GPU: how they are read, what is refused, and the 64-bit forms against differences."""
+import ctypes
+
 import pytest
 import torch
 
 import operators_reference as ref
 import ryft_b200
-from ryft_b200 import pjrt
+from ryft_b200 import kernels, pjrt
 from ryft_b200.stablehlo import Builder
 
 
@@ -39,6 +41,28 @@ def test_scratch_covers_what_the_operands_ask_for():
     assert "scratch=48 B" in dump
     dump = plan(lambda b: [b.attention(*[heads(b, S=300) for _ in range(3)], causal=True)])
     assert "scratch=0 B" in dump
+
+
+@pytest.mark.parametrize("B,Hq,Hk,Sq,Sk,D,causal,q_parts,k_parts", [
+    (1, 2, 1, 1300, 1300, 128, 1, 2, 4),
+    (1, 1, 1, 1100, 2100, 64, 0, 3, 2),
+    (1, 12, 1, 200, 200, 128, 1, 1, 5),
+    (1, 2, 2, 20, 1200, 40, 1, 2, 1),
+    (1, 16, 4, 8192, 8192, 128, 1, 1, 1),
+    (1, 1, 1, 40000, 100, 64, 0, 1, 16),
+    (0, 2, 1, 100, 100, 64, 0, 1, 1),
+    (1, 1, 1, 0, 100, 64, 0, 1, 1),
+    (1, 0, 0, 100, 100, 64, 0, 1, 1),
+])
+def test_scratch_and_launches_of_gradients_in_parts(B, Hq, Hk, Sq, Sk, D, causal, q_parts, k_parts):
+    lib = kernels.load()
+    a = kernels.HeadAttentionArgs(elem=10, causal=causal, B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, D=D)
+    rows, keys, wide = -(-Sq // 128) * 128, -(-Sk // 128) * 128, 64 if D <= 64 else 128
+    parts = max(q_parts * B * Hq * rows * wide * 4 if q_parts > 1 else 0, k_parts * 2 * B * Hk * keys * wide * 4 if k_parts > 1 else 0)
+    assert lib.b2x_head_attention_scratch_bytes(ctypes.byref(a), 1) == B * Hq * rows * 8 + parts
+    tiles = (2 + (q_parts > 1) if B * Hq * Sq else 0) + (1 + (k_parts > 1) if B * Hk * Sk else 0)
+    assert lib.b2x_head_attention_launches(ctypes.byref(a), 1) == tiles
+
 
 
 def test_rows_that_are_not_contiguous_are_copied():

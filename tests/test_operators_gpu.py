@@ -271,6 +271,32 @@ def test_nan_scores_make_their_own_rows_nan(client):
     assert torch.equal(torch.isnan(lse), bad) and torch.equal(torch.isnan(o).any(-1), bad)
 
 
+# fewer tiles than SMs: the gradient's sums over queries or keys are cut into parts
+PARTS = [
+    (dict(B=1, Sq=1300, Sk=1300, Hq=2, Hk=1, D=128, dtype="bf16", layout="bshd"), dict(causal=True, softcap=30.0)),
+    (dict(B=1, Sq=1100, Sk=2100, Hq=1, Hk=1, D=64, dtype="f16", layout="bhsd"), dict(lengths=[1500], slopes=True)),
+    (dict(B=2, Sq=1060, Sk=1060, Hq=3, Hk=1, D=80, dtype="bf16", layout="bshd"), dict(causal=True, documents=5, prefix=[0, 700])),
+    (dict(B=1, Sq=1100, Sk=1100, Hq=2, Hk=2, D=64, dtype="f16", layout="bhsd"), dict(documents=40, unsorted=True, causal=True)),
+    (dict(B=1, Sq=200, Sk=200, Hq=12, Hk=1, D=128, dtype="f16", layout="bhsd"), dict(causal=True)),       # keys only: many query heads
+    (dict(B=1, Sq=20, Sk=1200, Hq=2, Hk=2, D=40, dtype="bf16", layout="bshd"), dict(causal=True, query_offset=1180)),       # queries only
+    (dict(B=2, Sq=1030, Sk=1030, Hq=1, Hk=1, D=128, dtype="bf16", layout="bhsd"), dict(causal=True, lengths=[0, 70])),      # parts without a unit
+    (dict(B=1, Sq=64, Sk=64, Hq=40, Hk=1, D=8, dtype="f16", layout="bshd"), dict(scale=0.5, documents=3)),
+]
+
+
+@pytest.mark.parametrize("sizes,options", PARTS, ids=str)
+def test_gradients_in_parts(client, sizes, options):
+    attention_check(client, **sizes, **options)
+
+
+def test_gradients_in_parts_do_not_differ_from_run_to_run(client):
+    q, k, v, do, extra, how = attention_case(1, 1100, 1100, 4, 1, 128, "bf16", "bshd", 9, causal=True)
+    first = attention_run(client, q, k, v, do, extra, how, "bf16", "bshd")
+    for _ in range(3):
+        for a, c in zip(attention_run(client, q, k, v, do, extra, how, "bf16", "bshd"), first):
+            assert torch.equal(a, c)
+
+
 def test_results_do_not_differ_from_run_to_run(client):
     q, k, v, do, extra, how = attention_case(2, 500, 500, 4, 2, 128, "bf16", "bshd", 9, causal=True, softcap=30.0)
     first = attention_run(client, q, k, v, do, extra, how, "bf16", "bshd")
