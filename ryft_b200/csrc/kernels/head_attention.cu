@@ -46,19 +46,19 @@ extern "C" int64_t b2x_head_attention_scratch_bytes(const B2xHeadAttentionArgs* 
   const int64_t ranges = a->documents ? a->B * ((a->Sk + b2x::HA_BLOCK - 1) / b2x::HA_BLOCK) * 8 : 0;
   if (gradient) return b2x::ha_gradient_scratch(a, ranges);
   const b2x::HeadAttn p = b2x::ha_params(a);
-  return b2x::ha_token_takes(p) ? b2x::ha_token_scratch(p) : ranges;
+  return b2x::ha_token_takes(p) ? b2x::ha_token_scratch(p) : b2x::ha_forward_scratch(p, ranges);
 }
 
 extern "C" int b2x_head_attention_launches(const B2xHeadAttentionArgs* a, int gradient) {
   const int q = a->B * a->Hq * a->Sq > 0, k = a->B * a->Hk * a->Sk > 0, ranges = k && a->documents;
   if (gradient) return ranges + b2x::ha_gradient_launches(a);
   const b2x::HeadAttn p = b2x::ha_params(a);
-  return !q ? 0 : b2x::ha_token_takes(p) ? b2x::ha_token_launches(p) : 1 + ranges;
+  return !q ? 0 : b2x::ha_token_takes(p) ? b2x::ha_token_launches(p) : b2x::ha_forward_launches(p) + ranges;
 }
 
 extern "C" int b2x_launch_head_attention(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
-  if (!ha_valid(a) || (b2x_head_attention_scratch_bytes(a, 0) > 0 && !a->scratch)) return (int)cudaErrorInvalidValue;
+  if (!ha_valid(a) || (b2x_head_attention_scratch_bytes(a, 0) > 0 && !a->scratch) || ((uintptr_t)a->scratch & 15) != 0) return (int)cudaErrorInvalidValue;
   const HeadAttn p = ha_params(a);
   if (ha_token_takes(p)) return ha_launch_token(p, a->elem, a->scratch, (cudaStream_t)stream);
   return ha_launch_forward(p, a->elem, (int2*)a->scratch, status, (cudaStream_t)stream);

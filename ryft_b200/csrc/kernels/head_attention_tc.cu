@@ -7,6 +7,8 @@
 // registers through cap, bias, mask, maximum and exponential.  Per worker Q, one K and one V stage, half a buffer of weights (the
 // second half's first keys are exponentiated while the first half multiplies), 128 score columns and the accumulator in TMEM.
 //
+// Where there are fewer tiles than workers a tile's walk is cut into parts (tile_parts), which a second launch joins.
+//
 // What masks leave out is left out in three grades: blocks that no query of the tile sees are neither loaded nor multiplied (the
 // keys' end follows from the last query; with documents the loading warp compares ranges of document numbers and publishes the
 // tile's blocks as bits); blocks that every query sees run without a test; in the others a row's keys are 128 bits, from the
@@ -29,7 +31,9 @@ namespace {
 struct TileParams {
   HeadAttn a;
   const int2* ranges;          // documents' ranges per block, [B][key blocks]
-  int32_t q_tiles, group_heads, key_blocks, total;
+  int32_t q_tiles, group_heads, key_blocks, total, parts;   // total: tiles of all heads, times the parts of each (tile_parts)
+  float* part_o;               // parts' accumulators: [part][tile][128][D]
+  float2* part_ml;             // parts' maxima (log2 units) and sums: [part][tile][128]
   float mult;                  // scores in registers times this are log2 units: scale * log2(e), or 1 where cap or bias made them so
   uint64_t in2;                // scale * log2(e)
   HeadCap cap;
@@ -106,24 +110,26 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     // ---------------------------------------------- tiles and loads ------------------------------------------------
     uint32_t kc = 0, vc = 0;       // K and V blocks loaded so far
     uint32_t nq = 0;               // tiles with work so far
-    int fixed = (int)blockIdx.x * 2 + w;   // without a counter: every worker takes tiles in steps of all workers
+    int fixed = (int)blockIdx.x + w * (int)gridDim.x;   // without a counter: every worker takes tiles in steps of all workers
     for (int n = 0;; n++) {
       // the slot's previous tile has been read by the issuer and the four softmax warps (all lanes wait: they leave together)
       const bool free = n < 2 || ha_barrier(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21);
       if (!__all_sync(0xffffffffu, free)) break;
       int t = 0;
-      if (sched) {
+      if (w == 1 && p.total <= (int)gridDim.x) t = -1;     // one tile per SM: the first workers take them
+      else if (sched) {
         if (lane == 0) t = atomicAdd(sched, 1);
         t = __shfl_sync(0xffffffffu, t, 0);
       } else { t = fixed; fixed += 2 * (int)gridDim.x; }
       if (t >= p.total) t = -1;
       volatile TileSlot* s = slots + (n & 1);
-      int bh = 0, qt = 0, blocks = 0;
+      int bh = 0, qt = 0, blocks = 0, begin = 0;
       HeadSequence seq{};
       if (t >= 0) {
         // groups of heads whose keys stay in L2 together; inside a group the tiles with the longest causal prefix first
         const int per_group = p.group_heads * p.q_tiles;
-        const int g = t / per_group, in = t - g * per_group;
+        const int tile = t / p.parts;
+        const int g = tile / per_group, in = tile - g * per_group;
         const int heads = min(p.group_heads, p.a.B * p.a.Hq - g * p.group_heads);
         const int rank = in / heads;
         bh = g * p.group_heads + (in - rank * heads);
@@ -158,9 +164,23 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           blocks = count;
         }
+        if (p.parts > 1) {
+          // this part's share of the blocks
+          const int share = (blocks + p.parts - 1) / p.parts, skip = min((t - tile * p.parts) * share, blocks);
+          blocks = min(share, blocks - skip);
+          begin = skip;
+          if (listed && lane == 0) {
+            s->begin = 0;
+            BlockWalk walk;
+            walk.start(s, true);
+            for (int i = 0; i < skip; i++) walk.next();
+            begin = walk.j;
+          }
+        }
       }
       if (lane == 0) {
-        s->tile = t; s->b = bh / max(p.a.Hq, 1); s->h = bh % max(p.a.Hq, 1); s->at = qt * HA_BLOCK; s->begin = 0; s->blocks = blocks;
+        s->tile = t; s->b = bh / max(p.a.Hq, 1); s->h = bh % max(p.a.Hq, 1); s->at = qt * HA_BLOCK; s->begin = begin; s->blocks = blocks;
+        s->part = t >= 0 ? t % p.parts : 0;
         s->length = seq.length; s->first = seq.first; s->prefix = seq.prefix;
         mbar_arrive(bar_tf + 8 * (n & 1));
       }
@@ -577,6 +597,30 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tc_fence_after();
       }
       if (poisoned) l = __int_as_float(0x7fc00000);
+      if (p.parts > 1) {
+        const int64_t at = ((int64_t)s->part * (p.total / p.parts) + ((int64_t)s->b * p.a.Hq + s->h) * p.q_tiles + s->at / HA_BLOCK) * HA_BLOCK + row;
+#pragma unroll 1
+        for (int c = 0; c < D / 16; c++) {
+          uint32_t x[16];
+          if (blocks > 0) {
+            tmem_ld_32x16(o_addr + (uint32_t)(c * 16), x);
+            tc_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = 0;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) *(uint4*)(p.part_o + at * D + c * 16 + i) = make_uint4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        }
+        p.part_ml[at] = make_float2(m_used * p.mult, l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar_te + 8 * (n & 1));
+          if (blocks > 0) mbar_arrive(bar_of);
+        }
+        continue;
+      }
       const float inv = !(l <= 0.f) ? 1.0f / l : 0.f;   // a NaN sum stays NaN
       const int b = s->b, h = s->h, qrow = s->at + row;
       char* orow = p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)h * p.a.os.head + (int64_t)qrow * p.a.os.token);
@@ -616,6 +660,54 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (sched && threadIdx.x == 0 && atomicAdd(sched + 1, 1) == (int)gridDim.x - 1) { sched[0] = 0; sched[1] = 0; __threadfence(); }
 }
 
+// Parts that a tile's blocks are cut into.  Where there are fewer tiles than workers, the longest walk takes the whole time; parts of
+// four blocks and more, as many as give every worker one (two under a causal mask, which leaves half of the blocks).  2 heads, 3766 x 80,
+// cap and bias, causal: 162 -> 47 us; 2/1 heads, 2692 x 64, bias, 75 -> 31; 4 heads, 1024 x 128, 28 -> 20.  Where every SM has a tile as
+// it is, writing and joining the parts has to be worth it: 256 causal tiles of up to 32 blocks 84 -> 66 us, of up to 16 blocks 47 -> 51.
+template <typename Args> int tile_parts(const Args& a) {
+  const int64_t tiles = (int64_t)a.B * a.Hq * ((a.Sq + HA_BLOCK - 1) / HA_BLOCK), blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
+  if (tiles <= 0) return 1;
+  int64_t parts = (a.causal ? 4 : 2) * kNumSms / tiles;
+  if (parts > blocks / 4) parts = blocks / 4;
+  if (tiles > kNumSms && blocks < 24) parts = 1;
+  return parts < 1 ? 1 : (int)(parts < 16 ? parts : 16);
+}
+// Parts are joined as the blocks of a walk are: by their maxima.  One warp per row.
+template <int D, int EL>
+__global__ void __launch_bounds__(256) k_attention_join(const __grid_constant__ TileParams p) {
+  pdl_trigger();
+  pdl_wait();
+  const int64_t id = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), rows = (int64_t)(p.total / p.parts) * HA_BLOCK;
+  const int lane = threadIdx.x & 31, col = lane * 4;
+  const int tile = (int)(id / HA_BLOCK), bh = tile / p.q_tiles, i = (tile - bh * p.q_tiles) * HA_BLOCK + (int)(id % HA_BLOCK), b = bh / p.a.Hq, h = bh - b * p.a.Hq;
+  if (id < rows && i < p.a.Sq) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < p.parts) { const uint2 v = ld_global((const uint2*)(p.part_ml + lane * rows + id)); ml = make_float2(__uint_as_float(v.x), __uint_as_float(v.y)); }
+    // a part that saw nothing has a sum of 0 and is left out, whatever its accumulator holds
+    float m = ml.y == 0.f ? -INFINITY : ml.x;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float w = ml.y == 0.f ? 0.f : fast_exp2(ml.x - m);
+    float l = ml.y == 0.f ? 0.f : ml.y * w;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.parts; k++) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      if (wk != 0.f && col < p.a.D) {
+        const uint4 x = ld_global((const uint4*)(p.part_o + (k * rows + id) * D + col));
+        o.x = fmaf(__uint_as_float(x.x), wk, o.x); o.y = fmaf(__uint_as_float(x.y), wk, o.y);
+        o.z = fmaf(__uint_as_float(x.z), wk, o.z); o.w = fmaf(__uint_as_float(x.w), wk, o.w);
+      }
+    }
+    const float inv = !(l <= 0.f) ? 1.0f / l : 0.f;   // a NaN sum stays NaN
+    if (col < p.a.D)
+      *(uint2*)(p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)h * p.a.os.head + (int64_t)i * p.a.os.token + col)) =
+          inv == 0.f ? make_uint2(0, 0) : make_uint2(ha_pack<EL>(o.x * inv, o.y * inv), ha_pack<EL>(o.z * inv, o.w * inv));
+    if (lane == 0 && p.a.lse) p.a.lse[(int64_t)bh * p.a.Sq + i] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * 0.6931471805599453f;
+  }
+}
+
 // One warp per block of 128 tokens
 __global__ void __launch_bounds__(256) k_document_ranges(const int32_t* documents, int2* ranges, int32_t B, int32_t Sk, int32_t blocks) {
   pdl_trigger();
@@ -648,10 +740,15 @@ int launch_tiles(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& 
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) configured[dev].store(true, std::memory_order_release);
   }
-  const int ctas = (p.total + 1) / 2 < kNumSms ? (p.total + 1) / 2 : kNumSms;
+  const int ctas = p.total < kNumSms ? p.total : kNumSms;
   const cudaError_t e = launch_overlapped(kern, dim3((unsigned)ctas), dim3(384), SM::TOTAL, stream, q, k, v, p, sched, status);
   if (e != cudaSuccess) return (int)e;
   count_launch();
+  if (p.parts > 1) {
+    const cudaError_t f = launch_overlapped(k_attention_join<D, EL>, dim3((unsigned)((int64_t)(p.total / p.parts) * HA_BLOCK / 8)), dim3(256), 0, stream, p);
+    if (f != cudaSuccess) return (int)f;
+    count_launch();
+  }
   return (int)cudaGetLastError();
 }
 
@@ -676,6 +773,12 @@ int ha_launch_ranges(const HeadAttn& p, int2* ranges, cudaStream_t stream) {
   return (int)cudaGetLastError();
 }
 
+int64_t ha_forward_scratch(const HeadAttn& a, int64_t ranges) {
+  const int parts = tile_parts(a);
+  return parts == 1 ? ranges : (ranges + 15) / 16 * 16 + (int64_t)parts * a.B * a.Hq * ((a.Sq + HA_BLOCK - 1) / HA_BLOCK) * HA_BLOCK * ((a.D <= 64 ? 64 : 128) * 4 + 8);
+}
+int ha_forward_launches(const HeadAttn& a) { return 1 + (tile_parts(a) > 1); }
+
 int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status, cudaStream_t stream) {
   TileParams p{};
   p.a = a;
@@ -684,11 +787,16 @@ int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status
   const int64_t total = (int64_t)a.B * a.Hq * p.q_tiles;
   if (total == 0) return 0;
   if (total > 0x7fffff00) return (int)cudaErrorInvalidValue;
-  p.total = (int)total;
+  p.parts = tile_parts(a);
+  p.total = (int)total * p.parts;
   if (a.documents) {
     const int rc = ha_launch_ranges(a, ranges, stream);
     if (rc) return rc;
   }
+  // scratch: ranges, then from a multiple of 16 bytes on the parts
+  const int D = a.D <= 64 ? 64 : 128;
+  p.part_o = (float*)((char*)ranges + ((a.documents ? (int64_t)a.B * p.key_blocks * 8 : 0) + 15) / 16 * 16);
+  p.part_ml = (float2*)(p.part_o + (int64_t)p.total * HA_BLOCK * D);
   // longer sequences than a skip list covers walk all their blocks, and compare in each
   p.ranges = a.documents && p.key_blocks <= HA_MASK_WORDS * 32 ? ranges : nullptr;
   const int64_t kv_heads = (32ll << 20) / ((int64_t)(a.Sk > 0 ? a.Sk : 1) * a.D * 4);
@@ -698,7 +806,6 @@ int ha_launch_forward(const HeadAttn& a, int elem, int2* ranges, int32_t* status
   p.mult = p.scaled ? 1.0f : a.scale * kLog2e;
   p.in2 = ha_pair(a.scale * kLog2e);
   p.cap = ha_cap(a.softcap, a.scale);
-  const int D = a.D <= 64 ? 64 : 128;
   const uint32_t format = elem == EL_BF16 ? 1u : 0u;
   p.idesc_qk = sm100::make_idesc(format, false, false, HA_BLOCK, HA_BLOCK);
   p.idesc_pv = sm100::make_idesc(format, false, true, HA_BLOCK, (uint32_t)D);

@@ -211,7 +211,7 @@ struct TileSlot {
   int tile;                    // -1: no more
   int b, h, at;                // sequence, head, first query (or key) of the tile
   int begin, blocks;           // first block to walk, and how many
-  int skip, count, part;       // gradient: of the units of all heads that pass by, those before this part's, this part's, and its number
+  int part, skip, count;       // number of this part of the tile; gradient: of the units of all heads that pass by, those before and of this part
   int length, first, prefix;   // HeadSequence
   uint32_t visit[HA_MASK_WORDS], compare[HA_MASK_WORDS];   // with documents: blocks to walk, and those whose documents have to be compared
 };
@@ -250,6 +250,8 @@ int ha_token_launches(const HeadAttn& p);
 int ha_launch_token(const HeadAttn& p, int elem, void* scratch, cudaStream_t stream);
 int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a, int64_t ranges);
 int ha_gradient_launches(const B2xHeadAttentionArgs* a);
+int64_t ha_forward_scratch(const HeadAttn& p, int64_t ranges);
+int ha_forward_launches(const HeadAttn& p);
 int ha_launch_gradient(const HeadAttn& p, int elem, void* scratch, int32_t* status, cudaStream_t stream);
 int ha_launch_forward(const HeadAttn& p, int elem, int2* ranges, int32_t* status, cudaStream_t stream);
 

@@ -65,6 +65,16 @@ def test_scratch_and_launches_of_gradients_in_parts(B, Hq, Hk, Sq, Sk, D, causal
 
 
 
+@pytest.mark.parametrize("B,Hq,Sq,Sk,D,causal,parts", [(1, 2, 1300, 1300, 128, 1, 2), (1, 1, 1100, 2100, 64, 0, 4), (1, 2, 130, 2500, 80, 0, 5), (1, 1, 17, 100000, 64, 0, 16),
+                                                       (1, 16, 8192, 8192, 128, 1, 1), (1, 16, 2048, 2048, 128, 1, 1), (1, 8, 4096, 4096, 128, 1, 2), (3, 12, 1000, 1000, 64, 0, 1), (1, 1, 200, 500, 64, 0, 1), (0, 1, 200, 5000, 64, 0, 1), (1, 1, 200, 0, 64, 0, 1)])
+def test_scratch_and_launches_of_attention_in_parts(B, Hq, Sq, Sk, D, causal, parts):
+    lib = kernels.load()
+    a = kernels.HeadAttentionArgs(elem=10, causal=causal, B=B, Hq=Hq, Hk=Hq, Sq=Sq, Sk=Sk, D=D)
+    rows = B * Hq * -(-Sq // 128) * 128
+    assert lib.b2x_head_attention_scratch_bytes(ctypes.byref(a), 0) == (parts * rows * ((64 if D <= 64 else 128) * 4 + 8) if parts > 1 else 0)
+    assert lib.b2x_head_attention_launches(ctypes.byref(a), 0) == (0 if B == 0 else 1 + (parts > 1))
+
+
 def test_rows_that_are_not_contiguous_are_copied():
     dump = plan(lambda b: b.rotary([b.transpose(b.arg([2, 4, 64, 8], "bf16"), [0, 1, 3, 2])]))
     assert "copy:call_operand" in dump and "2 steps" in dump

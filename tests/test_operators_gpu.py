@@ -289,6 +289,37 @@ def test_gradients_in_parts(client, sizes, options):
     attention_check(client, **sizes, **options)
 
 
+# the same for the forward pass: parts of a walk over the keys, joined by their maxima
+FORWARD_PARTS = [
+    (dict(B=1, Sq=130, Sk=2500, Hq=2, Hk=1, D=128, dtype="bf16", layout="bhsd"), dict()),
+    (dict(B=1, Sq=513, Sk=513, Hq=1, Hk=1, D=64, dtype="f16", layout="bshd"), dict(causal=True, softcap=20.0)),
+    (dict(B=2, Sq=100, Sk=1537, Hq=2, Hk=2, D=72, dtype="bf16", layout="bshd"), dict(lengths=[1537, 3], softcap=50.0)),
+    (dict(B=1, Sq=300, Sk=1700, Hq=3, Hk=1, D=128, dtype="f16", layout="bhsd"), dict(causal=True, query_offset=1400, slopes=True)),
+    (dict(B=2, Sq=900, Sk=900, Hq=2, Hk=1, D=64, dtype="bf16", layout="bhsd"), dict(documents=7, softcap=30.0)),
+    (dict(B=1, Sq=600, Sk=1200, Hq=2, Hk=2, D=128, dtype="bf16", layout="bshd"), dict(documents=30, causal=True, query_offset=600)),
+    (dict(B=3, Sq=20, Sk=600, Hq=2, Hk=1, D=40, dtype="f16", layout="bhsd"), dict(causal=True, queries_at_end=True, lengths=[600, 0, 7])),
+    (dict(B=1, Sq=140, Sk=700, Hq=1, Hk=1, D=64, dtype="bf16", layout="bhsd"), dict(scale=-0.2)),
+]
+
+
+@pytest.mark.parametrize("sizes,options", FORWARD_PARTS, ids=str)
+def test_attention_in_parts(client, sizes, options):
+    attention_check(client, gradient=False, **sizes, **options)
+
+
+def test_nan_in_parts(client):
+    """A NaN key poisons the queries that see it, whatever part it lies in; what lies behind the length does not show."""
+    q, k, v, do, _, _ = attention_case(1, 200, 1200, 1, 1, 64, "bf16", "bhsd", 5)
+    k[0, 0, 700] = float("nan")
+    lengths = {"lengths": torch.tensor([1100], dtype=torch.int32)}
+    k[0, 0, 1100:] = float("nan")
+    v[0, 0, 1100:] = float("inf")
+    o, lse = attention_run(client, q, k, v, do, lengths, dict(causal=True, query_offset=600), "bf16", "bhsd", gradient=False)
+    sees = torch.arange(200) + 600 >= 700
+    assert torch.equal(torch.isnan(lse.double().cpu())[0, 0], sees) and torch.equal(torch.isnan(o.float().cpu())[0, 0].all(-1), sees)
+    assert torch.isfinite(o.float().cpu()[0, 0][~sees]).all()
+
+
 def test_gradients_in_parts_do_not_differ_from_run_to_run(client):
     q, k, v, do, extra, how = attention_case(1, 1100, 1100, 4, 1, 128, "bf16", "bshd", 9, causal=True)
     first = attention_run(client, q, k, v, do, extra, how, "bf16", "bshd")
