@@ -81,7 +81,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 //     (exchange algorithm of Remez, relative error 6e-7), seven packed instructions for two scores on the FMA pipe;
 //   else: cap - 2 cap q with q = 1 / (1 + e^2x), two special-function instructions per score, right for any score and infinity.
 // The special-function pipe does 16 a clock and SM and has the softmax's exponential to do for every score as it is: with the
-// second way alone a block of 128 x 128 keeps it busy for 3072 cycles where the tensor pipe needs 1024.
+// second way alone a block of 128 x 128 keeps it busy three times as long as the tensor pipe (1024 cycles).
 //
 // Constants are held as pairs, so that packed instructions take them as they are: splitting one value in front of every use cost
 // two moves each.
