@@ -73,13 +73,13 @@ namespace {
 
 // A generic attribute value: enough structure for the properties this subset reads.
 struct Attr {
-  enum Kind { NONE, INT, FLOAT, BOOL, STRING, ARRAY, DENSE, RAW } kind = NONE;
+  enum Kind { NONE, INT, FLOAT, BOOL, STRING, ARRAY, DENSE, DICT, RAW } kind = NONE;
   int64_t i = 0;
   double f = 0;
   bool b = false;
   std::string s;            // STRING, or RAW text of an attribute this reader does not interpret
   std::vector<Attr> items;  // ARRAY
-  std::map<std::string, Attr> entries;  // the dictionary of a backend_config
+  std::map<std::string, Attr> entries;  // DICT: the dictionary of a backend_config
   // DENSE: flattened literals (text tokens) + whether the literal was a single (splat) scalar + the type
   std::vector<std::string> dense_tokens;
   bool dense_splat = false;
@@ -373,11 +373,11 @@ class Parser {
       Attr v;
       if (try_char('=')) {
         skip_ws();
-        if (k == "backend_config" && peek() == '{') { v.kind = Attr::RAW; v.entries = parse_attr_dict(); }
+        if ((k == "backend_config" || k == "mhlo.backend_config") && peek() == '{') { v.kind = Attr::DICT; v.entries = parse_attr_dict(); }
         else v = parse_attr_value();
       }
       else { v.kind = Attr::BOOL; v.b = true; }  // unit attribute
-      d[k] = v;
+      if (!d.emplace(k, v).second) fail(kInvalidArgument, "attribute '" + k + "' is given twice");
     } while (try_char(','));
     expect('}');
     return d;
@@ -703,7 +703,8 @@ class Parser {
     for (auto& kv : d) {
       const std::string& k = kv.first;
       const Attr& a = kv.second;
-      if (k == "value" && op->kind == OpKind::CONSTANT) fill_constant(op, a);
+      if (op->kind == OpKind::CUSTOM_CALL) apply_call_prop(op, k, a);
+      else if (k == "value" && op->kind == OpKind::CONSTANT) fill_constant(op, a);
       else if (k == "iota_dimension") op->iota_dim = a.i;
       else if (k == "broadcast_dimensions" || k == "permutation" || k == "dimensions") op->dims = attr_ints(a);
       else if (k == "comparison_direction") { bool ok; op->cmp_dir = cmp_dir_of(a.s, &ok); if (!ok) fail(kInvalidArgument, "bad comparison_direction"); }
@@ -713,7 +714,6 @@ class Parser {
       else if (k == "channel_handle") op->has_channel = true;
       else if (k == "use_global_device_ids") op->use_global_device_ids = true;
       else if (k == "all_gather_dim") op->iota_dim = a.i;
-      else if (op->kind == OpKind::CUSTOM_CALL) apply_call_prop(op, k, a);
       // precision_config, algorithm, result_accuracy, frontend attributes: accepted and ignored
     }
   }
@@ -730,16 +730,19 @@ class Parser {
     }
     return c;
   }
-  // api_version, has_side_effect and the like say nothing that the operators depend on
+  // What an operator is asked for is read or refused: an option that is passed over would compute another function.
   void apply_call_prop(Op* op, const std::string& k, const Attr& a) {
+    const std::string what = "stablehlo.custom_call: ";
     if (k == "call_target_name") op->call_target = a.s;
-    else if (k == "backend_config") {
+    else if (k == "backend_config" || k == "mhlo.backend_config") {   // the second: the dictionary as older programs spell it
       if (a.kind == Attr::STRING && a.s.empty()) return;
-      if (a.kind != Attr::RAW) fail(kUnimplemented, "stablehlo.custom_call: backend_config must be a dictionary");
+      if (a.kind != Attr::DICT) fail(kUnimplemented, what + k + " must be a dictionary");
+      if (!op->call_attrs.empty()) fail(kUnimplemented, what + "the dictionary is given twice");
       for (auto& e : a.entries) op->call_attrs[e.first] = call_attr(e.second);
-    } else if (k == "called_computations" && !a.items.empty()) fail(kUnimplemented, "stablehlo.custom_call: called computations are not supported");
-    else if (k == "operand_layouts" || k == "result_layouts" || k == "output_operand_aliases") {
-      if (a.kind != Attr::ARRAY || !a.items.empty()) fail(kUnimplemented, "stablehlo.custom_call: " + k + " is not supported");
+    } else if (k == "called_computations" || k == "operand_layouts" || k == "result_layouts" || k == "output_operand_aliases") {
+      if (a.kind != Attr::ARRAY || !a.items.empty()) fail(kUnimplemented, what + k + " is not supported");
+    } else if (k != "api_version" && k != "has_side_effect" && k != "custom_call_schedule" && k != "frontend_attributes" && k != "mhlo.frontend_attributes") {
+      fail(kUnimplemented, what + "attribute '" + k + "' is not supported");
     }
   }
 
@@ -769,7 +772,10 @@ class Parser {
       expect(')');
     }
     skip_ws();
-    if (peek() == '{') { auto more = parse_attr_dict(); for (auto& kv : more) props[kv.first] = kv.second; }
+    if (peek() == '{') {
+      auto more = parse_attr_dict();
+      for (auto& kv : more) if (!props.insert(kv).second) fail(kInvalidArgument, "attribute '" + kv.first + "' is given twice");
+    }
     apply_props(op, props);
     expect(':');
     std::vector<TensorType> ins, outs;
