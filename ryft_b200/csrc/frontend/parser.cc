@@ -337,9 +337,13 @@ class Parser {
     if (isdigit((unsigned char)c) || c == '-' || c == '+') {
       std::string t;
       while (!eof() && (isalnum((unsigned char)peek()) || peek() == '.' || peek() == '-' || peek() == '+')) t.push_back(next());
-      if (t.find_first_of(".eE") != std::string::npos && t.compare(0, 2, "0x") != 0) { a.kind = Attr::FLOAT; a.f = std::stod(t); }
-      else { a.kind = Attr::INT; a.i = std::stoll(t, nullptr, 0); }
-      maybe_skip_type_suffix();
+      const bool hex = t.compare(0, 2, "0x") == 0;
+      if (!hex && t.find_first_of(".eE") != std::string::npos) { a.kind = Attr::FLOAT; a.f = std::stod(t); }
+      else { a.kind = Attr::INT; a.i = hex ? (int64_t)std::stoull(t, nullptr, 16) : std::stoll(t, nullptr, 0); }
+      const std::string type = maybe_skip_type_suffix();
+      if (hex && type == "f64") { a.kind = Attr::FLOAT; memcpy(&a.f, &a.i, 8); }      // the number's bits
+      else if (hex && type == "f32") { const uint32_t bits = (uint32_t)a.i; float f; memcpy(&f, &bits, 4); a.kind = Attr::FLOAT; a.f = f; }
+      else if (hex && (type == "f16" || type == "bf16")) fail(kUnimplemented, "the bits of an " + type + " attribute are not supported");
       return a;
     }
     // bare identifier / type-like attribute (e.g. `f32`, `tensor<...>`): keep raw
@@ -352,16 +356,18 @@ class Parser {
     return a;
   }
   void skip_ws_inline() { while (peek() == ' ' || peek() == '\t') next(); }
-  void maybe_skip_type_suffix() {  // `: i64`, `: tensor<...>`
+  std::string maybe_skip_type_suffix() {  // `: i64`, `: tensor<...>`; the type's name
     skip_ws();
+    std::string type;
     if (peek() == ':' ) {
       size_t save = p_; int save_line = line_;
       next(); skip_ws();
       if (isalpha((unsigned char)peek())) {
-        while (!eof() && ident_char(peek())) next();
+        while (!eof() && ident_char(peek())) type.push_back(next());
         if (peek() == '<') skip_balanced();
       } else { p_ = save; line_ = save_line; }
     }
+    return type;
   }
   // { name = value, name, ... }  or  <{ ... }>
   std::map<std::string, Attr> parse_attr_dict() {

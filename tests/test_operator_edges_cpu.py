@@ -56,3 +56,13 @@ def test_attributes_that_change_nothing_are_accepted(generic, dictionary):
 def test_a_name_given_twice_is_refused():
     plan_refused(attention_text("backend_config = {softcap = 3.0e+01 : f64, softcap = 5.0e+01 : f64}"), "INVALID_ARGUMENT", "twice")
     plan_refused(attention_text("api_version = 4 : i32, backend_config = {}, backend_config = {causal = true}"), "INVALID_ARGUMENT", "twice")
+
+
+def test_numbers_written_as_their_bits_are_read_as_such():
+    # MLIR prints infinities and NaN that way, and accepts it for every number
+    assert "call b2x.attention" in ryft_b200.plan_dump(attention_text("backend_config = {softcap = 0x403E000000000000 : f64, scale = 0x3DCCCCCD : f32}"))
+    plan_refused(attention_text("backend_config = {scale = 0x7FF0000000000000 : f64}"), "INVALID_ARGUMENT", "finite")
+    plan_refused(attention_text("backend_config = {scale = 0x7FC00000 : f32}"), "INVALID_ARGUMENT", "finite")
+    plan_refused(attention_text("backend_config = {softcap = 0xBFF0000000000000 : f64}"), "INVALID_ARGUMENT", "softcap")
+    plan_refused(attention_text("backend_config = {scale = 0x3C00 : f16}"), "UNIMPLEMENTED", "f16")
+    assert "call b2x.attention" in ryft_b200.plan_dump(attention_text("backend_config = {causal = true, query_offset = 0x10 : i64}"))
