@@ -160,7 +160,9 @@ B2X_API int b2x_launch_wide_reduce(const void* in, uint8_t elem, int64_t A, int6
 B2X_API int b2x_launch_wide_gemm(const B2xGemmArgs* host_args, uint8_t out_elem, void* out, b2x_stream_t stream);
 
 /* ---- operators that a program names through stablehlo.custom_call -------------------------------------------------------
- * A tensor of heads has a contiguous last dimension and is addressed by the element strides of its batch, head and token. */
+ * A tensor of heads has a contiguous last dimension and is addressed by the element strides of its batch, head and token.  A call
+ * that lacks memory which it would have to touch, or whose memory is not aligned to its elements (heads of attention: to 16 bytes),
+ * is refused with cudaErrorInvalidValue before anything is launched. */
 typedef struct { int64_t batch, head, token; } B2xHeadStrides;
 
 /* Rotary positions, with the norm of each head in the same pass.  A token at position p turns the pair i of its head's first R

@@ -13,15 +13,22 @@
 namespace b2x {
 namespace {
 
-// rows that 16-byte accesses can reach
+// Rows that 16-byte accesses can reach; where there are none, no memory is asked for.
 bool ha_rows(const void* p, const B2xHeadStrides& s, int64_t B, int64_t H, int64_t S) {
-  return ((uintptr_t)p & 15) == 0 && (B <= 1 || s.batch % 8 == 0) && (H <= 1 || s.head % 8 == 0) && (S <= 1 || s.token % 8 == 0);
+  if (B == 0 || H == 0 || S == 0) return true;
+  return p && ((uintptr_t)p & 15) == 0 && (B <= 1 || s.batch % 8 == 0) && (H <= 1 || s.head % 8 == 0) && (S <= 1 || s.token % 8 == 0);
+}
+bool ha_words(const void* p) { return ((uintptr_t)p & 3) == 0; }   // 32-bit values, or none
+bool ha_sizes(const B2xHeadAttentionArgs* a) {
+  constexpr int64_t most = 1ll << 31;
+  return a->B >= 0 && a->B < most && a->Hq >= 0 && a->Hq < most && a->Hk >= 0 && a->Hk < most && a->B * a->Hq < most && a->B * a->Hk < most && a->Sq >= 0 &&
+         a->Sq < (1ll << 30) && a->Sk >= 0 && a->Sk < (1ll << 30) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0);
 }
 bool ha_valid(const B2xHeadAttentionArgs* a) {
-  return ha_rows(a->q, a->qs, a->B, a->Hq, a->Sq) && ha_rows(a->k, a->ks, a->B, a->Hk, a->Sk) && ha_rows(a->v, a->vs, a->B, a->Hk, a->Sk) &&
-         ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && (a->elem == EL_BF16 || a->elem == EL_F16) && a->D > 0 && a->D % 8 == 0 && a->D <= 128 && a->Hk >= 0 &&
-         (a->Hk > 0 ? a->Hq % a->Hk == 0 : a->Hq == 0) && a->B * a->Hk < (1ll << 31) && (a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e6f)) && std::fabs(a->scale) <= 1e6f &&
-         a->Sq < (1ll << 30) && a->Sk < (1ll << 30) && a->query_offset >= 0 && a->query_offset < (1ll << 30) && (!a->queries_at_end || a->lengths);
+  return ha_sizes(a) && (a->elem == EL_BF16 || a->elem == EL_F16) && ha_rows(a->q, a->qs, a->B, a->Hq, a->Sq) && ha_rows(a->k, a->ks, a->B, a->Hk, a->Sk) &&
+         ha_rows(a->v, a->vs, a->B, a->Hk, a->Sk) && ha_rows(a->o, a->os, a->B, a->Hq, a->Sq) && ha_words(a->lse) && ha_words(a->slopes) && ha_words(a->documents) &&
+         ha_words(a->prefix) && ha_words(a->lengths) && (a->softcap == 0.f || (a->softcap >= 1e-6f && a->softcap <= 1e6f)) && std::fabs(a->scale) <= 1e6f &&
+         a->query_offset >= 0 && a->query_offset < (1ll << 30) && (!a->queries_at_end || a->lengths);
 }
 
 HeadAttn ha_params(const B2xHeadAttentionArgs* a) {
@@ -66,7 +73,7 @@ extern "C" int b2x_launch_head_attention(const B2xHeadAttentionArgs* a, int32_t*
 
 extern "C" int b2x_launch_head_attention_gradient(const B2xHeadAttentionArgs* a, int32_t* status, b2x_stream_t stream) {
   using namespace b2x;
-  if (!ha_valid(a) || !a->lse || (b2x_head_attention_scratch_bytes(a, 1) > 0 && !a->scratch) || ((uintptr_t)a->scratch & 15) != 0) return (int)cudaErrorInvalidValue;
+  if (!ha_valid(a) || (!a->lse && a->B * a->Hq * a->Sq > 0) || (b2x_head_attention_scratch_bytes(a, 1) > 0 && !a->scratch) || ((uintptr_t)a->scratch & 15) != 0) return (int)cudaErrorInvalidValue;
   if (!ha_rows(a->dout, a->dos, a->B, a->Hq, a->Sq) || !ha_rows(a->dq, a->dqs, a->B, a->Hq, a->Sq) || !ha_rows(a->dk, a->dks, a->B, a->Hk, a->Sk) ||
       !ha_rows(a->dv, a->dvs, a->B, a->Hk, a->Sk)) return (int)cudaErrorInvalidValue;
   return ha_launch_gradient(ha_params(a), a->elem, a->scratch, status, (cudaStream_t)stream);

@@ -494,9 +494,22 @@ __global__ void __launch_bounds__(1024) k_rotary_fold(const float* partial, floa
 
 int rot_elem_size(uint8_t e) { return e == EL_F32 ? 4 : 2; }
 
-bool rot_valid(const B2xRotaryArgs* a) {
-  return (a->elem == EL_BF16 || a->elem == EL_F16 || a->elem == EL_F32) && (a->weight_elem == EL_F32 || a->weight_elem == a->elem || !a->norm) &&
-         (a->n == 1 || a->n == 2) && a->D <= 256 && a->R >= 0 && a->R <= a->D && a->R % 2 == 0 && a->B * a->S < (1ll << 31);
+bool rot_valid(const B2xRotaryArgs* a, bool gradient) {
+  constexpr int64_t most = 1ll << 31;
+  const int64_t es = rot_elem_size(a->elem);
+  auto at = [](const void* p, int64_t size) { return p && (uintptr_t)p % (size_t)size == 0; };
+  if (!((a->elem == EL_BF16 || a->elem == EL_F16 || a->elem == EL_F32) && (a->weight_elem == EL_F32 || a->weight_elem == a->elem || !a->norm) && (a->n == 1 || a->n == 2) &&
+        a->B >= 0 && a->B < most && a->S >= 0 && a->S < most && a->B * a->S < most && a->D >= 0 && a->D <= 256 && a->R >= 0 && a->R <= a->D && a->R % 2 == 0)) return false;
+  if ((uintptr_t)a->positions % 4 != 0) return false;
+  bool any = false;
+  for (int i = 0; i < a->n; i++) {
+    if (a->heads[i] < 0 || a->heads[i] >= (1 << 20)) return false;
+    if (a->D > 0 && a->norm && (!at(a->weight[i], a->weight_elem == EL_F32 ? 4 : 2) || (gradient && !at(a->dweight[i], 4)))) return false;
+    if (a->B * a->S * a->heads[i] * a->D == 0) continue;
+    any = true;
+    if (!at(a->y[i], es) || ((!gradient || a->norm) && !at(a->x[i], es)) || (gradient && !at(a->dy[i], es))) return false;
+  }
+  return (!any || a->R == 0 || at(a->turns, 8)) && (!gradient || !a->norm || a->D == 0 || at(a->scratch, 4));
 }
 
 // Elements of a piece: 16 bytes where rows, pieces and partners start on that boundary, else 8 for 16-bit types, else one element.
@@ -589,7 +602,7 @@ int launch_rot(const B2xRotaryArgs* a, const RotaryParams& p, int V, bool norm_g
 
 extern "C" int b2x_launch_rotary(const B2xRotaryArgs* a, b2x_stream_t stream) {
   using namespace b2x;
-  if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
+  if (!rot_valid(a, false)) return (int)cudaErrorInvalidValue;
   if (a->D == 0) return 0;
   const int V = rot_piece(a, false);
   const RotaryParams p = rot_params(a, V, false);
@@ -610,7 +623,7 @@ extern "C" int b2x_rotary_launches(const B2xRotaryArgs* a, int gradient) {
 
 extern "C" int b2x_launch_rotary_gradient(const B2xRotaryArgs* a, b2x_stream_t stream) {
   using namespace b2x;
-  if (!rot_valid(a)) return (int)cudaErrorInvalidValue;
+  if (!rot_valid(a, true)) return (int)cudaErrorInvalidValue;
   if (a->D == 0) return 0;
   const int V = rot_piece(a, true);
   RotaryParams p = rot_params(a, V, a->norm);
@@ -621,7 +634,6 @@ extern "C" int b2x_launch_rotary_gradient(const B2xRotaryArgs* a, b2x_stream_t s
     if (p.tokens == 0 || p.heads[0] + p.heads[1] == 0) return 0;
     return launch_rot(a, p, V, false, (cudaStream_t)stream);
   }
-  if (!a->scratch) return (int)cudaErrorInvalidValue;
   p.partial = (float*)a->scratch;
   const int rows = p.tokens > 0 ? rot_gradient_ctas(p) : 0;
   if (rows > 0) {

@@ -1,8 +1,10 @@
 """The named operators at the edges of what is accepted, without a GPU: spellings of their options, and what the entry points refuse."""
+import ctypes
+
 import pytest
 
 import ryft_b200
-from ryft_b200 import pjrt
+from ryft_b200 import kernels, pjrt
 
 T = "tensor<1x2x8x64xbf16>"
 
@@ -66,3 +68,77 @@ def test_numbers_written_as_their_bits_are_read_as_such():
     plan_refused(attention_text("backend_config = {softcap = 0xBFF0000000000000 : f64}"), "INVALID_ARGUMENT", "softcap")
     plan_refused(attention_text("backend_config = {scale = 0x3C00 : f16}"), "UNIMPLEMENTED", "f16")
     assert "call b2x.attention" in ryft_b200.plan_dump(attention_text("backend_config = {causal = true, query_offset = 0x10 : i64}"))
+
+
+# ---- what the kernels' entry points refuse before they touch anything (cudaErrorInvalidValue, without a GPU) -----------------------
+
+REFUSED = 1
+SOMEWHERE = 1 << 12     # stands for memory: a call that is refused does not look at it
+
+
+def attention_call(**change):
+    a = kernels.HeadAttentionArgs(elem=kernels.EL_BF16, causal=1, B=2, Hq=4, Hk=2, Sq=32, Sk=48, D=64, scale=0.125)
+    for n in ("q", "k", "v", "o", "dout", "dq", "dk", "dv", "lse", "scratch"):
+        setattr(a, n, SOMEWHERE)
+    for n, h, s in (("qs", 4, 32), ("os", 4, 32), ("dos", 4, 32), ("dqs", 4, 32), ("ks", 2, 48), ("vs", 2, 48), ("dks", 2, 48), ("dvs", 2, 48)):
+        setattr(a, n, kernels.HeadStrides(h * s * 64, s * 64, 64))
+    for n, x in change.items():
+        setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("gradient,change", [(g, c) for g in (False, True) for c in (
+    dict(q=None), dict(k=None), dict(v=None), dict(o=None), dict(lse=SOMEWHERE + 2), dict(slopes=SOMEWHERE + 1), dict(documents=SOMEWHERE + 2),
+    dict(prefix=SOMEWHERE + 3), dict(lengths=SOMEWHERE + 2), dict(B=-1), dict(Sq=-1), dict(Sk=-128), dict(Hq=-4), dict(Hk=-2), dict(Hq=0, Hk=-2),
+    dict(B=1 << 40), dict(Hq=1 << 33, Hk=1), dict(scale=float("nan")), dict(softcap=float("nan")))
+] + [(True, c) for c in (dict(dout=None), dict(dq=None), dict(dk=None), dict(dv=None), dict(lse=None))], ids=str)
+@pytest.mark.parametrize("Sq", [1, 32])
+def test_attention_without_its_memory_is_refused(gradient, change, Sq):
+    lib = kernels.load()
+    a = attention_call(**{"Sq": Sq, **change})
+    before = lib.b2x_kernel_launch_count()
+    f = lib.b2x_launch_head_attention_gradient if gradient else lib.b2x_launch_head_attention
+    assert f(ctypes.byref(a), None, None) == REFUSED and lib.b2x_kernel_launch_count() == before
+
+
+@pytest.mark.parametrize("change", [dict(B=0), dict(Hq=0, Hk=0), dict(B=0, q=None, k=None, v=None, o=None), dict(Sq=0, q=None, o=None)], ids=str)
+def test_attention_of_nothing_needs_no_memory(change):
+    lib = kernels.load()
+    assert lib.b2x_launch_head_attention(ctypes.byref(attention_call(**change)), None, None) == 0
+
+
+def rotary_call(elem, **change):
+    a = kernels.RotaryArgs(elem=elem, weight_elem=kernels.EL_F32, n=2, norm=1, B=2, S=8, D=64, R=64, epsilon=1e-6)
+    for i in range(2):
+        a.heads[i] = 3
+        for n in ("x", "y", "dy"):
+            getattr(a, n)[i] = SOMEWHERE
+            getattr(a, n + "s")[i] = kernels.HeadStrides(3 * 8 * 64, 8 * 64, 64)
+        a.weight[i] = a.dweight[i] = SOMEWHERE
+    a.turns = a.scratch = SOMEWHERE
+    for n, x in change.items():
+        if isinstance(x, tuple):
+            getattr(a, n)[x[0]] = x[1]
+        else:
+            setattr(a, n, x)
+    return a
+
+
+@pytest.mark.parametrize("gradient,change", [(g, c) for g in (False, True) for c in (
+    dict(x=(0, None)), dict(x=(1, SOMEWHERE + 1)), dict(y=(1, None)), dict(y=(0, SOMEWHERE + 1)), dict(weight=(1, None)), dict(weight=(0, SOMEWHERE + 2)),
+    dict(turns=None), dict(turns=SOMEWHERE + 4), dict(positions=SOMEWHERE + 2), dict(B=-1), dict(S=-8), dict(B=1 << 40, S=1 << 40), dict(D=-64, R=0),
+    dict(heads=(0, -1)), dict(heads=(1, 1 << 40)))
+] + [(True, c) for c in (dict(dy=(1, None)), dict(dy=(0, SOMEWHERE + 1)), dict(dweight=(1, None)), dict(dweight=(0, SOMEWHERE + 2)), dict(scratch=None),
+                         dict(scratch=SOMEWHERE + 2))], ids=str)
+@pytest.mark.parametrize("elem", [kernels.EL_BF16, kernels.EL_F32])
+def test_rotary_without_its_memory_is_refused(gradient, change, elem):
+    lib = kernels.load()
+    before = lib.b2x_kernel_launch_count()
+    f = lib.b2x_launch_rotary_gradient if gradient else lib.b2x_launch_rotary
+    assert f(ctypes.byref(rotary_call(elem, **change)), None) == REFUSED and lib.b2x_kernel_launch_count() == before
+
+
+def test_rotary_of_nothing_needs_no_memory():
+    lib = kernels.load()
+    for change in (dict(D=0, R=0), dict(B=0, x=(0, None), turns=None)):
+        assert lib.b2x_launch_rotary(ctypes.byref(rotary_call(kernels.EL_BF16, **change)), None) == 0
