@@ -733,8 +733,10 @@ int ha_gradient_launches(const B2xHeadAttentionArgs* a) {
 }
 
 // scratch: ha_gradient_scratch
-int ha_launch_gradient(const HeadAttn& a, int elem, void* scratch, int32_t* status, cudaStream_t stream) {
-  if (a.B == 0 || a.Hq == 0) return 0;
+int ha_launch_gradient(const HeadAttn& call, int elem, void* scratch, int32_t* status, cudaStream_t stream) {
+  HeadAttn a = call;
+  if (a.B == 0 || a.Hk == 0) return 0;
+  if (a.Hq == 0) { a.Hq = a.Hk; a.group = 1; a.Sq = 0; }   // keys that no head reads: gradients of zero, as without queries
   GradParams p{};
   p.a = a;
   p.rows = grad_rows(a.Sq);
