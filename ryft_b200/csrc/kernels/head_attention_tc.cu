@@ -434,7 +434,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (hi != -INFINITY) {
             const uint64_t x = mul2(splat2(hi), p.cap.in2);
             uint32_t v0, v1;
-            unpack2(small ? cap_small(p.cap, x) : fma2(cap_rest(x), p.cap.twice2, p.cap.out2), v0, v1);
+            unpack2(small ? cap_small(p.cap, x) : cap_any(p.cap, x), v0, v1);
             mx = __uint_as_float(v0);
           }
           if (hi != hi || lo != lo) { poisoned = true; mx = 0.f; }
@@ -462,7 +462,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 const uint64_t x = mul2(pack2(r[2 * h2], r[2 * h2 + 1]), p.cap.in2);
                 uint64_t y;
                 if constexpr (decltype(SMALL)::value) y = cap_small_plus(p.cap, x, mn2);
-                else y = add2(fma2(cap_rest(x), p.cap.twice2, p.cap.out2), mn2);
+                else y = add2(cap_any(p.cap, x), mn2);
                 uint32_t t0, t1;
                 unpack2(y, t0, t1);
                 if constexpr (decltype(MASK)::value) {
@@ -497,11 +497,18 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (lane == 0) mbar_arrive(bar_se);
         sc++;
         if (CAP && p.cap.cap > 0.f) {
+          const float largest = max3(max3(ha_largest(r[0]), ha_largest(r[1]), 0.f), ha_largest(r[2]), ha_largest(r[3]));
+          if (__all_sync(0xffffffffu, largest <= p.cap.small)) {
 #pragma unroll
-          for (int c = 0; c < 4; c++)
+            for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-              unpack2(fma2(cap_rest(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), p.cap.twice2, p.cap.out2), r[c][2 * i], r[c][2 * i + 1]);
+              for (int i = 0; i < 16; i++) unpack2(cap_small(p.cap, mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), r[c][2 * i], r[c][2 * i + 1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+#pragma unroll
+              for (int i = 0; i < 16; i++) unpack2(cap_any(p.cap, mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.cap.in2)), r[c][2 * i], r[c][2 * i + 1]);
+          }
         } else if (MODE == TILE_ANY && !p.a.slopes) {
 #pragma unroll
           for (int c = 0; c < 4; c++)

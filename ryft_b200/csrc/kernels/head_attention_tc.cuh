@@ -79,7 +79,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // softcap * tanh(x) in log2 units, x = scale / softcap times the product.  Two ways:
 //   |x| <= 0.75 (scores up to 0.75 caps, the usual case): an odd polynomial of degree 9, the minimax fit of tanh(x) / x in x^2
 //     (exchange algorithm of Remez, relative error 6e-7), seven packed instructions for two scores on the FMA pipe;
-//   else: cap - 2 cap q with q = 1 / (1 + e^2x), two special-function instructions per score, right for any score and infinity.
+//   beyond: cap - 2 cap q with q = 1 / (1 + e^2x), two special-function instructions per score, right for infinities, too.  Its error
+//     goes with the cap, not with the score (2e-7 caps), so that it is for scores of the cap's size only.
+// Where all scores of a warp's block are small only the polynomial is worked out; else both, and each score takes its own.
 // The special-function pipe does 16 a clock and SM and has the softmax's exponential to do for every score as it is: with the
 // second way alone a block of 128 x 128 keeps it busy three times as long as the tensor pipe (1024 cycles).
 //
@@ -103,12 +105,17 @@ inline HeadCap ha_cap(float softcap, float scale) {
   if (!(softcap > 0.f)) return h;
   h.cap = softcap * kLog2e;
   h.in2 = ha_pair(scale / softcap);
-  h.small = scale != 0.f ? 0.75f * softcap / fabsf(scale) : 0.f;
+  h.small = scale != 0.f ? fminf(0.75f * softcap / fabsf(scale), 3e38f) : 0.f;   // infinite products are beyond it
   h.c0 = ha_pair(0.99999946f * h.cap); h.c1 = ha_pair(-0.3332825f * h.cap); h.c2 = ha_pair(0.13258983f * h.cap);
   h.c3 = ha_pair(-0.0500563f * h.cap); h.c4 = ha_pair(0.012929632f * h.cap);
   h.back2 = ha_pair(-1.0f / (h.cap * h.cap));
   h.out2 = ha_pair(h.cap); h.twice2 = ha_pair(-2.0f * h.cap);
   return h;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 // cap * tanh(x) of a pair, and the same plus something
 __device__ __forceinline__ uint64_t cap_share(const HeadCap& h, uint64_t x) {
@@ -127,11 +134,15 @@ __device__ __forceinline__ uint64_t cap_rest(uint64_t x) {
   unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), splat2(1.f)), a0, a1);
   return pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
 }
-__device__ __forceinline__ float min3(float a, float b, float c) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
+// cap * tanh(x) of a pair of any size: of the polynomial's and the other, each x takes its own
+__device__ __forceinline__ uint64_t cap_choose(const HeadCap& h, uint64_t x, uint64_t q) {
+  uint32_t x0, x1, s0, s1, l0, l1;
+  unpack2(x, x0, x1);
+  unpack2(cap_small(h, x), s0, s1);
+  unpack2(fma2(q, h.twice2, h.out2), l0, l1);
+  return pack2(fabsf(__uint_as_float(x0)) <= 0.75f ? s0 : l0, fabsf(__uint_as_float(x1)) <= 0.75f ? s1 : l1);
 }
+__device__ __forceinline__ uint64_t cap_any(const HeadCap& h, uint64_t x) { return cap_choose(h, x, cap_rest(x)); }
 // Waits for a TMEM load; naming its registers keeps their uses behind the wait.
 __device__ __forceinline__ void ha_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"

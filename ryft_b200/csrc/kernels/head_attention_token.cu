@@ -27,7 +27,7 @@ struct TokenParams {
   int32_t tiles;               // of all key heads and sequences
   int32_t chunk, chunks;       // keys per CTA; CTAs per tile
   float mult;                  // scale * log2(e)
-  float cap, cap_in;           // cap * log2(e) and the exponent 2 * scale / cap * log2(e); 0: none
+  HeadCap cap;
   float* part_o;               // [tile][chunk][16][D]
   float2* part_ml;             // [tile][chunk][16]: maximum (log2 units) and sum
 };
@@ -172,11 +172,22 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
           token_mma<EL>(s[m], qf[2 * q + 1], f[2], f[3]);
         }
       // element x of s[m]: row x >> 1, key k0 + 8 m + 2 c + (x & 1)
-      if (p.cap > 0.f) {
+      if (p.cap.cap > 0.f) {
+        float largest = 0.f;
 #pragma unroll
         for (int m = 0; m < 2; m++)
 #pragma unroll
-          for (int x = 0; x < 4; x++) s[m][x] = fmaf(-2.f * p.cap, fast_rcp(1.f + fast_exp2(s[m][x] * p.cap_in)), p.cap);
+          for (int x = 0; x < 4; x += 2) largest = max3(largest, fabsf(s[m][x]), fabsf(s[m][x + 1]));
+        const bool small = __all_sync(0xffffffffu, largest <= p.cap.small);
+#pragma unroll
+        for (int m = 0; m < 2; m++)
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {
+            const uint64_t v = mul2(pack2(__float_as_uint(s[m][x]), __float_as_uint(s[m][x + 1])), p.cap.in2);
+            uint32_t a, b;
+            unpack2(small ? cap_small(p.cap, v) : cap_any(p.cap, v), a, b);
+            s[m][x] = __uint_as_float(a); s[m][x + 1] = __uint_as_float(b);
+          }
       } else {
 #pragma unroll
         for (int m = 0; m < 2; m++)
@@ -403,8 +414,7 @@ int ha_launch_token(const HeadAttn& a, int elem, void* scratch, cudaStream_t str
   p.part_o = (float*)scratch;
   p.part_ml = (float2*)(p.part_o + (int64_t)a.B * a.Hk * p.row_tiles * p.chunks * TOKEN_ROWS * D);
   p.mult = a.scale * kLog2e;
-  p.cap = a.softcap > 0.f ? a.softcap * kLog2e : 0.f;
-  p.cap_in = a.softcap > 0.f ? 2.0f * a.scale / a.softcap * kLog2e : 0.f;
+  p.cap = ha_cap(a.softcap, a.scale);
   if (D == 64) return elem == EL_BF16 ? launch_token<64, EL_BF16>(p, stream) : launch_token<64, EL_F16>(p, stream);
   return elem == EL_BF16 ? launch_token<128, EL_BF16>(p, stream) : launch_token<128, EL_F16>(p, stream);
 }

@@ -41,3 +41,50 @@ def test_key_heads_without_query_heads_have_gradients_of_zero(lib, documents):
     assert rc == 0 and not status.item()
     assert lib.b2x_kernel_launch_count() - before == lib.b2x_head_attention_launches(C.byref(a), 1)
     assert not grads[2].any() and not grads[3].any()
+
+
+# ---- caps over the whole accepted range ------------------------------------------------------------------------------------------
+
+CAPS = [
+    dict(B=2, Sq=1, Sk=300, Hq=4, Hk=2, D=64, dtype="f16", layout="bhsd"),
+    dict(B=1, Sq=5, Sk=700, Hq=2, Hk=1, D=128, dtype="bf16", layout="bshd"),
+    dict(B=1, Sq=150, Sk=150, Hq=2, Hk=1, D=128, dtype="f16", layout="bshd"),
+]
+
+
+@pytest.mark.parametrize("softcap", [1e-6, 1e-3, 1e3, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("options", [dict(), dict(slopes=True), dict(scale=-0.2), dict(causal=True)], ids=str)
+@pytest.mark.parametrize("sizes", CAPS, ids=str)
+def test_caps_of_any_size(client, sizes, options, softcap):
+    """A cap far above the scores changes hardly anything: its error must go with the score, not with the cap.
+
+    Far below them the gradient is a matter of chance in 32 bits: an error of a product, 2^-24 of the sum of its terms' sizes (some 100
+    here, times the scale: 1e-6), is 1e-3 of a cap of 1e-3 and 1 of a cap of 1e-6, and e^-2x changes by twice that.  There o and the log sums count."""
+    how, sizes = dict(options), dict(sizes)
+    dtype, layout = sizes["dtype"], sizes["layout"]
+    gradient = softcap >= 1
+    q, k, v, do, extra, how = program.attention_case(**sizes, seed=7, softcap=softcap, **how)
+    got = program.attention_run(client, q, k, v, do, extra, how, dtype, layout, gradient)
+    scale = how.pop("scale", sizes["D"] ** -0.5)
+    # the bounds are for scales that are positive: the same scores from queries of the other sign
+    sign = -1.0 if scale < 0 else 1.0
+    want = ref.attention(sign * q, k, v, dtype, layout, abs(scale), do=do if gradient else None, **extra, **how)
+    for name, x in zip(("o", "lse", "dq", "dk", "dv"), got):
+        program.within(x, sign * want[name][0] if name == "dq" else want[name][0], want[name][1], name)
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("Sq", [2, 150])
+def test_one_large_score_leaves_the_others_as_they_are(client, Sq, slopes):
+    """One query whose scores go beyond its cap of 1e5, next to queries whose scores are a few units."""
+    q, k, v, do, extra, how = program.attention_case(1, Sq, 200, 2, 1, 64, "f16", "bhsd", 5, softcap=1e5, slopes=slopes)
+    q[:, :, 1] = (q[:, :, 1].float() * 2000).half()
+    how["scale"] = 8.0
+    q[:, :, 0] = (q[:, :, 0].float() / 64).half()
+    q[:, :, 2:] = (q[:, :, 2:].float() / 64).half()
+    got = program.attention_run(client, q, k, v, do, extra, how, "f16", "bhsd")
+    scale = how.pop("scale")
+    want = ref.attention(q, k, v, "f16", "bhsd", scale, do=do, **extra, **how)
+    others = [i for i in range(Sq) if i != 1]
+    for name, x in (("o", got[0]), ("lse", got[1]), ("dq", got[2])):
+        program.within(x[:, :, others], want[name][0][:, :, others], want[name][1].expand_as(want[name][0])[:, :, others], name)
