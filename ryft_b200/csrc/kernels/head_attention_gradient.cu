@@ -75,9 +75,11 @@ __device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (
       bend2 = fma2(mul2(t2, t2), p.cap.back2, splat2(1.f));
       x2 = add2(t2, nl(i));
     } else if constexpr (CAP == 2) {
-      // the derivative 1 - tanh^2 = 4 q (1 - q)
-      const uint64_t c2 = mul2(s2, p.cap.in2), q2 = cap_rest(c2);
-      bend2 = mul2(mul2(q2, splat2(4.f)), fma2(q2, splat2(-1.f), splat2(1.f)));
+      const uint64_t c2 = mul2(s2, p.cap.in2);
+      uint64_t e2;
+      const uint64_t q2 = cap_rest<true>(c2, e2);
+      // 1 - tanh^2 = 4 e^2x q^2
+      bend2 = mul2(mul2(mul2(e2, q2), q2), splat2(4.f));
       x2 = add2(cap_choose(p.cap, c2, q2), nl(i));
     } else {
       x2 = fma2(s2, p.in2, nl(i));

@@ -127,11 +127,14 @@ __device__ __forceinline__ uint64_t cap_share(const HeadCap& h, uint64_t x) {
 }
 __device__ __forceinline__ uint64_t cap_small(const HeadCap& h, uint64_t x) { return mul2(x, cap_share(h, x)); }
 __device__ __forceinline__ uint64_t cap_small_plus(const HeadCap& h, uint64_t x, uint64_t plus) { return fma2(x, cap_share(h, x), plus); }
-// q = 1 / (1 + e^2x)
-__device__ __forceinline__ uint64_t cap_rest(uint64_t x) {
+// e^2x and q = 1 / (1 + e^2x); with BOUNDED e^2x stays finite (2^126 at most), as products with q need it
+template <bool BOUNDED> __device__ __forceinline__ uint64_t cap_rest(uint64_t x, uint64_t& e2) {
   uint32_t a0, a1;
   unpack2(mul2(x, splat2(2.f * kLog2e)), a0, a1);
-  unpack2(add2(pack2(__float_as_uint(fast_exp2(__uint_as_float(a0))), __float_as_uint(fast_exp2(__uint_as_float(a1)))), splat2(1.f)), a0, a1);
+  float x0 = __uint_as_float(a0), x1 = __uint_as_float(a1);
+  if constexpr (BOUNDED) { x0 = min3(x0, 126.f, 126.f); x1 = min3(x1, 126.f, 126.f); }
+  e2 = pack2(__float_as_uint(fast_exp2(x0)), __float_as_uint(fast_exp2(x1)));
+  unpack2(add2(e2, splat2(1.f)), a0, a1);
   return pack2(__float_as_uint(fast_rcp(__uint_as_float(a0))), __float_as_uint(fast_rcp(__uint_as_float(a1))));
 }
 // cap * tanh(x) of a pair of any size: of the polynomial's and the other, each x takes its own
@@ -142,7 +145,11 @@ __device__ __forceinline__ uint64_t cap_choose(const HeadCap& h, uint64_t x, uin
   unpack2(fma2(q, h.twice2, h.out2), l0, l1);
   return pack2(fabsf(__uint_as_float(x0)) <= 0.75f ? s0 : l0, fabsf(__uint_as_float(x1)) <= 0.75f ? s1 : l1);
 }
-__device__ __forceinline__ uint64_t cap_any(const HeadCap& h, uint64_t x) { return cap_choose(h, x, cap_rest(x)); }
+__device__ __forceinline__ uint64_t cap_any(const HeadCap& h, uint64_t x) {
+  uint64_t e2;
+  const uint64_t q = cap_rest<false>(x, e2);
+  return cap_choose(h, x, q);
+}
 // Waits for a TMEM load; naming its registers keeps their uses behind the wait.
 __device__ __forceinline__ void ha_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"

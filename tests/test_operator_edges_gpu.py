@@ -88,3 +88,19 @@ def test_one_large_score_leaves_the_others_as_they_are(client, Sq, slopes):
     others = [i for i in range(Sq) if i != 1]
     for name, x in (("o", got[0]), ("lse", got[1]), ("dq", got[2])):
         program.within(x[:, :, others], want[name][0][:, :, others], want[name][1].expand_as(want[name][0])[:, :, others], name)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_far_beyond_the_cap_keep_the_slope_of_it(client, sign):
+    """1 - tanh^2 of scores of 3 to 8 caps, on either side of zero: 2e-2 down to 5e-7, each as good as the score's own rounding."""
+    B, H, S, D, cap = 1, 2, 70, 64, 2.0
+    q, k, v, do, extra, how = program.attention_case(B, S, S, H, H, D, "f16", "bhsd", 3, softcap=cap)
+    q, k = torch.zeros_like(q), torch.zeros_like(k)
+    q[..., 0] = sign
+    k[..., 0] = torch.linspace(6.0, 16.0, S)
+    q[..., 1:9], k[..., 1:9] = torch.randn(B, H, S, 8).half() / 16, torch.randn(B, H, S, 8).half() / 16
+    do = (do.float() * 4096).half()
+    got = program.attention_run(client, q, k, v, do, extra, {**how, "scale": 1.0}, "f16", "bhsd")
+    want = ref.attention(q, k, v, "f16", "bhsd", 1.0, do=do, **extra, **how)
+    for name, x in zip(("o", "lse", "dq", "dk", "dv"), got):
+        program.within(x, *want[name], name)
