@@ -431,7 +431,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           const bool small = __all_sync(0xffffffffu, hi <= p.cap.small && lo >= -p.cap.small);
           float mx = -INFINITY;
-          if (hi != -INFINITY) {
+          if (!need_mask || (seen[0] | seen[1] | seen[2] | seen[3]) != 0) {   // products of -inf are scores of -cap
             const uint64_t x = mul2(splat2(hi), p.cap.in2);
             uint32_t v0, v1;
             unpack2(small ? cap_small(p.cap, x) : cap_any(p.cap, x), v0, v1);

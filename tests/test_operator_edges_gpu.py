@@ -104,3 +104,17 @@ def test_scores_far_beyond_the_cap_keep_the_slope_of_it(client, sign):
     want = ref.attention(q, k, v, "f16", "bhsd", 1.0, do=do, **extra, **how)
     for name, x in zip(("o", "lse", "dq", "dk", "dv"), got):
         program.within(x, *want[name], name)
+
+
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("Sq", [1, 40])
+def test_products_beyond_f32_are_capped(client, Sq, slopes):
+    """Products of -2e77 are infinite in f32 and -softcap as a score: every key weighs the same."""
+    q = torch.full((1, 2, Sq, 64), 1e38).bfloat16()
+    k = torch.full((1, 1, 150, 64), -1e38).bfloat16()
+    v = program.normal(1, [1, 1, 150, 64])[0].bfloat16()
+    extra = {"slopes": torch.zeros(2)} if slopes else {}
+    o, lse = program.attention_run(client, q, k, v, None, extra, {"softcap": 300.0}, "bf16", "bhsd", gradient=False)
+    want = ref.attention(q, k, v, "bf16", "bhsd", 0.125, softcap=300.0, **extra)
+    program.within(o, *want["o"], "o")
+    program.within(lse, *want["lse"], "lse")
