@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
       for (int k = 0; k < TOKEN_WARPS; k++) rm = fmaxf(rm, sml[k][orow].x);
 #pragma unroll
       for (int k = 0; k < TOKEN_WARPS; k++) { const float2 v = sml[k][orow]; rl += v.x == -INFINITY ? v.y : v.y * fast_exp2(v.x - rm); }
-      const float inv = p.chunks > 1 ? 1.f : rl == 0.f ? 0.f : 1.0f / rl;
+      const float inv = 1.0f / rl;
       float* part = p.part_o + (((int64_t)tile * p.chunks + chunk) * TOKEN_ROWS + orow) * D;
       char* out = p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)o.h * p.a.os.head + (int64_t)o.i * p.a.os.token);
       for (int d = (threadIdx.x & 7) * 2; d < p.a.D; d += 16) {
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
 #pragma unroll
         for (int k = 0; k < TOKEN_WARPS; k++) { const float2 v = *(const float2*)&so[k][orow][d]; v0 += v.x; v1 += v.y; }
         if (p.chunks > 1) *(float2*)(part + d) = make_float2(v0, v1);
-        else *(uint32_t*)(out + 2 * d) = ha_pack<EL>(rl != rl ? rl : v0 * inv, rl != rl ? rl : v1 * inv);
+        else *(uint32_t*)(out + 2 * d) = rl == 0.f ? 0u : ha_pack<EL>(rl != rl ? rl : v0 * inv, rl != rl ? rl : v1 * inv);   // sees nothing: 0, whatever was multiplied
       }
       if ((threadIdx.x & 7) == 0) {
         if (p.chunks > 1) p.part_ml[((int64_t)tile * p.chunks + chunk) * TOKEN_ROWS + orow] = make_float2(rm, rl);
@@ -341,8 +341,7 @@ __global__ void __launch_bounds__(128) k_attention_token_join(const __grid_const
 #pragma unroll
       for (int x = 0; x < 4; x++) v[x] = fmaf(ld_global(src + (int64_t)(k + x) * TOKEN_ROWS * D), weight[k + x], v[x]);
     for (; k < n; k++) v[0] = fmaf(ld_global(src + (int64_t)k * TOKEN_ROWS * D), weight[k], v[0]);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-    const float f = l != l ? l : ((v[0] + v[1]) + (v[2] + v[3])) * inv;
+    const float f = l == 0.f ? 0.f : l != l ? l : ((v[0] + v[1]) + (v[2] + v[3])) * (1.0f / l);
     *(uint16_t*)(p.a.o + 2 * ((int64_t)b * p.a.os.batch + (int64_t)o.h * p.a.os.head + (int64_t)o.i * p.a.os.token + tid)) = (uint16_t)(ha_pack<EL>(f, 0.f) & 0xffffu);
   }
   if (tid == 0 && p.a.lse) p.a.lse[((int64_t)b * p.a.Hq + o.h) * p.a.Sq + o.i] = l == 0.f ? -INFINITY : (m + fast_log2(l)) * 0.6931471805599453f;

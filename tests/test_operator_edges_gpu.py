@@ -118,3 +118,16 @@ def test_products_beyond_f32_are_capped(client, Sq, slopes):
     want = ref.attention(q, k, v, "bf16", "bhsd", 0.125, softcap=300.0, **extra)
     program.within(o, *want["o"], "o")
     program.within(lse, *want["lse"], "lse")
+
+
+# ---- rows that see nothing, far distances ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("Sk", [40, 700])
+def test_a_query_that_sees_nothing_yields_0_whatever_others_see(client, Sk):
+    """Queries in front of the first token see nothing; the value that the last query sees may be infinite or not a number."""
+    q, k, v, do, _, _ = program.attention_case(1, 3, Sk, 2, 1, 64, "bf16", "bhsd", 2)
+    v[0, 0, 0, :5], v[0, 0, 0, 5:9] = float("inf"), float("nan")
+    extra = {"lengths": torch.tensor([1], dtype=torch.int32)}
+    o, lse = program.attention_run(client, q, k, v, do, extra, dict(causal=True, queries_at_end=True), "bf16", "bhsd", gradient=False)
+    assert not o[:, :, :2].any() and torch.equal(lse[:, :, :2], torch.full((1, 2, 2), -float("inf")))
+    assert torch.isinf(o[:, :, 2, :5]).all() and torch.isnan(o[:, :, 2, 5:9]).all() and torch.isfinite(o[:, :, 2, 9:]).all()
