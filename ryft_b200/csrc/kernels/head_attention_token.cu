@@ -113,8 +113,8 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
 
     // this lane's rows r and r + 8
     TokenRow row[2];
-    int lim[2], doc[2];
-    float slope[2], pos[2];
+    int lim[2], doc[2], pos[2];
+    float slope[2];
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
         else if (row[x].there) lim[x] = 0;
       }
       slope[x] = p.a.slopes ? ld_global(p.a.slopes + row[x].h) * kLog2e : 0.f;
-      pos[x] = (float)at;
+      pos[x] = at;
       const char* q = p.a.q + 2 * ((int64_t)b * p.a.qs.batch + (int64_t)row[x].h * p.a.qs.head + (int64_t)row[x].i * p.a.qs.token);
 #pragma unroll
       for (int k = 0; k < D / 16; k++)
@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(TOKEN_WARPS * 32, 2) k_attention_token(const _
           for (int x = 0; x < 4; x++) {
             const int key = k0 + 8 * m + 2 * c + (x & 1), w = x >> 1;
             float v = s[m][x];
-            if (p.a.slopes) v = fmaf(fabsf(pos[w] - (float)key), -slope[w], v);
+            if (p.a.slopes) v = fmaf(fabsf((float)(pos[w] - key)), -slope[w], v);
             bool see = key < lim[w] && key < k_end;
             if (p.a.documents) see = see && (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + min(key, p.a.Sk - 1)) == doc[w];
             s[m][x] = see ? v : -INFINITY;

@@ -131,3 +131,19 @@ def test_a_query_that_sees_nothing_yields_0_whatever_others_see(client, Sk):
     o, lse = program.attention_run(client, q, k, v, do, extra, dict(causal=True, queries_at_end=True), "bf16", "bhsd", gradient=False)
     assert not o[:, :, :2].any() and torch.equal(lse[:, :, :2], torch.full((1, 2, 2), -float("inf")))
     assert torch.isinf(o[:, :, 2, :5]).all() and torch.isnan(o[:, :, 2, 5:9]).all() and torch.isfinite(o[:, :, 2, 9:]).all()
+
+
+@pytest.mark.parametrize("Sq", [1, 17])
+def test_distances_of_positions_that_f32_does_not_hold(lib, Sq):
+    """The end of a cache of more than 2^24 tokens: neighbouring keys' distances differ by one, as near its start."""
+    Sk, D, near = (1 << 24) + 333, 8, 4096
+    k, v = torch.zeros(1, 1, Sk, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 1, Sk, D, dtype=torch.bfloat16, device="cuda")
+    q, k[:, :, -near:], v[:, :, -near:], _ = direct.make(1, 1, 2, 1, Sq, near, D)
+    slopes = torch.tensor([0.5, 0.03], device="cuda")      # at a distance of `near` the weights are below e^-122
+    o, lse = torch.empty_like(q), torch.empty(1, 2, Sq, device="cuda")
+    rc, status = direct.launch(lib, direct.attention_args(lib, q, k, v, o, lse, slopes=slopes, query_offset=Sk - Sq, causal=1))
+    torch.cuda.synchronize()
+    assert rc == 0 and not status.item()
+    want = ref.attention(q.cpu(), k[:, :, -near:].cpu(), v[:, :, -near:].cpu(), "bf16", "bhsd", D ** -0.5, slopes=slopes.cpu(), query_offset=near - Sq, causal=True)
+    direct.close(o, *want["o"], "o")
+    direct.close(lse, *want["lse"], "lse")
