@@ -125,9 +125,6 @@ __device__ __forceinline__ void grad_wait(uint32_t (&a)[16], uint32_t (&b)[16]) 
                : "memory");
 }
 
-// Lets the loads in flight land before shared memory goes away.
-__device__ __forceinline__ void grad_linger() { for (uint32_t i = 0; i < 4096; i++) __nanosleep(256); }
-
 // Sixteen columns of a row of an accumulator times `f`, as 16-bit values; `width` of them exist
 template <int EL>
 __device__ __forceinline__ void grad_write(uint32_t taddr, char* row, bool there, int width, float f, bool zero) {
@@ -265,8 +262,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     uint32_t uc = 0, nt = 0;       // units loaded, tiles with work
     int fixed = (int)blockIdx.x;
     for (int n = 0;; n++) {
-      const bool free = n < 2 || ha_barrier(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 61);
-      if (!__all_sync(0xffffffffu, free)) break;
+      if (n >= 2 && !ha_barrier_warp(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 61)) break;
       int t = 0;
       if (sched) {
         if (lane == 0) t = atomicAdd(sched, 1);
@@ -368,7 +364,6 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
             else { it = 0; hh++; walk.start(s, listed); }
           }
         }
-        if (!ok) grad_linger();
       }
       __syncwarp();
       uc += (uint32_t)count; nt++;
@@ -448,7 +443,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     uint32_t uc = 0, mine = 0, nt = 0;            // units of all groups before this tile, this group's units, tiles with work
     bool ok = true;
     for (int n = 0; ok; n++) {
-      if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
+      if (!ha_barrier_warp(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
       volatile TileSlot* s = slots + (n & 1);
       const int t = s->tile, units = s->blocks, b = s->b, th = s->h, at = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
@@ -504,8 +499,8 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         for (int i = 0; i < GROUPS && k < total; i++, k++) advance();
         if (KEYS && k < total) ahead = fetch(hh, walk.j);
         // the group's four warps have stored theirs (and read those of two units ago)
-        if (KEYS && !ha_barrier(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
-        if (!ha_barrier(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
+        if (KEYS && !ha_barrier_warp(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
+        if (!ha_barrier_warp(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
         tc_fence_after();
         const int u0 = unit * GRAD_UNIT;           // the unit's first key or query
         const float slope = p.a.slopes ? ld_global(p.a.slopes + head) * kLog2e : 0.f;
@@ -590,7 +585,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1));   // the tile's list has been walked
       if (total > 0) {
-        if (!ha_barrier(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
+        if (!ha_barrier_warp(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
         tc_fence_after();
         nt++;
       }
@@ -615,6 +610,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     }
   }
 
+  ha_linger(abort_flag);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) { tc_fence_after(); tmem_dealloc(tmem_base, TMEM_COLS); }

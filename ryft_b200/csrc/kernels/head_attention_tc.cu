@@ -113,8 +113,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     int fixed = (int)blockIdx.x + w * (int)gridDim.x;   // without a counter: every worker takes tiles in steps of all workers
     for (int n = 0;; n++) {
       // the slot's previous tile has been read by the issuer and the four softmax warps (all lanes wait: they leave together)
-      const bool free = n < 2 || ha_barrier(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21);
-      if (!__all_sync(0xffffffffu, free)) break;
+      if (n >= 2 && !ha_barrier_warp(bar_te + 8 * (n & 1), (uint32_t)(((n >> 1) - 1) & 1), abort_flag, status, 21)) break;
       int t = 0;
       if (w == 1 && p.total <= (int)gridDim.x) t = -1;     // one tile per SM: the first workers take them
       else if (sched) {
@@ -222,10 +221,6 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (idle > 16) { if (*abort_flag) { ok = false; break; } __nanosleep(idle > 4096 ? 256 : 32); }
           }
         }
-        if (!ok) {
-          // the other roles stop at their next wait; let copies already in flight land before shared memory goes away
-          for (uint32_t i = 0; i < 4096; i++) __nanosleep(256);
-        }
       }
       __syncwarp();
       kc += (uint32_t)blocks; vc += (uint32_t)blocks; nq++;
@@ -297,7 +292,6 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t prow_s = wbase + (uint32_t)(SM::P_OFF + row * 128);
     const uint32_t sw = (uint32_t)(row & 7);
     uint32_t sc = 0, hc = 0;                      // score blocks consumed, half-steps of weights published
-    bool ok = true;
     const uint64_t mult2 = splat2(p.mult);
     // 32 scores -> exp2, partial row sums, 16 words of 16-bit pairs
     auto exps = [&](const uint32_t (&r)[32], uint64_t mn2, uint64_t (&ps2)[2], uint32_t (&pw)[16]) {
@@ -324,8 +318,8 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (lane == 0) mbar_arrive(bar_pf);
       hc++;
     };
-    for (int n = 0; ok; n++) {
-      if (!ha_barrier(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) { ok = false; break; }
+    for (int n = 0;; n++) {
+      if (!ha_barrier_warp(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 25)) break;
       volatile TileSlot* s = slots + (n & 1);
       const int t = s->tile, blocks = s->blocks;
       if (t < 0) break;
@@ -346,10 +340,15 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       float m_used = -INFINITY, l = 0.f;
       bool poisoned = false;
+      // A wait inside the tile that runs out lets its lane go on with what is there: the lanes of a warp have to stay together for
+      // its votes and TMEM loads.  They leave as one, every 64 blocks and at the tile's end, and such a tile's rows are not written.
+      // (With a vote behind every wait a capped prompt took 1 % longer still.)
+      auto wait = [&](uint32_t bar, uint32_t parity, int code) { ha_barrier(bar, parity & 1, abort_flag, status, code); };
+      auto given_up = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag != 0); };
       // the previous block's second half-product has retired: the buffer of weights is free and the accumulator at rest
-      auto settle = [&](int it, bool rescale, float alpha) -> bool {
-        if (it == 0) return true;
-        if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 18)) return false;
+      auto settle = [&](int it, bool rescale, float alpha) {
+        if (it == 0) return;
+        wait(bar_pv, hc - 1, 18);
         tc_fence_after();
         if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
@@ -363,30 +362,29 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           tc_wait_st();
         }
-        return true;
       };
       // values behind the sequence's end: zero before they meet their weights of zero
       uint32_t vc = sc;                           // the tile's first V block; its count goes with the score blocks
-      auto clear_tail = [&](int j) -> bool {
+      auto clear_tail = [&](int j) {
         const uint32_t turn = vc++;
-        if (!p.a.lengths || s->length >= p.a.Sk || s->length >= (j + 1) * HA_BLOCK) return true;
-        if (!ha_barrier(bar_vf, turn & 1, abort_flag, status, 26)) return false;
+        if (!p.a.lengths || s->length >= p.a.Sk || s->length >= (j + 1) * HA_BLOCK) return;
+        wait(bar_vf, turn, 26);
         if (j * HA_BLOCK + row >= s->length) {
 #pragma unroll 1
           for (int c = 0; c < DC; c++)
 #pragma unroll
             for (int q = 0; q < 8; q++) sts_v4(wbase + (uint32_t)(SM::V_OFF + c * HA_CHUNK + row * 128 + q * 16), 0, 0, 0, 0);
         }
-        return true;
       };
       BlockWalk walk;
       if (blocks > 0) walk.start(s, listed);
-      for (int it = 0; it < blocks && ok; it++) {
+      for (int it = 0; it < blocks; it++) {
         const int j = walk.j;
         bool compare = false;
         if constexpr (DOCUMENTS) compare = listed ? (s->compare[j >> 5] >> (j & 31)) & 1 : p.a.documents != nullptr;
         if (it + 1 < blocks) walk.next();
-        if (!ha_barrier(bar_sf, sc & 1, abort_flag, status, 17)) { ok = false; break; }
+        if ((it & 63) == 63 && given_up()) break;
+        wait(bar_sf, sc, 17);
         tc_fence_after();
         // keys of this block that this row sees: [0, lim], and among them those of its document
         const int lim = end - 1 - j * HA_BLOCK;
@@ -442,7 +440,8 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           bool rescale = false;
           if (it == 0) m_used = mx;
           else if (mx - m_used > 8.0f) { alpha = fast_exp2(m_used - mx); l *= alpha; m_used = mx; rescale = true; }
-          if (!settle(it, rescale, alpha) || !clear_tail(j)) { ok = false; break; }
+          settle(it, rescale, alpha);
+          clear_tail(j);
           const uint64_t mn2 = splat2(m_used == -INFINITY ? 0.f : -m_used);
           uint64_t ps2[2] = {0ull, 0ull};
           auto chunks = [&](auto SMALL, auto MASK) {
@@ -474,7 +473,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
                 pw[h2] = ha_pack<EL>(e0, e1);
               }
               // the first half's product has retired: its buffer takes the second half
-              if (c == 2 && !ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
+              if (c == 2) wait(bar_pv, hc - 1, 19);
               store(c & 1, pw);
               if (c & 1) publish();
             }
@@ -483,7 +482,6 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (small) { if (need_mask) chunks(bool_constant<true>{}, bool_constant<true>{}); else chunks(bool_constant<true>{}, bool_constant<false>{}); }
           else { if (need_mask) chunks(bool_constant<false>{}, bool_constant<true>{}); else chunks(bool_constant<false>{}, bool_constant<false>{}); }
           sc++;
-          if (!ok) break;
           uint32_t a0, a1, b0, b1;
           unpack2(ps2[0], a0, a1); unpack2(ps2[1], b0, b1);
           l += (__uint_as_float(a0) + __uint_as_float(a1)) + (__uint_as_float(b0) + __uint_as_float(b1));
@@ -571,7 +569,8 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         bool rescale = false;
         if (it == 0) m_used = mx;
         else if ((mx - m_used) * p.mult > 8.0f) { alpha = fast_exp2((m_used - mx) * p.mult); l *= alpha; m_used = mx; rescale = true; }
-        if (!settle(it, rescale, alpha) || !clear_tail(j)) { ok = false; break; }
+        settle(it, rescale, alpha);
+        clear_tail(j);
         const float mneg = (m_used == -INFINITY) ? 0.f : -m_used * p.mult;
         const uint64_t mn2 = splat2(mneg);
         uint64_t ps2[2] = {0ull, 0ull};
@@ -585,7 +584,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // the second half: its first 32 keys are exponentiated while the first half multiplies
           uint32_t pw[16];
           exps(r[2], mn2, ps2, pw);
-          if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 19)) { ok = false; break; }
+          wait(bar_pv, hc - 1, 19);
           store(0, pw);
           exps(r[3], mn2, ps2, pw); store(1, pw);
         }
@@ -597,12 +596,12 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         }
       }
-      if (!ok) break;
       // ---- the tile's last product has retired: normalise and write the rows ----
       if (blocks > 0) {
-        if (!ha_barrier(bar_pv, (hc - 1) & 1, abort_flag, status, 20)) { ok = false; break; }
+        wait(bar_pv, hc - 1, 20);
         tc_fence_after();
       }
+      if (given_up()) break;
       if (poisoned) l = __int_as_float(0x7fc00000);
       if (p.parts > 1) {
         const int64_t at = ((int64_t)s->part * (p.total / p.parts) + ((int64_t)s->b * p.a.Hq + s->h) * p.q_tiles + s->at / HA_BLOCK) * HA_BLOCK + row;
@@ -660,6 +659,7 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   }
 
+  ha_linger(abort_flag);
   tc_fence_before();
   __syncthreads();
   if (warp == 2) { tc_fence_after(); tmem_dealloc(tmem_base, TMEM_COLS); }

@@ -224,6 +224,15 @@ __device__ __forceinline__ bool ha_barrier(uint32_t bar, uint32_t parity, volati
   return false;
 }
 
+// The same for all lanes of a warp, with one answer: lanes that gave up by themselves would miss from the votes of the others.
+__device__ __forceinline__ bool ha_barrier_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
+  return __all_sync(0xffffffffu, ha_barrier(bar, parity, abort_flag, status, code));
+}
+// Before a CTA that has given up leaves: what it has in flight (copies, products) ends while shared memory and TMEM are still its own.
+__device__ __forceinline__ void ha_linger(const volatile int* abort_flag) {
+  if (*abort_flag) for (uint32_t i = 0; i < 4096; i++) __nanosleep(256);
+}
+
 // A tile as its loading warp publishes it.
 struct TileSlot {
   int tile;                    // -1: no more
