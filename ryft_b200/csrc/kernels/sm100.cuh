@@ -226,7 +226,7 @@ __device__ __forceinline__ uint64_t make_smem_desc(uint32_t smem_addr, uint32_t 
 typedef CUresult (*PFN_encodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                     const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                     CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-inline PFN_encodeTiled get_encode_tiled() {
+inline PFN_encodeTiled find_encode_tiled() {
   static PFN_encodeTiled fn = [] {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -234,6 +234,17 @@ inline PFN_encodeTiled get_encode_tiled() {
     return (PFN_encodeTiled)p;
   }();
   return fn;
+}
+// The driver wants a current context, which a thread has only once the runtime has worked on its device: where it answers with an
+// error the device is set and it is asked once more.
+inline PFN_encodeTiled get_encode_tiled() {
+  if (!find_encode_tiled()) return nullptr;
+  return [](auto... args) -> CUresult {
+    CUresult r = find_encode_tiled()(args...);
+    int dev = 0;
+    if (r != CUDA_SUCCESS && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = find_encode_tiled()(args...);
+    return r;
+  };
 }
 // 3-D map over a [dim2][dim1][dim0] tensor (dim0 contiguous) with a swizzled box {box0, box1, 1} (128-byte swizzle
 // unless told otherwise).

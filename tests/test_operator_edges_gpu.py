@@ -1,5 +1,6 @@
 """The named operators at the edges of what they accept, on the GPU, against 64-bit forms (operators_reference.py)."""
 import ctypes as C
+import threading
 
 import pytest
 import torch
@@ -147,3 +148,24 @@ def test_distances_of_positions_that_f32_does_not_hold(lib, Sq):
     want = ref.attention(q.cpu(), k[:, :, -near:].cpu(), v[:, :, -near:].cpu(), "bf16", "bhsd", D ** -0.5, slopes=slopes.cpu(), query_offset=near - Sq, causal=True)
     direct.close(o, *want["o"], "o")
     direct.close(lse, *want["lse"], "lse")
+
+
+# ---- threads and streams ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("Sq", [1, 40])
+@pytest.mark.parametrize("gradient", [False, True])
+def test_the_first_call_of_a_thread(lib, gradient, Sq):
+    """A thread that has not used CUDA yet has no current context."""
+    q, k, v, do = direct.make(1, 1, 2, 1, Sq, 70, 64)
+    o, lse = torch.empty_like(q), torch.empty(1, 2, Sq, device="cuda")
+    grads = (do, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+    assert direct.launch(lib, direct.attention_args(lib, q, k, v, o, lse))[0] == 0
+    a = direct.attention_args(lib, q, k, v, o, lse, grads if gradient else None)
+    status, codes = torch.zeros(1, dtype=torch.int32, device="cuda"), []
+    torch.cuda.synchronize()
+    f = lib.b2x_launch_head_attention_gradient if gradient else lib.b2x_launch_head_attention
+    t = threading.Thread(target=lambda: codes.append(f(C.byref(a), status.data_ptr(), None)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert codes == [0] and not status.item()
