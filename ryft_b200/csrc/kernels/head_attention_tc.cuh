@@ -261,9 +261,11 @@ struct BlockWalk {
 
 
 int32_t* sched_slot(cudaStream_t stream);   // gemm_tc.cu: a (tile counter, finished CTAs) pair per stream
-// The same, or nullptr (tiles dealt out in a fixed order) while the stream is captured: graphs of one stream may later run side by
-// side, and would share the counter.
+// The same, or nullptr (tiles dealt out in a fixed order) where launches that share a handle may run side by side and would share the
+// counter: while the stream is captured (graphs of one stream may later run at once), and on the per-thread default stream, one
+// handle for every thread's own stream.
 inline int32_t* ha_sched(cudaStream_t stream) {
+  if (stream == cudaStreamPerThread) return nullptr;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(stream, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) return nullptr;
   return sched_slot(stream);

@@ -169,3 +169,40 @@ def test_the_first_call_of_a_thread(lib, gradient, Sq):
     t.join()
     torch.cuda.synchronize()
     assert codes == [0] and not status.item()
+
+
+def test_threads_on_their_own_default_streams(lib):
+    """Every thread's own stream has the same handle; calls of two threads run side by side and each yields what it yields alone."""
+    per_thread, cases = 2, []
+    for seed in (1, 2):
+        q, k, v, do = direct.make(seed, 2, 8, 4, 1500, 1500, 64)
+        o, lse = torch.empty_like(q), torch.empty(2, 8, 1500, device="cuda")
+        grads = (do, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+        f, b = direct.attention_args(lib, q, k, v, o, lse, causal=1), direct.attention_args(lib, q, k, v, o, lse, grads, causal=1)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        for a, gradient in ((f, False), (b, True)):
+            assert direct.launch(lib, a, gradient)[0] == 0
+        torch.cuda.synchronize()
+        cases.append((f, b, status, (o, lse, *grads[1:]), [t.clone() for t in (o, lse, *grads[1:])]))
+        for t in cases[-1][3]:
+            t.zero_()
+    torch.cuda.synchronize()
+    failures, start = [], threading.Barrier(2)
+
+    def work(f, b, status):
+        start.wait()
+        for _ in range(10):
+            for launch, a in ((lib.b2x_launch_head_attention, f), (lib.b2x_launch_head_attention_gradient, b)):
+                if launch(C.byref(a), status.data_ptr(), per_thread) != 0:
+                    failures.append("launch")
+    threads = [threading.Thread(target=work, args=c[:3]) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failures
+    for _, _, status, now, alone in cases:
+        assert not status.item()
+        for x, y in zip(now, alone):
+            assert torch.equal(x, y)
