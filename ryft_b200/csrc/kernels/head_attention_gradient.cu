@@ -27,6 +27,11 @@
 // derivative double the instructions for the FMA pipe.  Both kernels and the row constants: 470 us, 731 TFLOP/s of the gradient's
 // five products; capped 548 us.
 //
+// f16: P (dP - delta) passes f16's range at both ends where the gradients do not, so that it is rounded as a multiple of a power of
+// two that its size allows (grad_shift): |P (dP - delta)| = P |dO (V - O)| <= 2 |dO| max|V|, as lengths of rows, is brought below f16's
+// largest value, for dQ row by row, for dK with the largest dO of all query heads that share the key head.  The row constants' kernel
+// finds the lengths (V is read once more); the factor sits in the sum dP - delta, and leaves with the last product.
+//
 // 384 threads, 512 with three pairs: warp 0 draws tiles and loads (TMA), warp 1 issues the MMAs, warps 4 and up do the arithmetic.
 #include <atomic>
 #include <type_traits>
@@ -49,8 +54,18 @@ struct GradParams {
   uint64_t in2;                       // scale * log2(e)
   HeadCap cap;
   float scale;
+  const float* row_size;              // f16: [B, Hq, rows] squared lengths of the rows of dO
+  const float2* head_size;            // f16: [B, Hk] their largest over all queries that see something, and that of the rows of V within the length
   uint32_t idesc_s, idesc_acc;
 };
+
+// The power of two that P (dP - delta) is divided by, from the squared lengths of dO and V (1 % for their roundings and P's).  0
+// where there is nothing to go by: zeros, and infinities or NaN, which come out as they are.
+__device__ __forceinline__ int grad_shift(float dout, float v) {
+  const float most = sqrtf(dout) * sqrtf(v) * (2.02f / 65504.f);
+  return most > 0.f && most < INFINITY ? (int)(__float_as_uint(most) >> 23) - 126 : 0;
+}
+__device__ __forceinline__ float grad_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Document ranges of the tokens at positions [lo, hi], from the blocks that hold them; nothing where there is no such token.
 __device__ __forceinline__ int2 grad_range(const GradParams& p, const int2* rs, int lo, int hi) {
@@ -61,10 +76,10 @@ __device__ __forceinline__ int2 grad_range(const GradParams& p, const int2* rs, 
 }
 
 // P and dS of 16 scores of a row as 16-bit words.  nl and nd are the row constants of the pair 2i, 2i + 1; far is the distance of
-// the first, bits say which are seen.  CAP: 0 none, 1 by the polynomial, 2 any.
+// the first, bits say which are seen.  f16: dS is worked out times `part`, nd included.  CAP: 0 none, 1 by the polynomial, 2 any.
 template <int EL, int CAP, bool SLOPE, bool MASK, typename L, typename N>
 __device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (&s)[16], const uint32_t (&dp)[16], const L& nl, const N& nd, float slope, float far, uint32_t bits,
-                                           uint32_t (&pw)[8], uint32_t (&dw)[8]) {
+                                           float part, uint32_t (&pw)[8], uint32_t (&dw)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; i++) {
     uint64_t x2, bend2 = 0;
@@ -88,7 +103,10 @@ __device__ __forceinline__ void grad_words(const GradParams& p, const uint32_t (
     float x0 = __uint_as_float(a0), x1 = __uint_as_float(a1);
     if constexpr (SLOPE) { x0 = fmaf(fabsf(far - (float)(2 * i)), -slope, x0); x1 = fmaf(fabsf(far - (float)(2 * i + 1)), -slope, x1); }
     const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-    uint64_t d2 = mul2(pack2(__float_as_uint(p0), __float_as_uint(p1)), add2(pack2(dp[2 * i], dp[2 * i + 1]), nd(i)));
+    uint64_t d2 = pack2(dp[2 * i], dp[2 * i + 1]);
+    if constexpr (EL == EL_F16) d2 = fma2(d2, splat2(part), nd(i));
+    else d2 = add2(d2, nd(i));
+    d2 = mul2(pack2(__float_as_uint(p0), __float_as_uint(p1)), d2);
     if constexpr (CAP != 0) d2 = mul2(d2, bend2);
     unpack2(d2, a0, a1);
     pw[i] = ha_pack<EL>(p0, p1);
@@ -462,16 +480,22 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
       }
       const int doc = p.a.documents && pos >= 0 && pos < p.a.Sk ? (int)ld_global((const uint32_t*)p.a.documents + (int64_t)b * p.a.Sk + pos) : 0;
       uint64_t nl2 = 0, nd2 = 0;
-      if constexpr (!KEYS) {
-        const int64_t rc = ((int64_t)b * p.a.Hq + th) * p.rows + self;
-        nl2 = splat2(ld_global(p.neg_lse + rc)); nd2 = splat2(ld_global(p.neg_delta + rc));
+      float part_of = 1.f, whole = p.scale;        // f16: dS is held as this part of itself; what the sums are multiplied by
+      const int64_t rc = ((int64_t)b * p.a.Hq + th) * p.rows + self;
+      if constexpr (EL == EL_F16) {
+        if (total > 0) {
+          const uint2 size = ld_global((const uint2*)(p.head_size + (int64_t)b * p.a.Hk + (KEYS ? th : th / p.a.group)));
+          const int shift = grad_shift(KEYS ? __uint_as_float(size.x) : ld_global(p.row_size + rc), __uint_as_float(size.y));
+          part_of = grad_power(-shift); whole *= grad_power(shift);
+        }
       }
+      if constexpr (!KEYS) { nl2 = splat2(ld_global(p.neg_lse + rc)); nd2 = splat2(ld_global(p.neg_delta + rc) * part_of); }
       BlockWalk walk;
       int hh = 0, it = 0;                          // head that passes by, unit of the head
       // keys: a unit's row constants, one value per thread, fetched a unit ahead
       auto fetch = [&](int head, int unit) {
         const int64_t rc = ((int64_t)b * p.a.Hq + th * p.a.group + head) * p.rows + unit * GRAD_UNIT + (tid & 63);
-        return ld_global((tid < 64 ? p.neg_lse : p.neg_delta) + rc);
+        return tid < 64 ? ld_global(p.neg_lse + rc) : ld_global(p.neg_delta + rc) * part_of;
       };
       auto advance = [&]() {                       // to the next unit, over the end of a head
         if (++it == units) { it = 0; hh++; if (hh < repeat) walk.start(s, listed); }
@@ -564,12 +588,12 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
               }
               grad_wait(sr, dr);
               grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr, dr, [&](int i) { return nlv[i]; }, [&](int i) { return ndv[i]; }, slope, far - (float)(c * 16),
-                                                                                         bits, pw, dw);
+                                                                                         bits, part_of, pw, dw);
               // words of 16 queries into 8 columns that this row has read
               tmem_st_32x8(s_addr + (uint32_t)(c * 8), pw);
             } else {
               grad_wait(sr, dr);
-              grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr, dr, [&](int) { return nl2; }, [&](int) { return nd2; }, slope, far - (float)(c * 16), bits, pw, dw);
+              grad_words<EL, decltype(C)::value, decltype(S)::value, decltype(M)::value>(p, sr, dr, [&](int) { return nl2; }, [&](int) { return nd2; }, slope, far - (float)(c * 16), bits, part_of, pw, dw);
             }
             tmem_st_32x8(s_addr + 64u + (uint32_t)(c * 8), dw);
           }
@@ -597,12 +621,12 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         if (p.parts > 1) {
           const int64_t tiles = p.total / p.parts, tile = ((int64_t)b * (KEYS ? p.a.Hk : p.a.Hq) + th) * p.tiles + at / HA_BLOCK;
           grad_part(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), p.partial + (((part * tiles + tile) * (KEYS ? 2 : 1) + second) * HA_BLOCK + row) * D + first,
-                    KEYS && !second ? 1.f : p.scale, total == 0);
+                    KEYS && !second ? 1.f : whole, total == 0);
           continue;
         }
         const B2xHeadStrides& o = !KEYS ? p.a.dqs : second ? p.a.dks : p.a.dvs;
         char* out = (!KEYS ? p.a.dq : second ? p.a.dk : p.a.dv) + 2 * ((int64_t)b * o.batch + (int64_t)th * o.head + (int64_t)self * o.token + first);
-        grad_write<EL>(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), out, self < (KEYS ? p.a.Sk : p.a.Sq), p.a.D - first, KEYS && !second ? 1.f : p.scale, total == 0);
+        grad_write<EL>(tmem_base + lane_addr + ACC + (uint32_t)(c * 16), out, self < (KEYS ? p.a.Sk : p.a.Sq), p.a.D - first, KEYS && !second ? 1.f : whole, total == 0);
       }
       tc_fence_before();
       __syncwarp();
@@ -621,15 +645,59 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
 // ---- row constants: -log sum in log2 units and -delta; rows behind the last query weigh nothing ---------------------------------
 // 32 rows of a head per block (`rows` is a multiple of 128), two per half warp, so that a thread has four loads of 16 bytes in flight;
 // a sequence's heads follow one another, for where tokens come before heads their rows are neighbours in memory.  2 x 16 heads of
-// 4096 rows of 128, 67 MB: 16 us with nothing in L2 (18 with one row per half warp, head by head).
+// 4096 rows of 128, 67 MB: 16 us with nothing in L2 (18 with one row per half warp, head by head).  f16: the squared lengths of the
+// rows of dO and, by further blocks, of V; the bits of floats that are not negative are ordered as they are (NaN above infinity), so
+// that the largest is one of whole numbers and does not depend on the order in which blocks find it.
+template <int EL> __device__ __forceinline__ void rows_floats(const uint4& w, float (&f)[8]) {
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    float2 u;
+    if constexpr (EL == EL_BF16) u = __bfloat1622float2(*(const __nv_bfloat162*)&ws[k]);
+    else u = __half22float2(*(const __half2*)&ws[k]);
+    f[2 * k] = u.x; f[2 * k + 1] = u.y;
+  }
+}
+// over the half warp that holds a row
+__device__ __forceinline__ float rows_dot(const float (&a)[8], const float (&b)[8]) {
+  float d = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; k++) d = fmaf(a[k], b[k], d);
+#pragma unroll
+  for (int off = 8; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+  return d;
+}
 template <int EL>
-__global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ HeadAttn p, float* neg_lse, float* neg_delta, int32_t rows) {
+__global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ HeadAttn p, float* neg_lse, float* neg_delta, int32_t rows, float* row_size, uint32_t* head_size) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, part = lane & 15;
-  const uint32_t per_head = (uint32_t)rows / 32u, at = blockIdx.x / (uint32_t)p.Hq;
+  const uint32_t per_head = (uint32_t)rows / 32u;
+  const int in_block = ((int)(threadIdx.x >> 5) * 2 + (lane >> 4)) * 2;
+  if constexpr (EL == EL_F16) {
+    const uint32_t query_blocks = (uint32_t)p.B * (uint32_t)p.Hq * per_head;
+    if (blockIdx.x >= query_blocks) {
+      // 32 rows of a head of V
+      const uint32_t key_blocks = ((uint32_t)p.Sk + 31u) / 32u, id = blockIdx.x - query_blocks, head = id / key_blocks;
+      const int b = (int)(head / (uint32_t)p.Hk), u = (int)(head - (uint32_t)b * (uint32_t)p.Hk), length = head_sequence(p, b).length;
+      const int first = (int)(id - head * key_blocks) * 32 + in_block;
+      uint32_t most = 0;
+#pragma unroll
+      for (int r = 0; r < 2; r++) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (first + r < length && part * 8 < p.D) x = ld_global((const uint4*)(p.v + 2 * ((int64_t)b * p.vs.batch + (int64_t)u * p.vs.head + (int64_t)(first + r) * p.vs.token)) + part);
+        float f[8];
+        rows_floats<EL>(x, f);
+        most = max(most, __float_as_uint(rows_dot(f, f)));
+      }
+      most = __reduce_max_sync(0xffffffffu, most);
+      if (lane == 0 && most != 0) atomicMax(head_size + 2 * head + 1, most);
+      return;
+    }
+  }
+  const uint32_t at = blockIdx.x / (uint32_t)p.Hq;
   const int h = (int)(blockIdx.x - at * (uint32_t)p.Hq), b = (int)(at / per_head), bh = b * p.Hq + h;
-  const int first = (int)(at - (uint32_t)b * per_head) * 32 + ((int)(threadIdx.x >> 5) * 2 + (lane >> 4)) * 2;
+  const int first = (int)(at - (uint32_t)b * per_head) * 32 + in_block;
   uint4 x[2], y[2];
 #pragma unroll
   for (int r = 0; r < 2; r++) {
@@ -639,20 +707,15 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
       y[r] = ld_global((const uint4*)(p.dout + 2 * ((int64_t)b * p.dos.batch + (int64_t)h * p.dos.head + (int64_t)(first + r) * p.dos.token)) + part);
     }
   }
+  uint32_t most = 0;
 #pragma unroll
   for (int r = 0; r < 2; r++) {
-    const uint32_t xs[4] = {x[r].x, x[r].y, x[r].z, x[r].w}, ys[4] = {y[r].x, y[r].y, y[r].z, y[r].w};
-    float d = 0.f;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-      float2 u, v;
-      if constexpr (EL == EL_BF16) { u = __bfloat1622float2(*(const __nv_bfloat162*)&xs[k]); v = __bfloat1622float2(*(const __nv_bfloat162*)&ys[k]); }
-      else { u = __half22float2(*(const __half2*)&xs[k]); v = __half22float2(*(const __half2*)&ys[k]); }
-      d = fmaf(u.x, v.x, d);
-      d = fmaf(u.y, v.y, d);
-    }
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+    float u[8], v[8];
+    rows_floats<EL>(x[r], u);
+    rows_floats<EL>(y[r], v);
+    const float d = rows_dot(u, v);
+    float size = 0.f;
+    if constexpr (EL == EL_F16) size = rows_dot(v, v);
     if (part == 0) {
       // a query that saw nothing has a log sum of -inf: its weights are 0
       const bool there = first + r < p.Sq;
@@ -660,7 +723,15 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
       const float l = there ? ld_global(p.lse + (int64_t)bh * p.Sq + first + r) : -INFINITY;
       neg_lse[id] = l == -INFINITY ? -INFINITY : -l * kLog2e;
       neg_delta[id] = there ? -d : 0.f;
+      if constexpr (EL == EL_F16) {
+        row_size[id] = size;
+        if (l != -INFINITY) most = max(most, __float_as_uint(size));
+      }
     }
+  }
+  if constexpr (EL == EL_F16) {
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0 && most != 0) atomicMax(head_size + 2 * ((uint32_t)b * (uint32_t)p.Hk + (uint32_t)(h / p.group)), most);
   }
 }
 
@@ -720,9 +791,11 @@ int grad_rows(int64_t Sq) { return (int)((Sq + HA_BLOCK - 1) / HA_BLOCK * HA_BLO
 
 }  // namespace
 
-// row constants [2][B, Hq, rows], the documents' ranges, and from a multiple of 16 bytes on the sums of parts, of one side at a time
+// row constants [2][B, Hq, rows], the documents' ranges, for f16 the sizes of heads [B, Hk, 2] and rows [B, Hq, rows], and from a
+// multiple of 16 bytes on the sums of parts, of one side at a time
+int64_t grad_size_bytes(int elem, int64_t B, int64_t Hq, int64_t Hk, int64_t rows) { return elem == EL_F16 ? B * (Hk * 8 + Hq * rows * 4) : 0; }
 int64_t ha_gradient_scratch(const B2xHeadAttentionArgs* a, int64_t ranges) {
-  const int64_t head = a->B * a->Hq * (int64_t)grad_rows(a->Sq) * 8 + ranges, q = grad_part_bytes(*a, false), k = grad_part_bytes(*a, true);
+  const int64_t rows = grad_rows(a->Sq), head = a->B * a->Hq * rows * 8 + ranges + grad_size_bytes(a->elem, a->B, a->Hq, a->Hk, rows), q = grad_part_bytes(*a, false), k = grad_part_bytes(*a, true);
   return q > 0 || k > 0 ? (head + 15) / 16 * 16 + (q > k ? q : k) : head;
 }
 int ha_gradient_launches(const B2xHeadAttentionArgs* a) {
@@ -743,7 +816,11 @@ int ha_launch_gradient(const HeadAttn& call, int elem, void* scratch, int32_t* s
   p.neg_delta = p.neg_lse + n;
   int2* ranges = (int2*)(p.neg_delta + n);
   p.key_blocks = (a.Sk + HA_BLOCK - 1) / HA_BLOCK;
-  p.partial = (float*)((char*)scratch + (n * 8 + (a.documents ? (int64_t)a.B * p.key_blocks * 8 : 0) + 15) / 16 * 16);
+  const int64_t fixed = n * 8 + (a.documents ? (int64_t)a.B * p.key_blocks * 8 : 0), heads = (int64_t)a.B * a.Hk;
+  uint32_t* head_size = (uint32_t*)((char*)scratch + fixed);
+  p.head_size = (const float2*)head_size;
+  p.row_size = (const float*)head_size + 2 * heads;
+  p.partial = (float*)((char*)scratch + (fixed + grad_size_bytes(elem, a.B, a.Hq, a.Hk, p.rows) + 15) / 16 * 16);
   p.scale = a.scale;
   p.in2 = ha_pair(a.scale * kLog2e);
   p.cap = ha_cap(a.softcap, a.scale);
@@ -752,8 +829,15 @@ int ha_launch_gradient(const HeadAttn& call, int elem, void* scratch, int32_t* s
     if (rc) return rc;
   }
   if (n > 0) {
-    const cudaError_t e = launch_overlapped(elem == EL_BF16 ? k_attention_rows<EL_BF16> : k_attention_rows<EL_F16>, dim3((unsigned)(n / 32)), dim3(256), 0, stream, a,
-                                            const_cast<float*>(p.neg_lse), const_cast<float*>(p.neg_delta), p.rows);
+    int64_t blocks = n / 32;
+    if (elem == EL_F16) {
+      blocks += heads * ((a.Sk + 31) / 32);
+      const cudaError_t z = cudaMemsetAsync(head_size, 0, (size_t)heads * 8, stream);
+      if (z != cudaSuccess) return (int)z;
+    }
+    if (blocks > 0x7fffffff) return (int)cudaErrorInvalidValue;
+    const cudaError_t e = launch_overlapped(elem == EL_BF16 ? k_attention_rows<EL_BF16> : k_attention_rows<EL_F16>, dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                                            const_cast<float*>(p.neg_lse), const_cast<float*>(p.neg_delta), p.rows, const_cast<float*>(p.row_size), head_size);
     if (e != cudaSuccess) return (int)e;
     count_launch();
   }

@@ -206,3 +206,88 @@ def test_threads_on_their_own_default_streams(lib):
         assert not status.item()
         for x, y in zip(now, alone):
             assert torch.equal(x, y)
+
+
+# ---- f16 gradients of any size that f16 holds --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -10, 1e4, 4e4])
+@pytest.mark.parametrize("sizes,options", [
+    (dict(B=2, Sq=130, Sk=130, Hq=4, Hk=2, D=128), dict(causal=True)),
+    (dict(B=1, Sq=200, Sk=200, Hq=2, Hk=1, D=64), dict(causal=True, softcap=20.0)),
+    (dict(B=1, Sq=1100, Sk=1100, Hq=2, Hk=1, D=80), dict(lengths=[700], slopes=True)),      # in parts
+], ids=str)
+def test_f16_gradients_over_the_range_of_f16(client, sizes, options, size):
+    """P (dP - delta) passes f16's largest value where the gradients do not.  Values behind a length may be anything."""
+    q, k, v, do, extra, how = program.attention_case(**sizes, dtype="f16", layout="bhsd", seed=3, **options)
+    do = (do.float().clamp(-1.2, 1.2) * size).half()
+    v, k, q = v.float().clamp(-2, 2).half(), (k.float() / 4).half(), (q.float() / 4).half()
+    if "lengths" in options:
+        v[:, :, options["lengths"][0]:] = float("inf")
+    got = program.attention_run(client, q, k, v, do, extra, how, "f16", "bhsd")
+    want = ref.attention(q, k, v, "f16", "bhsd", sizes["D"] ** -0.5, do=do, **extra, **how)
+    assert want["dq"][0].abs().max() < 65000 and want["dk"][0].abs().max() < 65000, "the case is meant to fit"
+    for name, x in zip(("o", "lse", "dq", "dk", "dv"), got):
+        fits = want[name][0].abs() < 65000       # dv itself is larger in places
+        program.within(torch.where(fits, x.double(), 0.0), torch.where(fits, want[name][0], 0.0), want[name][1], name)
+
+
+@pytest.mark.parametrize("S,D", [(4000, 128), (1500, 40)])
+def test_f16_gradients_of_many_small_shares_keep_their_figures(client, S, D):
+    """Every key has a weight of 1 / S, and P (dP - delta) lies below f16's normal values: rounded there it would have a step of 2^-24.
+
+    Three roundings of relative 2^-11 at most (P or dS, the result, O behind delta), each of root mean square 2^-11 / sqrt(3), and results
+    that are sums of many independent ones: below 2^-10 of the norm."""
+    q, k, v, do, extra, how = program.attention_case(1, S, S, 2, 1, D, "f16", "bshd", 5)
+    q = (q.float() / 1024).half()
+    k, v, do = (k.float() * 8).half(), (v.float() * 8).half(), (do.float() * 2.0 ** -12).half()
+    do[:, ::2] = (do[:, ::2].float() * 2.0 ** -3).half()
+    got = program.attention_run(client, q, k, v, do, extra, how, "f16", "bshd")
+    want = ref.attention(q, k, v, "f16", "bshd", D ** -0.5, do=do, **extra, **how)
+    dq, true = got[2].double(), want["dq"][0]
+    normal = true.abs() >= 2.0 ** -14           # of the result, too, only what f16 holds to its full width
+    assert normal[:, 1::2].double().mean() > 0.5
+    off = torch.where(normal, dq - true, 0.0).norm() / torch.where(normal, true, 0.0).norm()
+    assert off < 2.0 ** -10, float(off)
+
+
+def test_f16_queries_do_not_lose_figures_to_larger_ones(client):
+    """Neighbouring queries whose gradients differ by 2^18: dq goes by its own row."""
+    S, D = 300, 64
+    q, k, v, do, extra, how = program.attention_case(1, S, S, 2, 2, D, "f16", "bhsd", 5)
+    do = do.float().clamp(-2, 2)
+    do[:, :, ::2] *= 2.0 ** 12
+    do[:, :, 1::2] *= 2.0 ** -6
+    do, k = do.half(), (k.float() * 4).half()
+    q = (q.float() / 4).half()
+    got = program.attention_run(client, q, k, v, do, extra, how, "f16", "bhsd")[2].double()[:, :, 1::2]
+    true = ref.attention(q, k, v, "f16", "bhsd", D ** -0.5, do=do, **extra, **how)["dq"][0][:, :, 1::2]
+    assert (got - true).norm() / true.norm() < 2.0 ** -10
+
+
+def test_f16_gradients_in_captured_graphs(lib):
+    """The sizes of dO and V are found anew in every replay."""
+    q, k, v, do = direct.make(1, 2, 4, 2, 300, 300, 64, torch.float16)
+    o, lse = torch.empty_like(q), torch.empty(2, 4, 300, device="cuda")
+    grads = (do, torch.empty_like(q), torch.empty_like(k), torch.empty_like(v))
+    assert direct.launch(lib, direct.attention_args(lib, q, k, v, o, lse, causal=1))[0] == 0
+    a = direct.attention_args(lib, q, k, v, o, lse, grads, causal=1)
+    status, side = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.cuda.Stream()
+    large = do.clone().clamp_(-1, 1) * 8192
+    small = do * 2.0 ** -8
+    alone = []
+    for x in (large, small):
+        do.copy_(x)
+        assert direct.launch(lib, a, True)[0] == 0
+        torch.cuda.synchronize()
+        alone.append([t.clone() for t in grads[1:]])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        assert lib.b2x_launch_head_attention_gradient(C.byref(a), status.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    for _ in range(2):
+        for x, want in zip((large, small), alone):
+            do.copy_(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert not status.item()
+            for t, w in zip(grads[1:], want):
+                assert torch.isfinite(t).all() and torch.equal(t, w)
