@@ -513,22 +513,26 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
             for (int i = 0; i < 16; i++) unpack2(mul2(pack2(r[c][2 * i], r[c][2 * i + 1]), p.in2), r[c][2 * i], r[c][2 * i + 1]);
         }
+        float near = 0.f, grow = 0.f;              // SLOPES: what 32 keys' scores lack of their bias
+        auto lacking = [&](int c) -> float { return fmaf((float)(32 * c), grow, near); };
         if (SLOPES && p.a.slopes) {
           const int far = pos - j * HA_BLOCK;
           const uint64_t m2 = p.cap.cap > 0.f ? splat2(1.f) : p.in2;
           const bool before = __all_sync(0xffffffffu, far >= HA_BLOCK - 1), behind = __all_sync(0xffffffffu, far <= 0);
           if (before || behind) {
-            // all keys on one side of all the warp's queries: the bias grows by the slope from key to key, anew every 32 of them
-            const float grow = before ? slope : -slope;
+            // All keys on one side of all the warp's queries: the bias grows by the slope from key to key.  Its growth within 32 keys is added
+            // here, what is the same for all of them where a maximum is taken off anyway: added up along the keys, a bias far from its
+            // query lost a rounding with every key.
+            grow = before ? slope : -slope;
+            near = -(float)far * grow;
             const uint64_t step2 = splat2(2.f * grow);
 #pragma unroll
             for (int c = 0; c < 4; c++) {
-              const float first = (float)(c * 32 - far) * grow;
-              uint64_t bias2 = pack2(__float_as_uint(first), __float_as_uint(first + grow));
+              uint64_t on2 = pack2(0u, __float_as_uint(grow));
 #pragma unroll
               for (int i = 0; i < 16; i++) {
-                unpack2(fma2(pack2(r[c][2 * i], r[c][2 * i + 1]), m2, bias2), r[c][2 * i], r[c][2 * i + 1]);
-                bias2 = add2(bias2, step2);
+                unpack2(fma2(pack2(r[c][2 * i], r[c][2 * i + 1]), m2, on2), r[c][2 * i], r[c][2 * i + 1]);
+                on2 = add2(on2, step2);
               }
             }
           } else {
@@ -560,7 +564,11 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int c = 0; c < 4; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) mx4[i & 3] = max3(mx4[i & 3], __uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
+            for (int i = 0; i < 16; i++) mx4[SLOPES ? c : i & 3] = max3(mx4[SLOPES ? c : i & 3], __uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1]));
+          if constexpr (SLOPES) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) mx4[c] += lacking(c);
+          }
           mx = max3(mx4[0], mx4[1], max3(mx4[2], mx4[3], -INFINITY));
         }
         // a NaN score makes the whole row NaN; keep the arithmetic finite and poison the row sum at the end
@@ -572,21 +580,22 @@ k_head_attention(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         settle(it, rescale, alpha);
         clear_tail(j);
         const float mneg = (m_used == -INFINITY) ? 0.f : -m_used * p.mult;
-        const uint64_t mn2 = splat2(mneg);
+        const uint64_t same2 = splat2(mneg);
+        auto less = [&](int c) -> uint64_t { return SLOPES ? splat2(mneg + lacking(c)) : same2; };
         uint64_t ps2[2] = {0ull, 0ull};
         {
           uint32_t pw[16];
-          exps(r[0], mn2, ps2, pw); store(0, pw);
-          exps(r[1], mn2, ps2, pw); store(1, pw);
+          exps(r[0], less(0), ps2, pw); store(0, pw);
+          exps(r[1], less(1), ps2, pw); store(1, pw);
         }
         publish();
         {
           // the second half: its first 32 keys are exponentiated while the first half multiplies
           uint32_t pw[16];
-          exps(r[2], mn2, ps2, pw);
+          exps(r[2], less(2), ps2, pw);
           wait(bar_pv, hc - 1, 19);
           store(0, pw);
-          exps(r[3], mn2, ps2, pw); store(1, pw);
+          exps(r[3], less(3), ps2, pw); store(1, pw);
         }
         publish();
         {

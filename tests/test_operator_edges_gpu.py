@@ -291,3 +291,20 @@ def test_f16_gradients_in_captured_graphs(lib):
             assert not status.item()
             for t, w in zip(grads[1:], want):
                 assert torch.isfinite(t).all() and torch.equal(t, w)
+
+
+# ---- a bias by distance far from every key --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_the_bias_far_from_every_key(client, causal):
+    """Queries 3000 to 3200 positions behind the last key, with slopes up to 1/2: biases around -1600, where f32 has a step of 1.2e-4.
+
+    The bias is rounded (half a step, in log2 units of 1.44 times the size: 1.2e-4), then once more with the score: 2.4e-4 log2 units of
+    the score, 1.7e-4 of the log sum and of a weight, against a bound of 2e-5 + 2e-6 * 1600 = 3.2e-3 and the f16 bound of o (F = 2e-4 and
+    a rounding); the log sum itself is compared at an eighth of that bound."""
+    q, k, v, do, extra, how = program.attention_case(1, 200, 300, 4, 2, 64, "f16", "bhsd", 5, slopes=True, causal=causal, query_offset=3300)
+    extra["slopes"] = torch.tensor([0.5, 0.25, 0.43, 0.06])
+    o, lse = program.attention_run(client, q, k, v, do, extra, how, "f16", "bhsd", gradient=False)
+    want = ref.attention(q, k, v, "f16", "bhsd", 0.125, **extra, **how)
+    program.within(o, *want["o"], "o")
+    program.within(lse, want["lse"][0], want["lse"][1] / 8, "lse")
