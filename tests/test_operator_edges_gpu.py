@@ -308,3 +308,27 @@ def test_the_bias_far_from_every_key(client, causal):
     want = ref.attention(q, k, v, "f16", "bhsd", 0.125, **extra, **how)
     program.within(o, *want["o"], "o")
     program.within(lse, want["lse"][0], want["lse"][1] / 8, "lse")
+
+
+# ---- norms of nothing ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [16, 17, 128])
+def test_a_head_of_zeros_without_epsilon_is_not_a_number_and_the_others_are(lib, D):
+    """Its root is 0: its own result and gradient are NaN, and so is the gradient of the weights, which it is part of; no other head's."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, dy = (torch.randn(2, 5, 3, D, generator=g, device="cuda") for _ in range(2))
+    x[1, 2, 1] = 0.0
+    w, dw = 1 + 0.1 * torch.randn(D, generator=g, device="cuda"), torch.empty(D, device="cuda")
+    y, dx, turns, R = torch.empty_like(x), torch.empty_like(x), direct.turns_of(D // 2 * 2), D // 2 * 2
+    assert lib.b2x_launch_rotary(C.byref(direct.rotary_args(lib, [x], [y], turns, weight=[w], R=R, epsilon=0.0)), None) == 0
+    a = direct.rotary_args(lib, [x], [dx], turns, dy=[dy], weight=[w], dweight=[dw], R=R, epsilon=0.0)
+    assert lib.b2x_launch_rotary_gradient(C.byref(a), None) == 0
+    torch.cuda.synchronize()
+    how = (torch.arange(3).expand(2, 3), w.cpu(), "f32", "bhsd", R, False, 0.0)
+    others = torch.ones(2, 5, 3, dtype=torch.bool)
+    others[1, 2, 1] = False
+    want, bound = ref.rotary(x.cpu(), *how)
+    direct.close(y[others.cuda()], want[others], bound[others], "y")
+    want, bound, _, _ = ref.rotary_gradient(dy.cpu(), x.cpu(), *how)
+    direct.close(dx[others.cuda()], want[others], bound[others], "dx")
+    assert torch.isnan(y[1, 2, 1]).all() and torch.isnan(dx[1, 2, 1]).all() and torch.isnan(dw).all()
