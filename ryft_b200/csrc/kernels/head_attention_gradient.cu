@@ -459,9 +459,12 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
     const uint32_t lane_addr = (uint32_t)(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)(g * 128);
     uint32_t uc = 0, mine = 0, nt = 0;            // units of all groups before this tile, this group's units, tiles with work
-    bool ok = true;
-    for (int n = 0; ok; n++) {
-      if (!ha_barrier_warp(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) { ok = false; break; }
+    // A wait inside a tile that runs out lets its lane go on with what is there: the lanes of a warp have to stay together for its
+    // votes and TMEM loads.  They leave as one in front of the next tile, which nobody publishes any more.  (Looking for it at the tile's
+    // end, or a vote behind every wait, cost 1.5 %.)
+    auto wait = [&](uint32_t bar, uint32_t parity, int code) { ha_barrier(bar, parity & 1, abort_flag, status, code); };
+    for (int n = 0;; n++) {
+      if (!ha_barrier_warp(bar_tf + 8 * (n & 1), (uint32_t)((n >> 1) & 1), abort_flag, status, 81)) break;
       volatile TileSlot* s = slots + (n & 1);
       const int t = s->tile, units = s->blocks, b = s->b, th = s->h, at = s->at;
       const HeadSequence seq{s->length, s->first, s->prefix};
@@ -510,7 +513,7 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         for (uint32_t first = ((uint32_t)g + GROUPS - uc % GROUPS) % GROUPS; k < (int)first && k < total; k++) advance();
         if (KEYS && k < total) ahead = fetch(hh, walk.j);
       }
-      while (k < total && ok) {
+      while (k < total) {
         const int unit = walk.j, head = KEYS ? th * p.a.group + hh : th;
         const uint32_t stage = (uc + (uint32_t)k) % STAGES;
         const bool compare = listed ? (s->compare[unit >> 5] >> (unit & 31)) & 1 : p.a.documents != nullptr;
@@ -523,8 +526,8 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         for (int i = 0; i < GROUPS && k < total; i++, k++) advance();
         if (KEYS && k < total) ahead = fetch(hh, walk.j);
         // the group's four warps have stored theirs (and read those of two units ago)
-        if (KEYS && !ha_barrier_warp(bar_rf + 8 * g, mine & 1, abort_flag, status, 84)) { ok = false; break; }
-        if (!ha_barrier_warp(bar_sf + 8 * g, mine & 1, abort_flag, status, 82)) { ok = false; break; }
+        if (KEYS) wait(bar_rf + 8 * g, mine, 84);
+        wait(bar_sf + 8 * g, mine, 82);
         tc_fence_after();
         const int u0 = unit * GRAD_UNIT;           // the unit's first key or query
         const float slope = p.a.slopes ? ld_global(p.a.slopes + head) * kLog2e : 0.f;
@@ -604,12 +607,11 @@ k_attention_gradient(const __grid_constant__ CUtensorMap tmT0, const __grid_cons
         if (lane == 0) mbar_arrive(bar_pf + 8 * g);
         mine++;
       }
-      if (!ok) break;
       uc += (uint32_t)total;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_te + 8 * (n & 1));   // the tile's list has been walked
       if (total > 0) {
-        if (!ha_barrier_warp(bar_end, nt & 1, abort_flag, status, 83)) { ok = false; break; }
+        wait(bar_end, nt, 83);
         tc_fence_after();
         nt++;
       }
@@ -667,6 +669,8 @@ __device__ __forceinline__ float rows_dot(const float (&a)[8], const float (&b)[
   for (int off = 8; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
   return d;
 }
+// Most warps find a larger value there and leave the address to the others.
+__device__ __forceinline__ void rows_raise(uint32_t* at, uint32_t most) { if (most > ld_global(at)) atomicMax(at, most); }
 template <int EL>
 __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ HeadAttn p, float* neg_lse, float* neg_delta, int32_t rows, float* row_size, uint32_t* head_size) {
   pdl_trigger();
@@ -691,7 +695,7 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
         most = max(most, __float_as_uint(rows_dot(f, f)));
       }
       most = __reduce_max_sync(0xffffffffu, most);
-      if (lane == 0 && most != 0) atomicMax(head_size + 2 * head + 1, most);
+      if (lane == 0) rows_raise(head_size + 2 * head + 1, most);
       return;
     }
   }
@@ -731,7 +735,7 @@ __global__ void __launch_bounds__(256) k_attention_rows(const __grid_constant__ 
   }
   if constexpr (EL == EL_F16) {
     most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0 && most != 0) atomicMax(head_size + 2 * ((uint32_t)b * (uint32_t)p.Hk + (uint32_t)(h / p.group)), most);
+    if (lane == 0) rows_raise(head_size + 2 * ((uint32_t)b * (uint32_t)p.Hk + (uint32_t)(h / p.group)), most);
   }
 }
 
