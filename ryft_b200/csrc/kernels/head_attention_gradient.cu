@@ -16,6 +16,10 @@
 // the products.  Accumulators and buffers fill TMEM at a width of 128.  Query heads that share a key head follow one another into the
 // same accumulators of dK and dV.
 //
+// Rounded to 16 bits on the way: P and dS as those operands, and O, which delta is taken from as the caller hands it in.  Against 64 bits
+// dq and dk are off by 2.6e-3 of their norm (bf16; 1.7e-3 is the rounding of the results alone), by up to 3.8e-3 where queries see a few
+// dozen keys and dS is a difference of near equals.
+//
 // The arithmetic of a unit is a loop over 16 columns whose body is one of nine forms (cap, bias, mask), chosen once per unit: with
 // the four steps unrolled, or with the forms' branches inside, the warps waited for instructions more than for anything else
 // (dK and dV of 2 x 16/4 heads, 4096 x 128, causal, capped: 505 us with branches inside, 416 unrolled, 336 as a loop).
@@ -25,7 +29,7 @@
 // 1259 for dK and dV.  At that size dQ takes 201 us, about 30 % above its products, and dK and dV 273 us, 50 % above: with two
 // pairs a unit's arithmetic is on the way from its scores to its sums.  Capped they take 242 and 313 us: the cap's polynomial and its
 // derivative double the instructions for the FMA pipe.  Both kernels and the row constants: 470 us, 731 TFLOP/s of the gradient's
-// five products; capped 548 us.
+// five products; capped 548 us; f16 17 us more, for the lengths of dO and V and the launches that no longer overlap.
 //
 // f16: P (dP - delta) passes f16's range at both ends where the gradients do not, so that it is rounded as a multiple of a power of
 // two that its size allows (grad_shift): |P (dP - delta)| = P |dO (V - O)| <= 2 |dO| max|V|, as lengths of rows, is brought below f16's

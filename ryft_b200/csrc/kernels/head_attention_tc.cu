@@ -3,9 +3,10 @@
 // A worker owns a tile at a time (drawn from a device-wide counter), walks its blocks of 128 keys with the running maximum and
 // sum of a softmax, normalises and writes its rows, and draws the next; while one worker starts or ends a tile the tensor and
 // special-function pipes work for the other.  384 threads: warps 0, 1 draw tiles and load (TMA), warps 2, 3 issue the MMAs,
-// warps 4-7 and 8-11 are the workers' softmax, one thread per query: its 128 scores are read from TMEM once and stay in
-// registers through cap, bias, mask, maximum and exponential.  Per worker Q, one K and one V stage, half a buffer of weights (the
-// second half's first keys are exponentiated while the first half multiplies), 128 score columns and the accumulator in TMEM.
+// warps 4-7 and 8-11 are the workers' softmax, one thread per query: its 128 scores are read from TMEM once and stay in registers
+// through bias, mask, maximum and exponential; capped scores without a bias are read twice, 32 at a time.  Per worker Q, one K and
+// one V stage, half a buffer of weights (the second half's first keys are exponentiated while the first half multiplies), 128 score
+// columns and the accumulator in TMEM.
 //
 // Where there are fewer tiles than workers a tile's walk is cut into parts (tile_parts), which a second launch joins.
 //
@@ -15,8 +16,11 @@
 // row's last key and, by ballots over the warp's distinct documents, from the document numbers.
 //
 // What bounds it: the softmax warps, two for each of the SM's four schedulers, whose instructions wait for one another more than
-// the tensor pipe (42 % busy) waits for operands.  2 x 16/8 heads, 4096 x 128, causal: 157 us, 877 TFLOP/s; with a cap or a bias by distance
-// 220 us.
+// the tensor pipe (42 % busy) waits for operands.  2 x 16/8 heads, 4096 x 128, causal: 150 us, 915 TFLOP/s; with a bias by
+// distance 216 us, with a cap 225, with both 276.
+//
+// Scores, maxima, sums and the accumulator are f32; the weights are rounded to the operands' 16 bits before they multiply V: o is off by
+// 2.1e-3 of its norm against 64 bits (bf16; 1.6e-3 is the rounding of the result alone).
 //
 // Rows of V behind a sequence's length are set to zero in shared memory before they meet their zero weights: a product of 0 and
 // what happens to lie there might be NaN.
@@ -57,7 +61,7 @@ template <int D> struct TileSmem {
 
 // What a kernel can do beside causal, prefix and length masks.  One kernel for everything left the warps of a plain problem waiting
 // for instructions and its registers spilled (2 x 16 heads of 4096 x 128, causal: 199 us where the
-// plain form takes 157).
+// plain form took 157).  What is left of that: TILE_ANY spills 8 to 11 registers, TILE_DOCUMENTS two.
 enum TileMode { TILE_PLAIN, TILE_CAP /* and documents */, TILE_DOCUMENTS, TILE_ANY /* a bias by distance, scales that are not positive */ };
 
 template <int D, int EL, int MODE>

@@ -1,14 +1,15 @@
 // Attention of a few queries per sequence (up to 16; one, where a model answers) against a long cache.
 //
-// Bound by HBM: keys and values are read once, 4 * rows flops for every 2 bytes of them.  The query heads that share a key head are
-// the rows of one tile of 16, so that a cache line serves all of them.  The keys of a sequence are cut into chunks, a CTA of four
+// Bound by HBM: keys and values are read once for every 16 rows, 4 * rows flops for every 2 bytes of them.  The queries of all heads that
+// share a key head are the rows of tiles of 16, so that a cache line serves 16 of them; 16 queries of 8 heads are 8 tiles, each of
+// which reads the cache for itself.  The keys of a sequence are cut into chunks, a CTA of four
 // warps each, whatever the batch: long sequences spread over the chip, chunks behind a short one's end leave at once.  A warp walks
 // steps of 16 keys through a ring of its own in shared memory, filled two steps ahead by asynchronous copies of 16 bytes (keys
 // behind the sequence's end are filled with zeros, so that nothing that lies there meets a product), and multiplies with m16n8k16
 // from there; no warp waits for another before the end.  (The 128-row tiles of tcgen05 would be empty but for a few rows; the
 // products here are a fifth of the time that the loads take.)  Straight into registers, with one step in flight, the loads
 // reached 3.2 TB/s: their latency showed, and 520 instructions per step went into placing them.  32 sequences with caches of
-// various lengths up to 8192, 32/8 heads of 128, capped: 92 us, 5.9 TB/s (6.5 where all lengths are 8192).
+// various lengths up to 8192, 32/8 heads of 128, capped: 93 us, 5.9 TB/s (6.5 where all lengths are 8192).
 //
 // Each warp keeps its own maximum (raised only when a score passes it by 2^8), sum and accumulator; the four meet in shared memory,
 // chunks in a second launch that weighs them by their maxima.  Order of sums: fixed.

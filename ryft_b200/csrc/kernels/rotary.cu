@@ -10,7 +10,8 @@
 // cosines and sines are computed once, a few per lane, shared through shared memory and then held in registers for all the
 // heads that it walks.  8192 tokens of 40 heads of 128 bf16 elements, with norms: 37 us, 4.5 TB/s (54 % of the issue slots: the norm's
 // and the turn's arithmetic in f32; without norms 33.5 us, 5.0 TB/s); the gradient of 16384 such tokens 115 us, 4.4 TB/s.  Each layout
-// of pairs is a kernel of its own: with both in one, 38 and 118 us.
+// of pairs is a kernel of its own: with both in one, 38 and 118 us.  The gradient's instance for 16-byte pieces of bf16 spills 6
+// registers, that of f16 13, at the 128 that two CTAs per SM leave.
 //
 // Angles: a position times a frequency in f32 is off by whole turns far into a context.  Frequencies are therefore turns per
 // position as fractions of 2^64, computed in extended precision where the program is compiled; the product with the position
