@@ -235,14 +235,15 @@ inline PFN_encodeTiled find_encode_tiled() {
   }();
   return fn;
 }
-// The driver wants a current context, which a thread has only once the runtime has worked on its device: where it answers with an
-// error the device is set and it is asked once more.
+// The driver wants a current context, which a thread has only once the runtime has worked on its device: where there is none the
+// device is set and it is asked once more.
 inline PFN_encodeTiled get_encode_tiled() {
   if (!find_encode_tiled()) return nullptr;
   return [](auto... args) -> CUresult {
     CUresult r = find_encode_tiled()(args...);
     int dev = 0;
-    if (r != CUDA_SUCCESS && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = find_encode_tiled()(args...);
+    if ((r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+      r = find_encode_tiled()(args...);
     return r;
   };
 }
