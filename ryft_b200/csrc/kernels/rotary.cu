@@ -505,7 +505,8 @@ bool rot_valid(const B2xRotaryArgs* a, bool gradient) {
   bool any = false;
   for (int i = 0; i < a->n; i++) {
     if (a->heads[i] < 0 || a->heads[i] >= (1 << 20)) return false;
-    if (a->D > 0 && a->norm && (!at(a->weight[i], a->weight_elem == EL_F32 ? 4 : 2) || (gradient && !at(a->dweight[i], 4)))) return false;
+    if (a->D > 0 && a->norm && gradient && !at(a->dweight[i], 4)) return false;
+    if (a->B * a->S * a->D > 0 && a->norm && !at(a->weight[i], a->weight_elem == EL_F32 ? 4 : 2)) return false;
     if (a->B * a->S * a->heads[i] * a->D == 0) continue;
     any = true;
     if (!at(a->y[i], es) || ((!gradient || a->norm) && !at(a->x[i], es)) || (gradient && !at(a->dy[i], es))) return false;

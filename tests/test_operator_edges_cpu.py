@@ -140,5 +140,5 @@ def test_rotary_without_its_memory_is_refused(gradient, change, elem):
 
 def test_rotary_of_nothing_needs_no_memory():
     lib = kernels.load()
-    for change in (dict(D=0, R=0), dict(B=0, x=(0, None), turns=None)):
+    for change in (dict(D=0, R=0), dict(B=0, x=(0, None), turns=None), dict(S=0, weight=(1, None))):
         assert lib.b2x_launch_rotary(ctypes.byref(rotary_call(kernels.EL_BF16, **change)), None) == 0
