@@ -142,3 +142,18 @@ def test_rotary_of_nothing_needs_no_memory():
     lib = kernels.load()
     for change in (dict(D=0, R=0), dict(B=0, x=(0, None), turns=None), dict(S=0, weight=(1, None))):
         assert lib.b2x_launch_rotary(ctypes.byref(rotary_call(kernels.EL_BF16, **change)), None) == 0
+
+
+# ---- scratch of f16 gradients -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("B,Hq,Hk,Sq,Sk,D,parts", [(4, 8, 4, 1500, 1500, 64, 0), (1, 2, 1, 1300, 1300, 128, 4 * 2 * 1 * 1408 * 128 * 4), (1, 0, 3, 200, 200, 64, 0), (1, 4, 2, 0, 200, 64, 0),
+                                                   (0, 4, 2, 10, 10, 64, 0)])
+def test_f16_gradients_have_room_for_the_sizes_of_their_rows(B, Hq, Hk, Sq, Sk, D, parts):
+    """Beside the row constants (8 bytes a row) a squared length for each row and two for each key head; parts' sums start on 16 bytes."""
+    lib = kernels.load()
+    rows = -(-Sq // 128) * 128
+    of = lambda elem: lib.b2x_head_attention_scratch_bytes(ctypes.byref(kernels.HeadAttentionArgs(  # noqa: E731
+        elem=elem, causal=1, B=B, Hq=Hq, Hk=Hk, Sq=Sq, Sk=Sk, D=D)), 1)
+    assert of(kernels.EL_BF16) == B * Hq * rows * 8 + parts
+    head = B * Hq * rows * 12 + B * Hk * 8
+    assert of(kernels.EL_F16) == (-(-head // 16) * 16 + parts if parts else head)

@@ -332,3 +332,33 @@ def test_a_head_of_zeros_without_epsilon_is_not_a_number_and_the_others_are(lib,
     want, bound, _, _ = ref.rotary_gradient(dy.cpu(), x.cpu(), *how)
     direct.close(dx[others.cuda()], want[others], bound[others], "dx")
     assert torch.isnan(y[1, 2, 1]).all() and torch.isnan(dx[1, 2, 1]).all() and torch.isnan(dw).all()
+
+
+# ---- memory that a program is handed ------------------------------------------------------------------------------------------------
+
+def test_views_off_their_boundary_are_refused_and_the_program_goes_on(client):
+    """Rows of attention start on 16 bytes, values on their own size; a view that does not is an error of its execution, not a fault."""
+    from ryft_b200.stablehlo import Builder
+
+    def program_of(make):
+        b = Builder()
+        return client.compile(pjrt.Program.mlir(b.build(*make(b))))
+    T = [1, 2, 40, 64]
+    attention = program_of(lambda b: [b.attention(*[b.arg(T, "bf16") for _ in range(3)])])
+    rotary = program_of(lambda b: b.rotary([b.arg(T, "bf16")]))
+    memory = torch.randn(3, 2 * 40 * 64 + 64, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+
+    def run(exe, n, off):
+        bufs = [client.view_of_device_buffer(memory[i].data_ptr() + off, pjrt.BufferType.BF16, T, keep=memory) for i in range(n)]
+        return program.collect(exe.execute([pjrt.ExecutionDeviceInputs(bufs)])[0])
+    whole = run(attention, 3, 0)[0]
+    for off in (2, 8):
+        with pytest.raises(pjrt.PjrtError):
+            run(attention, 3, off)
+    with pytest.raises(pjrt.PjrtError):
+        run(rotary, 1, 1)
+    turned = run(rotary, 1, 2)[0]
+    x = memory[0, 1:1 + 2 * 40 * 64].cpu().reshape(T)
+    program.within(turned, *ref.rotary(x, torch.arange(40).expand(1, 40), None, "bf16", "bhsd", 64, False, 0.0), "y")
+    assert torch.equal(run(attention, 3, 0)[0], whole)
